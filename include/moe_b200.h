@@ -312,6 +312,59 @@ int moe_b200_norm_router(int32_t dtype, int64_t num_rows, int64_t hidden_size,
                          const float* gamma, float epsilon, const void* router_weight,
                          void* residual_out, void* normed, void* router_logits, void* stream);
 
+/* ------------------------------------------------ expert products, adapters */
+
+/* The layer's matrix products as operators of their own, for callers that compose a layer
+ * (its activation, a trained expert, a gradient) from the stages above: rows in expert
+ * order, as moe_b200_permute plans them.  expert_offsets int32 [E+1] on the device, non-
+ * decreasing: expert e has rows [expert_offsets[e], expert_offsets[e+1]), which may be
+ * none; rows from expert_offsets[E] on are neither read nor written.  (Offsets outside
+ * [0, num_rows] are clamped to it.)  weights [E, n, k], k contiguous; float, float16 or
+ * bfloat16 throughout, sums in fp32.  1 <= n, k <= 2^20; E <= 256.  Buffers need the
+ * alignment of their elements; 16-bit types with n and k multiples of 8 and 16-byte
+ * aligned buffers run on the tensor cores.  Outputs must not overlap inputs.  No host
+ * synchronisation, no allocation; results are the same bits on every call.
+ * Analog of the reference's batched product (musa/ep/src/kernels/math/matmul.cc:239-332,
+ * shared_inc/blas_utils.h:237-262), which takes equal sizes only. */
+
+/* y[p] = weights[e] x[p]:  x [num_rows, k], y [num_rows, n]. */
+int moe_b200_grouped_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
+                            int64_t num_experts, const void* x, const void* weights,
+                            const int32_t* expert_offsets, void* y, void* stream);
+/* Gradient with respect to x, dx[p] = weights[e]^T dy[p]:  dy [num_rows, n],
+ * dx [num_rows, k]. */
+int moe_b200_grouped_matmul_grad_input(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
+                                       int64_t num_experts, const void* dy, const void* weights,
+                                       const int32_t* expert_offsets, void* dx, void* stream);
+/* Gradient with respect to the weights, dw[e] = sum over the rows p of e of dy[p] x[p]^T,
+ * [E, n, k]; an expert without rows gets zeros.  `workspace`: 256-byte aligned, at least
+ * moe_b200_grouped_matmul_grad_weight_workspace_size bytes (NULL if that is 0). */
+int moe_b200_grouped_matmul_grad_weight_workspace_size(int32_t dtype, int64_t n, int64_t k,
+                                                       int64_t num_experts, size_t* bytes);
+int moe_b200_grouped_matmul_grad_weight(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
+                                        int64_t num_experts, const void* x, const void* dy,
+                                        const int32_t* expert_offsets, void* dw, void* workspace,
+                                        size_t workspace_bytes, void* stream);
+
+/* A projection shared by all rows plus the low-rank adapter of each row's request:
+ *   y[t] = weight x[t] + scales[a] * lora_b[a] (lora_a[a] x[t]),  a = adapter_ids[t],
+ * and y[t] = weight x[t] for an id outside [0, num_adapters) (-1: no adapter).
+ * x [num_rows, k], weight [n, k], lora_a [L, rank, k], lora_b [L, n, rank], adapter_ids
+ * int32 [num_rows], scales fp32 [L], y [num_rows, n]; 1 <= rank <= 256, an adapter of
+ * smaller rank is padded with zeros.  Rows may follow any adapters in any order; a row is
+ * touched by its own adapter only (an infinity or NaN in another one does not reach it).
+ * The rank-sized intermediate is kept in fp32.  Types, sizes and alignment as above (rank
+ * a multiple of 8 for the tensor cores).  `workspace`: 256-byte aligned, at least
+ * moe_b200_lora_matmul_workspace_size bytes, not shared by calls that may overlap.
+ * No counterpart in the reference. */
+int moe_b200_lora_matmul_workspace_size(int32_t dtype, int64_t num_rows, int64_t rank,
+                                        size_t* bytes);
+int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
+                         int64_t num_adapters, int64_t rank, const void* x, const void* weight,
+                         const void* lora_a, const void* lora_b, const int32_t* adapter_ids,
+                         const float* scales, void* y, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
 /* --------------------------------------- device-side expert parallelism (P2P) */
 
 /* Expert-parallel layer over the GPUs of one node with no host synchronisation and no

@@ -154,6 +154,18 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "moe_b200_route_noalloc": (ctypes.c_int, [_VP, _I32, _I64, _I64, _I32, _I32, _VP, _VP, _VP]),
     "moe_b200_permute_workspace_size": (_SZ, [_I64, _I32, _I64]),
     "moe_b200_permute": (ctypes.c_int, [_VP, _I64, _I32, _I64, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "moe_b200_grouped_matmul": (ctypes.c_int, [_I32, _I64, _I64, _I64, _I64, _VP, _VP, _VP, _VP,
+                                               _VP]),
+    "moe_b200_grouped_matmul_grad_input": (ctypes.c_int, [_I32, _I64, _I64, _I64, _I64, _VP, _VP,
+                                                          _VP, _VP, _VP]),
+    "moe_b200_grouped_matmul_grad_weight_workspace_size": (
+        ctypes.c_int, [_I32, _I64, _I64, _I64, ctypes.POINTER(_SZ)]),
+    "moe_b200_grouped_matmul_grad_weight": (ctypes.c_int, [_I32, _I64, _I64, _I64, _I64, _VP, _VP,
+                                                           _VP, _VP, _VP, _SZ, _VP]),
+    "moe_b200_lora_matmul_workspace_size": (ctypes.c_int, [_I32, _I64, _I64,
+                                                           ctypes.POINTER(_SZ)]),
+    "moe_b200_lora_matmul": (ctypes.c_int, [_I32, _I64, _I64, _I64, _I64, _I64, _VP, _VP, _VP, _VP,
+                                            _VP, _VP, _VP, _VP, _SZ, _VP]),
     "moe_b200_prepack_create": (ctypes.c_int, [ctypes.POINTER(Problem), ctypes.POINTER(Tensors),
                                                _I32, _VP, ctypes.POINTER(_VP)]),
     "moe_b200_prepack_info": (ctypes.c_int, [_VP, ctypes.POINTER(_SZ), _PI32]),
@@ -751,3 +763,174 @@ def permute(expert_idx, num_experts: int, stream=None):
                                  pos.data_ptr(), src.data_ptr(), ws.data_ptr(), nbytes,
                                  _stream_handle(stream)))
     return offsets, pos, src
+
+
+# ------------------------------------------------------- expert products, adapters
+
+def _operands(what: str, like, named, out, out_shape):
+    """Checks of the operators below: contiguous CUDA tensors of one device, the dtype of
+    the first (or the one named) and the expected shape.  ``named``: (name, tensor, shape,
+    dtype or None) with -1 for a free dimension; ``out`` None or a tensor of
+    ``out_shape``."""
+    dev, dt = like.device, like.dtype
+    if not like.is_cuda:
+        raise ValueError(f"{what}: tensors must be contiguous CUDA tensors")
+    if out is not None:
+        named = (*named, ("out", out, out_shape, None))
+    for name, t, shape, want in named:
+        if t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be a contiguous tensor on {dev}")
+        if t.dtype != (want or dt):
+            raise TypeError(f"{what}: {name} must be {want or dt}, not {t.dtype}")
+        if t.dim() != len(shape) or any(w >= 0 and w != d for w, d in zip(shape, t.shape)):
+            raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected "
+                             f"{tuple('*' if w < 0 else w for w in shape)}")
+
+
+class _On:
+    """Runs an operator on ``stream`` (None: the current stream of the tensors' device) of
+    the tensors' device: outputs and workspaces come from that stream's allocator pool, and
+    inputs used on a stream other than the current one are marked as in use there."""
+
+    __slots__ = ("handle", "_dev", "_ctx")
+
+    def __init__(self, stream, tensors):
+        torch = _torch()
+        dev = tensors[0].device
+        self._dev = self._ctx = None
+        if dev.index != torch.cuda.current_device():
+            self._dev = torch.cuda.device(dev)
+            self._dev.__enter__()
+        if stream is None:
+            self.handle = torch.cuda.current_stream(dev).cuda_stream
+            return
+        if isinstance(stream, int):
+            stream = torch.cuda.ExternalStream(stream, device=dev) if stream else \
+                torch.cuda.default_stream(dev)
+        self.handle = stream.cuda_stream
+        if self.handle != torch.cuda.current_stream(dev).cuda_stream:
+            for t in tensors:
+                if t is not None:
+                    t.record_stream(stream)
+            self._ctx = torch.cuda.stream(stream)
+            self._ctx.__enter__()
+
+    def __enter__(self):
+        return self.handle
+
+    def __exit__(self, *exc):
+        if self._ctx is not None:
+            self._ctx.__exit__(*exc)
+        if self._dev is not None:
+            self._dev.__exit__(*exc)
+
+
+def _rank2(what: str, name: str, t) -> tuple[int, int]:
+    if t.dim() != 2:
+        raise ValueError(f"{what}: {name} must have 2 dimensions, not {t.dim()}")
+    return t.shape
+
+
+def _rank3(what: str, name: str, t) -> tuple[int, int, int]:
+    if t.dim() != 3:
+        raise ValueError(f"{what}: {name} must have 3 dimensions, not {t.dim()}")
+    return t.shape
+
+
+def grouped_matmul(x, weights, expert_offsets, out=None, stream=None):
+    """Matrix products grouped by expert: ``y[p] = weights[e] @ x[p]`` for the rows
+    ``expert_offsets[e] <= p < expert_offsets[e + 1]`` of each expert.
+
+    ``x`` [R, K] in expert order (:func:`permute`, :func:`ep_dispatch`), ``weights``
+    [E, N, K], ``expert_offsets`` int32 [E + 1] on the device; returns [R, N] (``out`` if
+    given).  Rows from ``expert_offsets[E]`` on are neither read nor written.  float32,
+    float16 or bfloat16, fp32 sums."""
+    torch = _torch()
+    R, K = _rank2("grouped_matmul", "x", x)
+    E, N, _ = _rank3("grouped_matmul", "weights", weights)
+    _operands("grouped_matmul", x, (
+        ("x", x, (R, K), None), ("weights", weights, (E, N, K), None),
+        ("expert_offsets", expert_offsets, (E + 1,), torch.int32)), out, (R, N))
+    with _On(stream, (x, weights, expert_offsets, out)) as s:
+        if out is None:
+            out = torch.empty((R, N), dtype=x.dtype, device=x.device)
+        check(lib().moe_b200_grouped_matmul(
+            elem_type_of(x), R, N, K, E, x.data_ptr(), weights.data_ptr(),
+            expert_offsets.data_ptr(), out.data_ptr(), s))
+    return out
+
+
+def grouped_matmul_grad_input(dy, weights, expert_offsets, out=None, stream=None):
+    """Gradient of :func:`grouped_matmul` with respect to ``x``:
+    ``dx[p] = weights[e].T @ dy[p]``; ``dy`` [R, N], returns [R, K]."""
+    torch = _torch()
+    R, N = _rank2("grouped_matmul_grad_input", "dy", dy)
+    E, _, K = _rank3("grouped_matmul_grad_input", "weights", weights)
+    _operands("grouped_matmul_grad_input", dy, (
+        ("dy", dy, (R, N), None), ("weights", weights, (E, N, K), None),
+        ("expert_offsets", expert_offsets, (E + 1,), torch.int32)), out, (R, K))
+    with _On(stream, (dy, weights, expert_offsets, out)) as s:
+        if out is None:
+            out = torch.empty((R, K), dtype=dy.dtype, device=dy.device)
+        check(lib().moe_b200_grouped_matmul_grad_input(
+            elem_type_of(dy), R, N, K, E, dy.data_ptr(), weights.data_ptr(),
+            expert_offsets.data_ptr(), out.data_ptr(), s))
+    return out
+
+
+def grouped_matmul_grad_weight(x, dy, expert_offsets, out=None, stream=None):
+    """Gradient of :func:`grouped_matmul` with respect to the weights:
+    ``dw[e] = sum_p outer(dy[p], x[p])`` over the rows of expert e (zeros if it has none);
+    ``x`` [R, K], ``dy`` [R, N], returns [E, N, K]."""
+    torch = _torch()
+    R, K = _rank2("grouped_matmul_grad_weight", "x", x)
+    _, N = _rank2("grouped_matmul_grad_weight", "dy", dy)
+    if expert_offsets.dim() != 1 or expert_offsets.shape[0] < 2:
+        raise ValueError("grouped_matmul_grad_weight: expert_offsets must have E + 1 >= 2 entries")
+    E = expert_offsets.shape[0] - 1
+    _operands("grouped_matmul_grad_weight", x, (
+        ("x", x, (R, K), None), ("dy", dy, (R, N), None),
+        ("expert_offsets", expert_offsets, (E + 1,), torch.int32)), out, (E, N, K))
+    dt = elem_type_of(x)
+    nbytes = _SZ()
+    check(lib().moe_b200_grouped_matmul_grad_weight_workspace_size(dt, N, K, E,
+                                                                   ctypes.byref(nbytes)))
+    with _On(stream, (x, dy, expert_offsets, out)) as s:
+        if out is None:
+            out = torch.empty((E, N, K), dtype=x.dtype, device=x.device)
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=x.device)
+        check(lib().moe_b200_grouped_matmul_grad_weight(
+            dt, R, N, K, E, x.data_ptr(), dy.data_ptr(), expert_offsets.data_ptr(),
+            out.data_ptr(), ws.data_ptr(), nbytes.value, s))
+    return out
+
+
+def lora_matmul(x, weight, lora_a, lora_b, adapter_ids, scales, out=None, stream=None):
+    """A projection shared by all rows plus each row's own low-rank adapter:
+    ``y[t] = weight @ x[t] + scales[a] * lora_b[a] @ (lora_a[a] @ x[t])`` with
+    ``a = adapter_ids[t]``; an id outside [0, L) (-1) means no adapter.
+
+    ``x`` [T, K], ``weight`` [N, K], ``lora_a`` [L, r, K], ``lora_b`` [L, N, r] (adapters of
+    smaller rank padded with zeros), ``adapter_ids`` int32 [T], ``scales`` float32 [L];
+    returns [T, N].  float32, float16 or bfloat16; the intermediate stays in fp32."""
+    torch = _torch()
+    T, K = _rank2("lora_matmul", "x", x)
+    N, _ = _rank2("lora_matmul", "weight", weight)
+    L, r, _ = _rank3("lora_matmul", "lora_a", lora_a)
+    _operands("lora_matmul", x, (
+        ("x", x, (T, K), None), ("weight", weight, (N, K), None),
+        ("lora_a", lora_a, (L, r, K), None), ("lora_b", lora_b, (L, N, r), None),
+        ("adapter_ids", adapter_ids, (T,), torch.int32),
+        ("scales", scales, (L,), torch.float32)), out, (T, N))
+    dt = elem_type_of(x)
+    nbytes = _SZ()
+    check(lib().moe_b200_lora_matmul_workspace_size(dt, T, r, ctypes.byref(nbytes)))
+    with _On(stream, (x, weight, lora_a, lora_b, adapter_ids, scales, out)) as s:
+        if out is None:
+            out = torch.empty((T, N), dtype=x.dtype, device=x.device)
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=x.device)
+        check(lib().moe_b200_lora_matmul(
+            dt, T, N, K, L, r, x.data_ptr(), weight.data_ptr(), lora_a.data_ptr(),
+            lora_b.data_ptr(), adapter_ids.data_ptr(), scales.data_ptr(), out.data_ptr(),
+            ws.data_ptr(), nbytes.value, s))
+    return out

@@ -1,0 +1,63 @@
+// Internal launch interface of the expert products (grouped_matmul and its gradients) and
+// of the adapter projection (lora_matmul).  Not part of the public C ABI.
+#pragma once
+
+#include "moe_kernels.h"
+
+namespace moe {
+
+// Which of the three products of y[p] = W[e(p)] x[p] is formed.  `feat` is the output
+// feature side, `con` the contraction; W is [E, N, K].
+enum GroupedDir : int {
+  kGmmForward = 0,     // y  [R, N]    = x [R, K] W[e]^T          feat = N, con = K
+  kGmmGradInput = 1,   // dx [R, K]    = dy [R, N] W[e]           feat = K, con = N
+  kGmmGradWeight = 2,  // dW [E, N, K] = dy_e^T x_e               con = the rows of e
+};
+
+struct GroupedArgs {
+  int dtype;
+  GroupedDir dir;
+  int64_t rows;            // R
+  int N, K, E;
+  const void* x;           // [R, K]   (forward, grad_weight)
+  const void* dy;          // [R, N]   (grad_input, grad_weight)
+  const void* w;           // [E, N, K] (forward, grad_input)
+  const int32_t* offsets;  // [E + 1]; nullptr: one group of all rows (E = 1)
+  void* out;
+  void* workspace = nullptr;  // grad_weight on tensor cores: padded row tails
+};
+
+// The adapter term of lora_matmul, added to the forward product of one group.
+struct LoraTerm {
+  const float* t;         // [splits][rows][rank]: partial sums of A_a x over K
+  int splits;
+  int rank;               // r
+  int adapters;           // L
+  const void* b;          // [L, N, r]
+  const int32_t* ids;     // [rows]; outside [0, L): no adapter
+  const float* scales;    // [L]
+};
+
+// Largest feature and contraction length, and most rows, of a call (index arithmetic of
+// the kernels: tile numbers and TMA coordinates in 32 bits, offsets in 64).
+constexpr int64_t kGmmMaxDim = 1 << 20;
+constexpr int64_t kGmmMaxRows = 1 << 30;
+constexpr int kLoraMaxRank = 256;
+
+// t[row, j] = sum_k A_a[j, k] x[row, k] for rows with an adapter a (others are left).
+struct LoraShrink {
+  int dtype;
+  int64_t rows;
+  int K, rank, adapters;
+  const void* x;           // [rows, K]
+  const void* a;           // [L, r, K]
+  const int32_t* ids;
+  float* t;                // [splits][rows][rank]
+  int splits;
+};
+cudaError_t launch_lora_shrink_simt(const LoraShrink& l, cudaStream_t s);  // splits = 1
+
+// FFMA kernels: any size, alignment and float type.
+cudaError_t launch_grouped_simt(const GroupedArgs& g, const LoraTerm* lora, cudaStream_t s);
+
+}  // namespace moe

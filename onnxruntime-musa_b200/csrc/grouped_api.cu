@@ -1,0 +1,239 @@
+// C entries of the expert products (moe_b200_grouped_matmul*) and the adapter projection
+// (moe_b200_lora_matmul): argument checks and the choice of kernel.
+#include "../../include/moe_b200.h"
+#include "grouped.h"
+
+namespace {
+
+using moe::set_error;
+
+bool float_type(int32_t dt) {
+  return dt == moe::kDtF32 || dt == moe::kDtF16 || dt == moe::kDtBF16;
+}
+
+int cuda_status(cudaError_t st, const char* what) {
+  if (st == cudaSuccess) return MOE_B200_OK;
+  return set_error(MOE_B200_EP_FAIL, "%s: %s", what, cudaGetErrorString(st));
+}
+
+int check_shape(const char* what, int32_t dtype, int64_t rows, int64_t n, int64_t k,
+                int64_t groups, const char* group_name, int64_t max_groups) {
+  if (!float_type(dtype))
+    return set_error(MOE_B200_NOT_IMPLEMENTED, "%s: unsupported dtype %d", what, dtype);
+  if (rows < 0 || rows > moe::kGmmMaxRows)
+    return set_error(MOE_B200_INVALID_ARGUMENT, "%s: num_rows=%lld must be in [0, %lld]", what,
+                     static_cast<long long>(rows), static_cast<long long>(moe::kGmmMaxRows));
+  if (n < 1 || n > moe::kGmmMaxDim || k < 1 || k > moe::kGmmMaxDim)
+    return set_error(MOE_B200_INVALID_ARGUMENT, "%s: n=%lld and k=%lld must be in [1, %lld]", what,
+                     static_cast<long long>(n), static_cast<long long>(k),
+                     static_cast<long long>(moe::kGmmMaxDim));
+  if (groups < 1 || groups > max_groups)
+    return set_error(MOE_B200_INVALID_ARGUMENT, "%s: %s=%lld must be in [1, %lld]", what,
+                     group_name, static_cast<long long>(groups),
+                     static_cast<long long>(max_groups));
+  return MOE_B200_OK;
+}
+
+// Every buffer must be aligned to its element size (the kernels pick wider loads by the
+// alignment they find).
+int check_pointers(const char* what, int32_t dtype, const void* const* ptrs, int n,
+                   const void* const* words, int nw) {
+  const uintptr_t es = static_cast<uintptr_t>(moe::dtype_bytes(dtype));
+  for (int i = 0; i < n + nw; ++i) {
+    const void* q = i < n ? ptrs[i] : words[i - n];
+    if (q == nullptr)
+      return set_error(MOE_B200_INVALID_ARGUMENT, "%s: buffers must be non-NULL", what);
+    if (reinterpret_cast<uintptr_t>(q) % (i < n ? es : 4) != 0)
+      return set_error(MOE_B200_INVALID_ARGUMENT,
+                       "%s: buffers must be aligned to their element size", what);
+  }
+  return MOE_B200_OK;
+}
+
+int run_grouped(const char* what, moe::GroupedArgs& g, cudaStream_t s) {
+  return cuda_status(moe::launch_grouped_simt(g, nullptr, s), what);
+}
+
+size_t lora_bytes(int64_t rows, int64_t rank) {
+  return static_cast<size_t>(rows) * static_cast<size_t>(rank) * sizeof(float);
+}
+
+}  // namespace
+
+extern "C" {
+
+int moe_b200_grouped_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
+                            int64_t num_experts, const void* x, const void* weights,
+                            const int32_t* expert_offsets, void* y, void* stream) {
+  static const char* kWhat = "grouped_matmul";
+  moe::clear_stale_cuda_error();
+  int rc = check_shape(kWhat, dtype, num_rows, n, k, num_experts, "num_experts", moe::kMaxExperts);
+  if (rc != MOE_B200_OK || num_rows == 0) return rc;
+  const void* ptrs[] = {x, weights, y};
+  const void* words[] = {expert_offsets};
+  rc = check_pointers(kWhat, dtype, ptrs, 3, words, 1);
+  if (rc != MOE_B200_OK) return rc;
+  moe::GroupedArgs g{};
+  g.dtype = dtype;
+  g.dir = moe::kGmmForward;
+  g.rows = num_rows;
+  g.N = static_cast<int>(n);
+  g.K = static_cast<int>(k);
+  g.E = static_cast<int>(num_experts);
+  g.x = x;
+  g.w = weights;
+  g.offsets = expert_offsets;
+  g.out = y;
+  return run_grouped(kWhat, g, static_cast<cudaStream_t>(stream));
+}
+
+int moe_b200_grouped_matmul_grad_input(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
+                                       int64_t num_experts, const void* dy, const void* weights,
+                                       const int32_t* expert_offsets, void* dx, void* stream) {
+  static const char* kWhat = "grouped_matmul_grad_input";
+  moe::clear_stale_cuda_error();
+  int rc = check_shape(kWhat, dtype, num_rows, n, k, num_experts, "num_experts", moe::kMaxExperts);
+  if (rc != MOE_B200_OK || num_rows == 0) return rc;
+  const void* ptrs[] = {dy, weights, dx};
+  const void* words[] = {expert_offsets};
+  rc = check_pointers(kWhat, dtype, ptrs, 3, words, 1);
+  if (rc != MOE_B200_OK) return rc;
+  moe::GroupedArgs g{};
+  g.dtype = dtype;
+  g.dir = moe::kGmmGradInput;
+  g.rows = num_rows;
+  g.N = static_cast<int>(n);
+  g.K = static_cast<int>(k);
+  g.E = static_cast<int>(num_experts);
+  g.dy = dy;
+  g.w = weights;
+  g.offsets = expert_offsets;
+  g.out = dx;
+  return run_grouped(kWhat, g, static_cast<cudaStream_t>(stream));
+}
+
+int moe_b200_grouped_matmul_grad_weight_workspace_size(int32_t dtype, int64_t n, int64_t k,
+                                                       int64_t num_experts, size_t* bytes) {
+  static const char* kWhat = "grouped_matmul_grad_weight_workspace_size";
+  int rc = check_shape(kWhat, dtype, 0, n, k, num_experts, "num_experts", moe::kMaxExperts);
+  if (rc != MOE_B200_OK) return rc;
+  if (bytes == nullptr)
+    return set_error(MOE_B200_INVALID_ARGUMENT, "%s: bytes must be non-NULL", kWhat);
+  *bytes = 0;
+  return MOE_B200_OK;
+}
+
+int moe_b200_grouped_matmul_grad_weight(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
+                                        int64_t num_experts, const void* x, const void* dy,
+                                        const int32_t* expert_offsets, void* dw, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+  static const char* kWhat = "grouped_matmul_grad_weight";
+  moe::clear_stale_cuda_error();
+  int rc = check_shape(kWhat, dtype, num_rows, n, k, num_experts, "num_experts", moe::kMaxExperts);
+  if (rc != MOE_B200_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (num_rows == 0) {  // no rows: every expert's gradient is zero
+    const void* out[] = {dw};
+    rc = check_pointers(kWhat, dtype, out, 1, nullptr, 0);
+    if (rc != MOE_B200_OK) return rc;
+    return cuda_status(cudaMemsetAsync(dw, 0,
+                                       static_cast<size_t>(num_experts) * n * k *
+                                           moe::dtype_bytes(dtype), s),
+                       kWhat);
+  }
+  const void* ptrs[] = {x, dy, dw};
+  const void* words[] = {expert_offsets};
+  rc = check_pointers(kWhat, dtype, ptrs, 3, words, 1);
+  if (rc != MOE_B200_OK) return rc;
+  size_t need = 0;
+  rc = moe_b200_grouped_matmul_grad_weight_workspace_size(dtype, n, k, num_experts, &need);
+  if (rc != MOE_B200_OK) return rc;
+  if (workspace_bytes < need || (need > 0 && (workspace == nullptr ||
+                                              reinterpret_cast<uintptr_t>(workspace) % 256 != 0)))
+    return set_error(MOE_B200_INVALID_ARGUMENT,
+                     "%s: workspace must be 256-byte aligned and hold %zu bytes", kWhat, need);
+  moe::GroupedArgs g{};
+  g.dtype = dtype;
+  g.dir = moe::kGmmGradWeight;
+  g.rows = num_rows;
+  g.N = static_cast<int>(n);
+  g.K = static_cast<int>(k);
+  g.E = static_cast<int>(num_experts);
+  g.x = x;
+  g.dy = dy;
+  g.offsets = expert_offsets;
+  g.out = dw;
+  g.workspace = workspace;
+  return run_grouped(kWhat, g, s);
+}
+
+int moe_b200_lora_matmul_workspace_size(int32_t dtype, int64_t num_rows, int64_t rank,
+                                        size_t* bytes) {
+  static const char* kWhat = "lora_matmul_workspace_size";
+  int rc = check_shape(kWhat, dtype, num_rows, 1, 1, rank, "rank", moe::kLoraMaxRank);
+  if (rc != MOE_B200_OK) return rc;
+  if (bytes == nullptr)
+    return set_error(MOE_B200_INVALID_ARGUMENT, "%s: bytes must be non-NULL", kWhat);
+  *bytes = lora_bytes(num_rows, rank);
+  return MOE_B200_OK;
+}
+
+int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
+                         int64_t num_adapters, int64_t rank, const void* x, const void* weight,
+                         const void* lora_a, const void* lora_b, const int32_t* adapter_ids,
+                         const float* scales, void* y, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+  static const char* kWhat = "lora_matmul";
+  moe::clear_stale_cuda_error();
+  int rc = check_shape(kWhat, dtype, num_rows, n, k, num_adapters, "num_adapters",
+                       moe::kGmmMaxDim);
+  if (rc != MOE_B200_OK) return rc;
+  if (rank < 1 || rank > moe::kLoraMaxRank)
+    return set_error(MOE_B200_INVALID_ARGUMENT, "%s: rank=%lld must be in [1, %d]", kWhat,
+                     static_cast<long long>(rank), moe::kLoraMaxRank);
+  if (num_rows == 0) return MOE_B200_OK;
+  const void* ptrs[] = {x, weight, lora_a, lora_b, y};
+  const void* words[] = {adapter_ids, scales};
+  rc = check_pointers(kWhat, dtype, ptrs, 5, words, 2);
+  if (rc != MOE_B200_OK) return rc;
+  const size_t need = lora_bytes(num_rows, rank);
+  if (workspace_bytes < need || workspace == nullptr ||
+      reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
+    return set_error(MOE_B200_INVALID_ARGUMENT,
+                     "%s: workspace must be 256-byte aligned and hold %zu bytes", kWhat, need);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  moe::LoraShrink l{};
+  l.dtype = dtype;
+  l.rows = num_rows;
+  l.K = static_cast<int>(k);
+  l.rank = static_cast<int>(rank);
+  l.adapters = static_cast<int>(num_adapters);
+  l.x = x;
+  l.a = lora_a;
+  l.ids = adapter_ids;
+  l.t = static_cast<float*>(workspace);
+  l.splits = 1;
+  rc = cuda_status(moe::launch_lora_shrink_simt(l, s), kWhat);
+  if (rc != MOE_B200_OK) return rc;
+  moe::GroupedArgs g{};
+  g.dtype = dtype;
+  g.dir = moe::kGmmForward;
+  g.rows = num_rows;
+  g.N = static_cast<int>(n);
+  g.K = static_cast<int>(k);
+  g.E = 1;
+  g.x = x;
+  g.w = weight;
+  g.out = y;
+  moe::LoraTerm term{};
+  term.t = l.t;
+  term.splits = l.splits;
+  term.rank = l.rank;
+  term.adapters = l.adapters;
+  term.b = lora_b;
+  term.ids = adapter_ids;
+  term.scales = scales;
+  return cuda_status(moe::launch_grouped_simt(g, &term, s), kWhat);
+}
+
+}  // extern "C"

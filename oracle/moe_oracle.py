@@ -377,3 +377,53 @@ def make_qmoe_inputs(T, H, I, E, k, bits, block_size, scale_mu, scale_sigma,
                 fc2_scales=s2, fc3_q=q3, fc3_scales=s3,
                 attrs=dict(activation_type="silu", k=k, normalize_routing_weights=1,
                            expert_weight_bits=bits, block_size=block_size))
+
+
+# ------------------------------------------------- expert products and adapters
+
+def grouped_matmul(x, weights, offsets):
+    """y[p] = weights[e] x[p] for offsets[e] <= p < offsets[e+1], float64; rows outside every
+    group are NaN (the operator does not write them).  Also returns sum_k |w||x|, the scale
+    of the rounding bounds."""
+    x, w = np.asarray(x, np.float64), np.asarray(weights, np.float64)
+    y = np.full((x.shape[0], w.shape[1]), np.nan)
+    mag = np.full_like(y, np.nan)
+    for e in range(w.shape[0]):
+        s = slice(int(offsets[e]), int(offsets[e + 1]))
+        y[s] = x[s] @ w[e].T
+        mag[s] = np.abs(x[s]) @ np.abs(w[e]).T
+    return y, mag
+
+
+def grouped_matmul_grad_input(dy, weights, offsets):
+    """dx[p] = weights[e]^T dy[p] (see :func:`grouped_matmul`)."""
+    return grouped_matmul(dy, np.swapaxes(np.asarray(weights, np.float64), 1, 2), offsets)
+
+
+def grouped_matmul_grad_weight(x, dy, offsets):
+    """dw[e] = sum over the rows p of expert e of dy[p] x[p]^T, and the sum of magnitudes."""
+    x, dy = np.asarray(x, np.float64), np.asarray(dy, np.float64)
+    E = len(offsets) - 1
+    dw = np.zeros((E, dy.shape[1], x.shape[1]))
+    mag = np.zeros_like(dw)
+    for e in range(E):
+        s = slice(int(offsets[e]), int(offsets[e + 1]))
+        dw[e] = dy[s].T @ x[s]
+        mag[e] = np.abs(dy[s]).T @ np.abs(x[s])
+    return dw, mag
+
+
+def lora_matmul(x, weight, lora_a, lora_b, ids, scales):
+    """y[t] = weight x[t] + scales[a] lora_b[a] (lora_a[a] x[t]), a = ids[t] (no adapter
+    outside [0, L)), float64.  Also the magnitudes of the rounding bounds: sum |w||x|, and
+    |s| sum_j |b_j| sum_k |a_jk||x_k| for the adapter term."""
+    x, w = np.asarray(x, np.float64), np.asarray(weight, np.float64)
+    a, b = np.asarray(lora_a, np.float64), np.asarray(lora_b, np.float64)
+    y, mag = x @ w.T, np.abs(x) @ np.abs(w).T
+    mag_l = np.zeros_like(y)
+    for t, i in enumerate(np.asarray(ids)):
+        if 0 <= i < a.shape[0]:
+            s = float(scales[i])
+            y[t] += s * (b[i] @ (a[i] @ x[t]))
+            mag_l[t] = abs(s) * (np.abs(b[i]) @ (np.abs(a[i]) @ np.abs(x[t])))
+    return y, mag, mag_l
