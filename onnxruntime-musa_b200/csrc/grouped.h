@@ -27,6 +27,13 @@ struct GroupedArgs {
   void* workspace = nullptr;  // grad_weight on tensor cores: padded row tails
 };
 
+// Tensor-core path: 16-bit types, N and K multiples of 8, 16-byte aligned buffers.
+bool grouped_tc_supported(const GroupedArgs& g);
+size_t grouped_tc_workspace(int dtype, GroupedDir dir, int64_t N, int64_t K, int64_t E);
+cudaError_t launch_grouped_pair(const GroupedArgs& g, int num_sms, cudaStream_t s);
+// Error word of the kernel on the current device (synchronises), cleared.
+cudaError_t take_grouped_pair_error(int* err);
+
 // The adapter term of lora_matmul, added to the forward product of one group.
 struct LoraTerm {
   const float* t;         // [splits][rows][rank]: partial sums of A_a x over K

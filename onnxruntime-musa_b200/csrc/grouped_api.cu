@@ -1,5 +1,7 @@
 // C entries of the expert products (moe_b200_grouped_matmul*) and the adapter projection
 // (moe_b200_lora_matmul): argument checks and the choice of kernel.
+#include <cstdlib>
+
 #include "../../include/moe_b200.h"
 #include "grouped.h"
 
@@ -50,8 +52,32 @@ int check_pointers(const char* what, int32_t dtype, const void* const* ptrs, int
   return MOE_B200_OK;
 }
 
-int run_grouped(const char* what, moe::GroupedArgs& g, cudaStream_t s) {
-  return cuda_status(moe::launch_grouped_simt(g, nullptr, s), what);
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 148;
+  return n;
+}
+
+// With MOE_B200_TRACE_SYNC set: wait for the call and report a device-side timeout.
+int finish(const char* what, cudaStream_t s) {
+  const char* v = std::getenv("MOE_B200_TRACE_SYNC");
+  if (v == nullptr || *v == '\0' || *v == '0') return MOE_B200_OK;
+  int rc = cuda_status(cudaStreamSynchronize(s), what);
+  if (rc != MOE_B200_OK) return rc;
+  int err = 0;
+  rc = cuda_status(moe::take_grouped_pair_error(&err), what);
+  if (rc == MOE_B200_OK && err != 0)
+    return set_error(MOE_B200_EP_FAIL, "%s: device error code %d", what, err);
+  return rc;
+}
+
+int run_grouped(const char* what, const moe::GroupedArgs& g, cudaStream_t s) {
+  const cudaError_t st = moe::grouped_tc_supported(g) ? moe::launch_grouped_pair(g, sm_count(), s)
+                                                      : moe::launch_grouped_simt(g, nullptr, s);
+  const int rc = cuda_status(st, what);
+  return rc != MOE_B200_OK ? rc : finish(what, s);
 }
 
 size_t lora_bytes(int64_t rows, int64_t rank) {
@@ -119,7 +145,7 @@ int moe_b200_grouped_matmul_grad_weight_workspace_size(int32_t dtype, int64_t n,
   if (rc != MOE_B200_OK) return rc;
   if (bytes == nullptr)
     return set_error(MOE_B200_INVALID_ARGUMENT, "%s: bytes must be non-NULL", kWhat);
-  *bytes = 0;
+  *bytes = moe::grouped_tc_workspace(dtype, moe::kGmmGradWeight, n, k, num_experts);
   return MOE_B200_OK;
 }
 

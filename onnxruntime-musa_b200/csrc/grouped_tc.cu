@@ -1,0 +1,522 @@
+// The expert products on the 5th-generation tensor cores: 256 x 256 tiles by CTA pairs.
+//
+// All three products are one kernel that differs in which operand dimension lies contiguous
+// in memory, so no operand is ever transposed in memory:
+//                 M (256 per tile)      N (<= 256 per tile)   contraction
+//   forward       W[e] rows n, K-major  x rows, K-major       K
+//   grad_input    W[e] cols k, MN-major dy rows, K-major      N
+//   grad_weight   dy cols n, MN-major   x cols k, MN-major    rows of e
+// The ragged dimension (the rows of an expert) is the MMA's N in the first two: an expert's
+// rows are cut into ceil(rows / 256) tiles of equal height rounded up to 16, so a tile
+// computes at most 15 rows too many instead of up to 255; rows are columns of the
+// accumulator, so what a tile reads beyond its expert only reaches columns that are not
+// stored.  In grad_weight the ragged dimension is summed over: whole 16-row steps come from
+// dy and x, and the last rows % 16 rows of each expert from a zero-padded copy
+// (tail_kernel), because a neighbour's row in the step would be added (and a zero in only
+// one operand would not stop its infinities).
+//
+// Per CTA: warp 0 TMA producer, warp 1 MMA issuer (leader CTA), warps 2..9 epilogue.  Each
+// CTA stages its 128 of the 256 M entries and half of the N entries of a 64-deep slice
+// (32 KB, six stages); two 256-column accumulators, so the epilogue of a tile overlaps the
+// MMAs of the next.  Bound: the tensor pipe; a slice of the pair is 512 cycles of MMA
+// for 64 KB from L2.
+#include <algorithm>
+#include <mutex>
+
+#include "grouped_tc.cuh"
+
+namespace moe {
+
+namespace {
+
+// Set by a kernel whose bounded wait ran out (a DeviceError); read and cleared by the host
+// under MOE_B200_TRACE_SYNC.  One word per device, not per call: a call has no zeroed
+// workspace to put it in, and zeroing one would cost every call a launch.
+__device__ int g_pair_error;
+
+constexpr int kBK = 64;
+constexpr int kTileM = 256;
+constexpr int kTileN = 256;
+constexpr int kStages = 6;
+constexpr int kABytes = 128 * kBK * 2;
+constexpr int kBBytes = 128 * kBK * 2;
+constexpr int kBox = 64 * kBK * 2;       // one 64 x 64 box of a 16-bit operand
+constexpr int kThreads = 320;
+constexpr int kEpiWarps = 8;
+constexpr int kStageRow = 64;            // bytes of one staged output row (32 elements)
+constexpr int kEpiBytes = 2 * 8 * kStageRow;  // per warp: two buffers of 8 rows
+constexpr int kRaster = 8;               // M-fastest runs of this many tiles (L2 reuse)
+constexpr int kTailRows = 16;
+constexpr int kSmem = 1024 + kStages * (kABytes + kBBytes) + kEpiWarps * kEpiBytes + 256 +
+                      kMaxExperts * 8 + (kMaxExperts + 1) * 4;
+static_assert(kSmem <= 227 * 1024, "shared memory of the pair kernel");
+
+struct PairParams {
+  const int32_t* offsets;
+  int rows, E;
+  int m_dim;      // extent of the M side (features; grad_weight: N)
+  int n_dim;      // grad_weight: K
+  int con;        // contraction length (not grad_weight)
+  int m_tiles, n_tiles;
+  void* out;
+  int64_t ldo;
+};
+
+struct PairTile {
+  int e;
+  int m0;          // first entry of the M side
+  int n0;          // first row (forward, grad_input) or column of x (grad_weight)
+  int n;           // valid N entries
+  int nt;          // MMA N
+  int blocks;      // 64-deep slices
+  int begin, cnt;  // grad_weight: the expert's rows
+};
+
+// Position `local` of an a x b grid walked in runs of kRaster of the first coordinate: the
+// 74 tiles that run at a time then share few operand slices of either side.
+__device__ __forceinline__ void raster(int local, int a, int b, int& i, int& j) {
+  const int run = local / (kRaster * b), in = local - run * kRaster * b;
+  const int w = min(kRaster, a - run * kRaster);
+  j = in / w;
+  i = run * kRaster + in - j * w;
+}
+
+template <int DIR>
+__device__ __forceinline__ PairTile pair_tile(int L, const GroupTable& g, const PairParams& p) {
+  PairTile t;
+  if (DIR == kGmmGradWeight) {
+    const int per = p.m_tiles * p.n_tiles;
+    t.e = L / per;
+    int i, j;
+    raster(L - t.e * per, p.m_tiles, p.n_tiles, i, j);
+    t.m0 = i * kTileM;
+    t.n0 = j * kTileN;
+    t.n = min(kTileN, p.n_dim - t.n0);
+    t.nt = kTileN;
+    t.begin = g.rows[t.e].x;
+    t.cnt = g.rows[t.e].y - t.begin;
+    const int rem = t.cnt % kBK;
+    t.blocks = t.cnt / kBK + (rem >= kTailRows ? 1 : 0) + (rem % kTailRows ? 1 : 0);
+  } else {
+    t.e = find_group(g.tiles, p.E, p.m_tiles, L);
+    const int nt = g.tiles[t.e + 1] - g.tiles[t.e];
+    int i, j;
+    raster(L - g.tiles[t.e] * p.m_tiles, nt, p.m_tiles, i, j);
+    const int2 r = g.rows[t.e];
+    const int h = ((r.y - r.x + nt - 1) / nt + 15) & ~15;
+    t.m0 = j * kTileM;
+    t.n0 = r.x + i * h;
+    t.n = min(h, r.y - t.n0);
+    t.nt = (t.n + 15) & ~15;
+    t.blocks = (p.con + kBK - 1) / kBK;
+    t.begin = t.cnt = 0;
+  }
+  return t;
+}
+
+// MMA steps of 16 in slice `b` of the tile.
+template <int DIR>
+__device__ __forceinline__ int block_steps(const PairTile& t, int b) {
+  if (DIR != kGmmGradWeight) return kBK / 16;
+  const int left = t.cnt - b * kBK;
+  if (left >= kBK) return kBK / 16;
+  // Behind the full slices: the whole steps of the remainder, then the padded tail.
+  return left >= kTailRows && b == t.cnt / kBK ? left / kTailRows : 1;
+}
+// True for the slice that holds the padded tail of the expert.
+__device__ __forceinline__ bool is_tail(const PairTile& t, int b) {
+  return t.cnt % kTailRows != 0 && b == t.blocks - 1;
+}
+
+template <typename T, int DIR>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
+                    const __grid_constant__ CUtensorMap map_b,
+                    const __grid_constant__ CUtensorMap map_at,
+                    const __grid_constant__ CUtensorMap map_bt, const PairParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + kStages * kABytes;
+  uint8_t* stage_out = sB + kStages * kBBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(stage_out + kEpiWarps * kEpiBytes);
+  uint64_t* full = bars;
+  uint64_t* empty = bars + kStages;
+  uint64_t* tfull = bars + 2 * kStages;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* done = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert((2 * kStages + 5) * 8 + 8 <= 256, "barrier block");
+  GroupTable table;
+  table.rows = reinterpret_cast<int2*>(bars + 32);
+  table.tiles = reinterpret_cast<int*>(table.rows + kMaxExperts);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 2 * kEpiWarps);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_mbarrier_init();
+    tma_prefetch_desc(&map_a);
+    tma_prefetch_desc(&map_b);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 2 * kTileN);
+    tmem_relinquish_pair();
+  }
+  pdl_wait();  // grad_weight: the padded tails are written by the launch before
+  if (warp == 2) build_group_table(p.offsets, p.E, p.rows, kTileN, table);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers are initialised before any remote signal
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int total =
+      DIR == kGmmGradWeight ? p.E * p.m_tiles * p.n_tiles : table.tiles[p.E] * p.m_tiles;
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  constexpr bool kAMn = DIR != kGmmForward;
+  constexpr bool kBMn = DIR == kGmmGradWeight;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------- TMA producer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int L = pair; L < total && !*abort_flag; L += npairs) {
+        const PairTile t = pair_tile<DIR>(L, table, p);
+        const int a0 = t.m0 + static_cast<int>(rank) * 128;
+        // Rows of this CTA's half of the MMA's N, in boxes of 64.
+        const int half = t.nt / 2;
+        const int b0 = t.n0 + static_cast<int>(rank) * half;
+        const int b_boxes = DIR == kGmmGradWeight ? 2 : (half + 63) / 64;
+        for (int b = 0; b < t.blocks; ++b) {
+          if (!mbar_wait(&empty[stage], phase ^ 1)) {
+            atomicExch(&g_pair_error, kErrTimeoutProducer);
+            *abort_flag = 1;
+            break;
+          }
+          const bool tail = DIR == kGmmGradWeight && is_tail(t, b);
+          const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);
+          if (leader)
+            mbar_arrive_expect_tx(&full[stage], tail ? 2 * 4 * kTailRows * 128
+                                                     : 2 * (kABytes + b_boxes * kBox));
+          uint8_t* da = sA + stage * kABytes;
+          uint8_t* db = sB + stage * kBBytes;
+          const int c = b * kBK;
+          if (DIR == kGmmForward) {
+            tma_load_3d_pair(da, &map_a, bar, c, a0, t.e);
+          } else if (DIR == kGmmGradInput) {
+            tma_load_3d_pair(da, &map_a, bar, a0, c, t.e);
+            tma_load_3d_pair(da + kBox, &map_a, bar, a0 + 64, c, t.e);
+          } else {
+            const CUtensorMap* m = tail ? &map_at : &map_a;
+            const int r = tail ? t.e * kTailRows : t.begin + c;
+            tma_load_3d_pair(da, m, bar, a0, r, 0);
+            tma_load_3d_pair(da + kBox, m, bar, a0 + 64, r, 0);
+          }
+          if (DIR == kGmmGradWeight) {
+            const CUtensorMap* m = tail ? &map_bt : &map_b;
+            const int r = tail ? t.e * kTailRows : t.begin + c;
+            tma_load_3d_pair(db, m, bar, b0, r, 0);
+            tma_load_3d_pair(db + kBox, m, bar, b0 + 64, r, 0);
+          } else {
+            for (int j = 0; j < b_boxes; ++j)
+              tma_load_3d_pair(db + j * kBox, &map_b, bar, c, b0 + j * 64, 0);
+          }
+          if (++stage == kStages) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------- MMA issuer (leader CTA only)
+    if (lane == 0 && leader) {
+      int stage = 0, i = 0;
+      uint32_t phase = 0;
+      for (int L = pair; L < total && !*abort_flag; L += npairs, ++i) {
+        const PairTile t = pair_tile<DIR>(L, table, p);
+        const uint32_t idesc = idesc_f16(TcFormat<T>::kId, kTileM, t.nt) |
+                               (kAMn ? kIdescAMn : 0) | (kBMn ? kIdescBMn : 0);
+        const int acc = i & 1;
+        if (!mbar_wait(&tempty[acc], ((i >> 1) & 1) ^ 1)) {
+          atomicExch(&g_pair_error, kErrTimeoutMma);
+          *abort_flag = 1;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem_base + acc * kTileN;
+        bool ok = true;
+        for (int b = 0; b < t.blocks; ++b) {
+          if (!mbar_wait(&full[stage], phase)) {
+            atomicExch(&g_pair_error, kErrTimeoutMma);
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a = smem_u32(sA + stage * kABytes);
+          const uint32_t bb = smem_u32(sB + stage * kBBytes);
+          const int steps = block_steps<DIR>(t, b);
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k) {
+            if (k >= steps) break;
+            // 16 contraction entries on: 32 bytes along a K-major row, 16 rows of 128
+            // bytes of an MN-major block.
+            const uint64_t ad = kAMn ? smem_desc_mn_sw128(a + k * 2048, kBox)
+                                     : smem_desc_k_sw128(a + k * 32);
+            const uint64_t bd = kBMn ? smem_desc_mn_sw128(bb + k * 2048, kBox)
+                                     : smem_desc_k_sw128(bb + k * 32);
+            tc_mma_f16_pair(d, ad, bd, idesc, (b | k) != 0 ? 1u : 0u);
+          }
+          tc_commit_pair(&empty[stage], 0x3);
+          if (++stage == kStages) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        tc_commit_pair(&tfull[acc], 0x3);
+      }
+      tc_commit_pair(done, 0x1);
+      mbar_wait(done, 0);
+    }
+  } else {
+    // ----------------------------------------------------- epilogue (both CTAs)
+    const int q = warp & 3;               // TMEM lane quarter of this warp
+    const int first = warp < 6 ? 0 : 32;  // its 32-column chunks: every other one
+    uint8_t* buf = stage_out + (warp - 2) * kEpiBytes;
+    // stmatrix row addresses: lane 8i + t is row t of block i; 16-byte granules are XORed
+    // with the row so that neither the blocks nor the 16-byte reads conflict.
+    const int st_row = lane & 7, st_blk = lane >> 3;
+    const uint32_t st_addr =
+        smem_u32(buf) + st_row * kStageRow + ((st_blk ^ ((st_row >> 1) & 3)) << 4);
+    const int rd_row = lane >> 2, rd_blk = lane & 3;
+    const uint8_t* rd_ptr = buf + rd_row * kStageRow + ((rd_blk ^ ((rd_row >> 1) & 3)) << 4);
+    T* out = static_cast<T*>(p.out);
+    int i = 0;
+    for (int L = pair; L < total && !*abort_flag; L += npairs, ++i) {
+      const PairTile t = pair_tile<DIR>(L, table, p);
+      const int acc = i & 1;
+      if (!mbar_wait(&tfull[acc], (i >> 1) & 1)) {
+        atomicExch(&g_pair_error, kErrTimeoutEpilogue);
+        *abort_flag = 1;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t taddr =
+          tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * kTileN;
+      const int m = t.m0 + static_cast<int>(rank) * 128 + q * 32;  // first M entry of the warp
+      for (int c = first; c < t.n; c += 64) {
+        float lo[16], hi[16];
+        if (DIR == kGmmGradWeight && t.cnt == 0) {  // an expert without rows: zeros
+#pragma unroll
+          for (int j = 0; j < 16; ++j) lo[j] = hi[j] = 0.f;
+        } else {
+          tmem_ld_frag4(taddr + c, lo);
+          tmem_ld_frag4(taddr + (16u << 16) + c, hi);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int sel = (j & 1) * 8 * kStageRow;
+          T* dst;
+          bool ok;
+          if (DIR == kGmmGradWeight) {
+            // Eight M rows (block j of the 32) x 32 columns.
+            const float(&v)[16] = j < 2 ? lo : hi;
+            const int o = (j & 1) * 2;
+            stmatrix4(st_addr + sel, pack2<T>(v[o], v[o + 1]), pack2<T>(v[4 + o], v[5 + o]),
+                      pack2<T>(v[8 + o], v[9 + o]), pack2<T>(v[12 + o], v[13 + o]));
+            const int row = m + 8 * j + rd_row, col = c + 8 * rd_blk;
+            ok = row < p.m_dim && col < t.n;
+            dst = out + (static_cast<int64_t>(t.e) * p.m_dim + row) * p.ldo + t.n0 + col;
+          } else {
+            // Eight rows of the output (accumulator columns) x 32 features, transposed.
+            stmatrix4_t(st_addr + sel, pack2<T>(lo[4 * j], lo[4 * j + 1]),
+                        pack2<T>(lo[4 * j + 2], lo[4 * j + 3]), pack2<T>(hi[4 * j], hi[4 * j + 1]),
+                        pack2<T>(hi[4 * j + 2], hi[4 * j + 3]));
+            const int row = c + 8 * j + rd_row, col = m + 8 * rd_blk;
+            ok = row < t.n && col < p.m_dim;
+            dst = out + static_cast<int64_t>(t.n0 + row) * p.ldo + col;
+          }
+          __syncwarp();
+          const uint4 w = *reinterpret_cast<const uint4*>(rd_ptr + sel);
+          if (ok) *reinterpret_cast<uint4*>(dst) = w;
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while its peer may still signal it or read its smem
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 2 * kTileN);
+  }
+}
+
+// The last cnt % 16 rows of each expert's dy and x, padded with zero rows to 16, as
+// [E][16][N] and [E][16][K] (16-byte vectors; N and K are multiples of 8).
+__global__ void __launch_bounds__(256)
+tail_kernel(const int32_t* __restrict__ offsets, int rows, const uint4* __restrict__ dy, int nv,
+            const uint4* __restrict__ x, int kv, uint4* __restrict__ ty, uint4* __restrict__ tx) {
+  pdl_launch_dependents();
+  const int e = blockIdx.y;
+  const int begin = min(max(__ldg(offsets + e), 0), rows);
+  const int end = max(min(max(__ldg(offsets + e + 1), 0), rows), begin);
+  const int rem = (end - begin) % kTailRows, r0 = end - rem;
+  if (rem == 0) return;  // no tail slice reads this expert's part
+  const int per = nv + kv;
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < kTailRows * per; i += gridDim.x * 256) {
+    const int r = i / per, c = i - r * per;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (c < nv) {
+      if (r < rem) v = dy[static_cast<int64_t>(r0 + r) * nv + c];
+      ty[(static_cast<int64_t>(e) * kTailRows + r) * nv + c] = v;
+    } else {
+      if (r < rem) v = x[static_cast<int64_t>(r0 + r) * kv + c - nv];
+      tx[(static_cast<int64_t>(e) * kTailRows + r) * kv + c - nv] = v;
+    }
+  }
+}
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* q = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &q, cudaEnableDefault, &r) ==
+            cudaSuccess &&
+        r == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(q);
+  });
+  return fn;
+}
+
+size_t tail_bytes(int64_t E, int64_t width) {
+  return (static_cast<size_t>(E) * kTailRows * static_cast<size_t>(width) * 2 + 255) & ~size_t{255};
+}
+
+template <typename T, int DIR>
+cudaError_t launch_pair(const GroupedArgs& g, int num_sms, cudaStream_t s) {
+  CUtensorMap ma, mb, mat, mbt;
+  PairParams p{};
+  p.offsets = g.offsets;
+  p.rows = static_cast<int>(g.rows);
+  p.E = g.E;
+  p.out = g.out;
+  bool ok;
+  int64_t tiles;
+  if (DIR == kGmmGradWeight) {
+    auto* ty = static_cast<uint8_t*>(g.workspace);
+    uint8_t* tx = ty + tail_bytes(g.E, g.N);
+    p.m_dim = g.N;
+    p.n_dim = g.K;
+    p.ldo = g.K;
+    p.n_tiles = (g.K + kTileN - 1) / kTileN;
+    ok = grouped_map(&ma, g.dtype, g.dy, g.N, g.rows, 1, 64) &&
+         grouped_map(&mb, g.dtype, g.x, g.K, g.rows, 1, 64) &&
+         grouped_map(&mat, g.dtype, ty, g.N, static_cast<int64_t>(g.E) * kTailRows, 1, kTailRows) &&
+         grouped_map(&mbt, g.dtype, tx, g.K, static_cast<int64_t>(g.E) * kTailRows, 1, kTailRows);
+    if (!ok) return cudaErrorInvalidValue;
+    const int vecs = kTailRows * (g.N + g.K) / 8;
+    tail_kernel<<<dim3(std::min(32, (vecs + 255) / 256), g.E), 256, 0, s>>>(
+        g.offsets, p.rows, static_cast<const uint4*>(g.dy), g.N / 8,
+        static_cast<const uint4*>(g.x), g.K / 8, reinterpret_cast<uint4*>(ty),
+        reinterpret_cast<uint4*>(tx));
+    cudaError_t st = cudaGetLastError();
+    if (st != cudaSuccess) return st;
+  } else {
+    const int feat = DIR == kGmmForward ? g.N : g.K;
+    p.m_dim = feat;
+    p.con = DIR == kGmmForward ? g.K : g.N;
+    p.ldo = feat;
+    ok = grouped_map(&ma, g.dtype, g.w, g.K, g.N, g.E, DIR == kGmmForward ? 128 : 64) &&
+         grouped_map(&mb, g.dtype, DIR == kGmmForward ? g.x : g.dy, p.con, g.rows, 1, 64);
+    if (!ok) return cudaErrorInvalidValue;
+    mat = ma;
+    mbt = mb;
+  }
+  p.m_tiles = (p.m_dim + kTileM - 1) / kTileM;
+  tiles = DIR == kGmmGradWeight
+              ? static_cast<int64_t>(g.E) * p.m_tiles * p.n_tiles
+              : (g.rows / kTileN + std::min<int64_t>(g.rows, g.E)) * p.m_tiles;
+  static SmemOptIn opt_in;
+  cudaError_t st = opt_in.set(grouped_pair_kernel<T, DIR>, kSmem);
+  if (st != cudaSuccess) return st;
+  const int64_t pairs = std::min<int64_t>(tiles, num_sms / 2);
+  return launch_dependent(DIR == kGmmGradWeight, grouped_pair_kernel<T, DIR>,
+                          dim3(static_cast<unsigned>(2 * pairs)), dim3(kThreads), kSmem, s, ma, mb,
+                          mat, mbt, p);
+}
+
+template <typename T>
+cudaError_t launch_pair_type(const GroupedArgs& g, int num_sms, cudaStream_t s) {
+  if (g.dir == kGmmForward) return launch_pair<T, kGmmForward>(g, num_sms, s);
+  if (g.dir == kGmmGradInput) return launch_pair<T, kGmmGradInput>(g, num_sms, s);
+  return launch_pair<T, kGmmGradWeight>(g, num_sms, s);
+}
+
+}  // namespace
+
+bool grouped_map(CUtensorMap* m, int dtype, const void* ptr, int64_t dim0, int64_t dim1,
+                 int64_t dim2, int box1) {
+  EncodeTiledFn enc = encode_fn();
+  if (enc == nullptr) return false;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim0), static_cast<cuuint64_t>(dim1),
+                        static_cast<cuuint64_t>(dim2)};
+  cuuint64_t strides[2] = {dims[0] * 2, dims[0] * dims[1] * 2};
+  cuuint32_t box[3] = {kBK, static_cast<cuuint32_t>(box1), 1};
+  cuuint32_t es[3] = {1, 1, 1};
+  return enc(m, dtype == kDtBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+             3, const_cast<void*>(ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+size_t grouped_tc_workspace(int dtype, GroupedDir dir, int64_t N, int64_t K, int64_t E) {
+  if (dir != kGmmGradWeight || dtype == kDtF32 || N % 8 != 0 || K % 8 != 0) return 0;
+  return tail_bytes(E, N) + tail_bytes(E, K);
+}
+
+bool grouped_tc_supported(const GroupedArgs& g) {
+  if (g.dtype != kDtF16 && g.dtype != kDtBF16) return false;
+  if (g.N % 8 != 0 || g.K % 8 != 0) return false;
+  auto aligned = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
+  // A direction's unused operand is NULL and so aligned.
+  return aligned(g.x) && aligned(g.dy) && aligned(g.w) && aligned(g.out);
+}
+
+cudaError_t launch_grouped_pair(const GroupedArgs& g, int num_sms, cudaStream_t s) {
+  if (g.dtype == kDtF16) return launch_pair_type<__half>(g, num_sms, s);
+  if (g.dtype == kDtBF16) return launch_pair_type<__nv_bfloat16>(g, num_sms, s);
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t take_grouped_pair_error(int* err) {
+  cudaError_t st = cudaMemcpyFromSymbol(err, g_pair_error, sizeof(int));
+  if (st != cudaSuccess || *err == 0) return st;
+  const int zero = 0;
+  return cudaMemcpyToSymbol(g_pair_error, &zero, sizeof(int));
+}
+
+}  // namespace moe
