@@ -27,13 +27,6 @@ struct GroupedArgs {
   void* workspace = nullptr;  // grad_weight on tensor cores: padded row tails
 };
 
-// Tensor-core path: 16-bit types, N and K multiples of 8, 16-byte aligned buffers.
-bool grouped_tc_supported(const GroupedArgs& g);
-size_t grouped_tc_workspace(int dtype, GroupedDir dir, int64_t N, int64_t K, int64_t E);
-cudaError_t launch_grouped_pair(const GroupedArgs& g, int num_sms, cudaStream_t s);
-// Error word of the kernel on the current device (synchronises), cleared.
-cudaError_t take_grouped_pair_error(int* err);
-
 // The adapter term of lora_matmul, added to the forward product of one group.
 struct LoraTerm {
   const float* t;         // [splits][rows][rank]: partial sums of A_a x over K
@@ -63,6 +56,27 @@ struct LoraShrink {
   int splits;
 };
 cudaError_t launch_lora_shrink_simt(const LoraShrink& l, cudaStream_t s);  // splits = 1
+
+// The tensor-core form (16-bit types, K and rank multiples of 8, 16-byte aligned x and a)
+// leaves `splits` partial sums.
+int lora_shrink_splits(int64_t rows, int K);
+bool lora_shrink_tc_supported(const LoraShrink& l);
+cudaError_t launch_lora_shrink_tc(const LoraShrink& l, cudaStream_t s);
+
+// Tensor-core path: 16-bit types, N and K multiples of 8, 16-byte aligned buffers.
+bool grouped_tc_supported(const GroupedArgs& g);
+size_t grouped_tc_workspace(int dtype, GroupedDir dir, int64_t N, int64_t K, int64_t E);
+// 256 x 256 tiles by CTA pairs, and weight streaming for few rows per group (not
+// grad_weight).  `lora` (forward, one group, rank % 8 == 0) may be nullptr; t is then
+// awaited with pdl_wait().
+cudaError_t launch_grouped_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
+                                cudaStream_t s);
+cudaError_t launch_grouped_small(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
+                                 cudaStream_t s);
+// Error words of the tensor-core kernels on the current device (each synchronises), cleared.
+cudaError_t take_grouped_pair_error(int* err);
+cudaError_t take_grouped_small_error(int* err);
+cudaError_t take_lora_error(int* err);
 
 // FFMA kernels: any size, alignment and float type.
 cudaError_t launch_grouped_simt(const GroupedArgs& g, const LoraTerm* lora, cudaStream_t s);

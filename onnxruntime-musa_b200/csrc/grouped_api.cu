@@ -66,22 +66,43 @@ int finish(const char* what, cudaStream_t s) {
   if (v == nullptr || *v == '\0' || *v == '0') return MOE_B200_OK;
   int rc = cuda_status(cudaStreamSynchronize(s), what);
   if (rc != MOE_B200_OK) return rc;
-  int err = 0;
-  rc = cuda_status(moe::take_grouped_pair_error(&err), what);
-  if (rc == MOE_B200_OK && err != 0)
-    return set_error(MOE_B200_EP_FAIL, "%s: device error code %d", what, err);
-  return rc;
+  for (auto take : {moe::take_grouped_pair_error, moe::take_grouped_small_error,
+                    moe::take_lora_error}) {
+    int err = 0;
+    rc = cuda_status(take(&err), what);
+    if (rc == MOE_B200_OK && err != 0)
+      rc = set_error(MOE_B200_EP_FAIL, "%s: device error code %d", what, err);
+    if (rc != MOE_B200_OK) return rc;
+  }
+  return MOE_B200_OK;
+}
+
+// The pair kernel once its 256-row tiles are filled (mean rows per group) and there are
+// enough of them for the SM pairs; else the weight-streaming kernel.
+bool use_pair(const moe::GroupedArgs& g, int sms) {
+  if (g.dir == moe::kGmmGradWeight) return true;
+  const int64_t feat = g.dir == moe::kGmmForward ? g.N : g.K;
+  const int64_t per = g.rows / g.E;
+  const int64_t tiles = (per + 255) / 256 * g.E * ((feat + 255) / 256);
+  return per >= 128 && tiles >= sms / 2 * 3 / 4;
+}
+
+cudaError_t launch_tc(const moe::GroupedArgs& g, const moe::LoraTerm* lora, cudaStream_t s) {
+  const int sms = sm_count();
+  return use_pair(g, sms) ? moe::launch_grouped_pair(g, lora, sms, s)
+                          : moe::launch_grouped_small(g, lora, sms, s);
 }
 
 int run_grouped(const char* what, const moe::GroupedArgs& g, cudaStream_t s) {
-  const cudaError_t st = moe::grouped_tc_supported(g) ? moe::launch_grouped_pair(g, sm_count(), s)
+  const cudaError_t st = moe::grouped_tc_supported(g) ? launch_tc(g, nullptr, s)
                                                       : moe::launch_grouped_simt(g, nullptr, s);
   const int rc = cuda_status(st, what);
   return rc != MOE_B200_OK ? rc : finish(what, s);
 }
 
-size_t lora_bytes(int64_t rows, int64_t rank) {
-  return static_cast<size_t>(rows) * static_cast<size_t>(rank) * sizeof(float);
+size_t lora_bytes(int32_t dtype, int64_t rows, int64_t k, int64_t rank) {
+  const int64_t splits = dtype == moe::kDtF32 ? 1 : moe::lora_shrink_splits(rows, static_cast<int>(k));
+  return static_cast<size_t>(rows * splits) * static_cast<size_t>(rank) * sizeof(float);
 }
 
 }  // namespace
@@ -193,14 +214,14 @@ int moe_b200_grouped_matmul_grad_weight(int32_t dtype, int64_t num_rows, int64_t
   return run_grouped(kWhat, g, s);
 }
 
-int moe_b200_lora_matmul_workspace_size(int32_t dtype, int64_t num_rows, int64_t rank,
-                                        size_t* bytes) {
+int moe_b200_lora_matmul_workspace_size(int32_t dtype, int64_t num_rows, int64_t k,
+                                        int64_t rank, size_t* bytes) {
   static const char* kWhat = "lora_matmul_workspace_size";
-  int rc = check_shape(kWhat, dtype, num_rows, 1, 1, rank, "rank", moe::kLoraMaxRank);
+  int rc = check_shape(kWhat, dtype, num_rows, 1, k, rank, "rank", moe::kLoraMaxRank);
   if (rc != MOE_B200_OK) return rc;
   if (bytes == nullptr)
     return set_error(MOE_B200_INVALID_ARGUMENT, "%s: bytes must be non-NULL", kWhat);
-  *bytes = lora_bytes(num_rows, rank);
+  *bytes = lora_bytes(dtype, num_rows, k, rank);
   return MOE_B200_OK;
 }
 
@@ -222,7 +243,7 @@ int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
   const void* words[] = {adapter_ids, scales};
   rc = check_pointers(kWhat, dtype, ptrs, 5, words, 2);
   if (rc != MOE_B200_OK) return rc;
-  const size_t need = lora_bytes(num_rows, rank);
+  const size_t need = lora_bytes(dtype, num_rows, k, rank);
   if (workspace_bytes < need || workspace == nullptr ||
       reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
     return set_error(MOE_B200_INVALID_ARGUMENT,
@@ -238,9 +259,6 @@ int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
   l.a = lora_a;
   l.ids = adapter_ids;
   l.t = static_cast<float*>(workspace);
-  l.splits = 1;
-  rc = cuda_status(moe::launch_lora_shrink_simt(l, s), kWhat);
-  if (rc != MOE_B200_OK) return rc;
   moe::GroupedArgs g{};
   g.dtype = dtype;
   g.dir = moe::kGmmForward;
@@ -251,6 +269,12 @@ int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
   g.x = x;
   g.w = weight;
   g.out = y;
+  const bool a16 = (reinterpret_cast<uintptr_t>(lora_b) & 15) == 0;
+  const bool tc = moe::grouped_tc_supported(g) && moe::lora_shrink_tc_supported(l) && a16;
+  l.splits = tc ? moe::lora_shrink_splits(num_rows, l.K) : 1;
+  rc = cuda_status(tc ? moe::launch_lora_shrink_tc(l, s) : moe::launch_lora_shrink_simt(l, s),
+                   kWhat);
+  if (rc != MOE_B200_OK) return rc;
   moe::LoraTerm term{};
   term.t = l.t;
   term.splits = l.splits;
@@ -259,7 +283,8 @@ int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
   term.b = lora_b;
   term.ids = adapter_ids;
   term.scales = scales;
-  return cuda_status(moe::launch_grouped_simt(g, &term, s), kWhat);
+  rc = cuda_status(tc ? launch_tc(g, &term, s) : moe::launch_grouped_simt(g, &term, s), kWhat);
+  return rc != MOE_B200_OK ? rc : finish(kWhat, s);
 }
 
 }  // extern "C"

@@ -1,0 +1,345 @@
+// The expert products and the adapter projection for few rows per group: streaming the
+// weights.
+//
+// y[p] = W[e] x[p] with a handful of rows reads every weight once for a few products; the
+// floor is the weights' bytes over the HBM rate, and what decides is how many bytes are in
+// flight.  So a tile is 128 features x all rows of the group (<= the tile cap), as
+// D[feature, row] (weights are the MMA's M = 128, rows its N = 16 .. 256), and the
+// contraction is split over a cluster of 1..8 CTAs so that the tiles of a call fill the
+// GPU: each CTA streams its share of the slices through a TMA ring of about 100 KB (two
+// CTAs an SM, 200 KB in flight) into one tcgen05 accumulator.  The partial sums are joined
+// through distributed shared memory -- 8-row blocks of the accumulator go to the CTA that
+// owns the block, which adds them in rank order -- so there is no global workspace, no
+// counter to clear, no second launch, and the result is the same bits on every call.
+#include <algorithm>
+
+#include "grouped_lora.cuh"
+
+namespace moe {
+namespace {
+
+__device__ int g_small_error;
+
+constexpr int kBK = 64;
+constexpr int kTileM = 128;
+constexpr int kWBytes = kTileM * kBK * 2;
+constexpr int kThreads = 256;
+constexpr int kMaxStages = 8;
+constexpr int kStageRow = 64;                    // bytes of a staged output row
+constexpr int kEpiBytes = 8 * kStageRow;         // per warp
+constexpr int kPartBytes = 4 * 8 * 32 * 4;       // one CTA's part of an 8-row block (fp32)
+constexpr int kFixed = 1024 + 8 * kEpiBytes + 256 + kMaxExperts * 8 + (kMaxExperts + 1) * 4 + 12;
+
+struct SmallParams {
+  const int32_t* offsets;
+  int64_t total_rows;
+  int E;
+  int m_dim, con;
+  int m_tiles;
+  int cap;            // most rows of a tile (16, 32, 64, 128 or 256)
+  int box;            // rows of one TMA box of the rows operand: min(cap, 64)
+  int splits;         // cluster size
+  int stages, stage_bytes;
+  uint32_t tmem_cols;
+  void* out;
+  int64_t ldo;
+  LoraTerm lora;
+};
+
+__device__ __forceinline__ void tmem_ld_frag1(uint32_t taddr, float (&v)[4]) {
+  uint32_t r[4];
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void st_cluster_f4(uint32_t addr, const float (&v)[4]) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v[0]),
+               "f"(v[1]), "f"(v[2]), "f"(v[3])
+               : "memory");
+}
+
+template <typename T, int DIR, bool LORA>
+__global__ void __launch_bounds__(kThreads)
+grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
+                     const __grid_constant__ CUtensorMap map_x, const SmallParams p) {
+  constexpr bool kAMn = DIR == kGmmGradInput;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* stage_out = ring + p.stages * p.stage_bytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(stage_out + 8 * kEpiBytes);
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* tfull = empty + kMaxStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert((2 * kMaxStages + 1) * 8 + 8 <= 256, "barrier block");
+  GroupTable table;
+  table.rows = reinterpret_cast<int2*>(full + 32);
+  table.tiles = reinterpret_cast<int*>(table.rows + kMaxExperts);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = p.splits == 1 ? 0 : static_cast<int>(cluster_ctarank());
+  const int L = blockIdx.x / p.splits;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(tfull, 1);
+    *abort_flag = 0;
+    fence_mbarrier_init();
+    tma_prefetch_desc(&map_w);
+    tma_prefetch_desc(&map_x);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, p.tmem_cols);
+    tmem_relinquish();
+  }
+  if (warp == 2)
+    build_group_table(p.offsets, p.E, static_cast<int>(p.total_rows), p.cap, table);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (L >= table.tiles[p.E] * p.m_tiles) {  // the grid is an upper bound; whole clusters leave
+    if (warp == 1) tmem_dealloc(tmem, p.tmem_cols);
+    return;
+  }
+
+  // Tile: the row tiles of a weight tile run side by side (the weights then come from L2).
+  const int e = find_group(table.tiles, p.E, p.m_tiles, L);
+  const int nt_tiles = table.tiles[e + 1] - table.tiles[e];
+  const int local = L - table.tiles[e] * p.m_tiles;
+  const int m0 = (local / nt_tiles) * kTileM;
+  const int2 gr = table.rows[e];
+  const int h = ((gr.y - gr.x + nt_tiles - 1) / nt_tiles + 15) & ~15;
+  const int row0 = gr.x + (local % nt_tiles) * h;
+  const int n = min(h, gr.y - row0);
+  const int nt = max((n + 15) & ~15, 16);
+  const int slices = (p.con + kBK - 1) / kBK;
+  const int s0 = static_cast<int>(static_cast<int64_t>(slices) * split / p.splits);
+  const int s1 = static_cast<int>(static_cast<int64_t>(slices) * (split + 1) / p.splits);
+
+  if (warp == 0 && lane == 0) {
+    const int boxes = (nt + p.box - 1) / p.box;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int s = s0; s < s1; ++s) {
+      if (!mbar_wait(&empty[stage], phase ^ 1)) {
+        atomicExch(&g_small_error, kErrTimeoutProducer);
+        *abort_flag = 1;
+        break;
+      }
+      uint8_t* w = ring + stage * p.stage_bytes;
+      mbar_arrive_expect_tx(&full[stage], kWBytes + boxes * p.box * kBK * 2);
+      const int c = s * kBK;
+      if (kAMn) {
+        tma_load_3d(w, &map_w, &full[stage], m0, c, e);
+        tma_load_3d(w + kWBytes / 2, &map_w, &full[stage], m0 + 64, c, e);
+      } else {
+        tma_load_3d(w, &map_w, &full[stage], c, m0, e);
+      }
+      for (int j = 0; j < boxes; ++j)
+        tma_load_3d(w + kWBytes + j * p.box * kBK * 2, &map_x, &full[stage], c,
+                    row0 + j * p.box, 0);
+      if (++stage == p.stages) { stage = 0; phase ^= 1; }
+    }
+  } else if (warp == 1 && lane == 0) {
+    const uint32_t idesc = idesc_f16(TcFormat<T>::kId, kTileM, nt) | (kAMn ? kIdescAMn : 0);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int s = s0; s < s1; ++s) {
+      if (!mbar_wait(&full[stage], phase)) {
+        atomicExch(&g_small_error, kErrTimeoutMma);
+        *abort_flag = 1;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t w = smem_u32(ring + stage * p.stage_bytes);
+#pragma unroll
+      for (int k = 0; k < kBK / 16; ++k) {
+        const uint64_t ad = kAMn ? smem_desc_mn_sw128(w + k * 2048, kWBytes / 2)
+                                 : smem_desc_k_sw128(w + k * 32);
+        tc_mma_f16(tmem, ad, smem_desc_k_sw128(w + kWBytes + k * 32), idesc,
+                   (s != s0 || k != 0) ? 1u : 0u);
+      }
+      tc_commit(&empty[stage]);
+      if (++stage == p.stages) { stage = 0; phase ^= 1; }
+    }
+    tc_commit(tfull);
+  }
+  __syncwarp();
+  const bool ok = mbar_wait(tfull, 0);
+  if (!ok) {
+    atomicExch(&g_small_error, kErrTimeoutEpilogue);
+    *abort_flag = 1;
+  }
+  tc_fence_after();
+
+  // Warp w reads TMEM lanes 32 (w % 4) ..; the warps of a lane quarter take alternate
+  // 8-row blocks of those this CTA owns (block b belongs to CTA b % splits).
+  const int q = warp & 3, pair = warp >> 2;
+  const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16);
+  const int blocks = (n + 7) / 8;
+  const bool empty_part = s0 == s1 || !ok;  // nothing accumulated: the part is zero
+  const int S = p.splits;
+  if (S > 1) {
+    cluster_sync();  // every CTA's MMAs have read its ring: the rings take the parts now
+    for (int b = pair; b < blocks; b += 2) {
+      const int owner = b % S;
+      if (owner == split) continue;
+      float lo[4] = {0.f, 0.f, 0.f, 0.f}, hi[4] = {0.f, 0.f, 0.f, 0.f};
+      if (!empty_part) {
+        tmem_ld_frag1(taddr + 8 * b, lo);
+        tmem_ld_frag1(taddr + (16u << 16) + 8 * b, hi);
+        tmem_ld_wait();
+      }
+      // Slot of this sender among the owner's S - 1, block b / S of the owner's.
+      const int slot = split < owner ? split : split - 1;
+      const uint32_t dst = smem_u32(ring) + ((b / S) * (S - 1) + slot) * kPartBytes +
+                           q * (kPartBytes / 4) + lane * 16;
+      st_cluster_f4(mapa_shared(dst, owner), lo);
+      st_cluster_f4(mapa_shared(dst + 512, owner), hi);
+    }
+    cluster_sync();
+  }
+  if (LORA) pdl_wait();  // t comes from the launch before this one
+
+  uint8_t* buf = stage_out + warp * kEpiBytes;
+  const int st_row = lane & 7, st_blk = lane >> 3;
+  const uint32_t st_addr =
+      smem_u32(buf) + st_row * kStageRow + ((st_blk ^ ((st_row >> 1) & 3)) << 4);
+  const int rd_row = lane >> 2, rd_blk = lane & 3;
+  const uint8_t* rd_ptr = buf + rd_row * kStageRow + ((rd_blk ^ ((rd_row >> 1) & 3)) << 4);
+  const int feat = m0 + q * 32;
+  for (int i = pair; i * S + split < blocks; i += 2) {
+    const int b = i * S + split;
+    float lo[4] = {0.f, 0.f, 0.f, 0.f}, hi[4] = {0.f, 0.f, 0.f, 0.f};
+    float own_lo[4] = {0.f, 0.f, 0.f, 0.f}, own_hi[4] = {0.f, 0.f, 0.f, 0.f};
+    if (!empty_part) {
+      tmem_ld_frag1(taddr + 8 * b, own_lo);
+      tmem_ld_frag1(taddr + (16u << 16) + 8 * b, own_hi);
+      tmem_ld_wait();
+    }
+    for (int r = 0; r < S; ++r) {  // the parts in rank order
+      if (r == split) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { lo[j] += own_lo[j]; hi[j] += own_hi[j]; }
+      } else {
+        const uint8_t* src = ring + (i * (S - 1) + (r < split ? r : r - 1)) * kPartBytes +
+                             q * (kPartBytes / 4) + lane * 16;
+        const float4 a = *reinterpret_cast<const float4*>(src);
+        const float4 c = *reinterpret_cast<const float4*>(src + 512);
+        lo[0] += a.x; lo[1] += a.y; lo[2] += a.z; lo[3] += a.w;
+        hi[0] += c.x; hi[1] += c.y; hi[2] += c.z; hi[3] += c.w;
+      }
+    }
+    if (LORA) lora_add<T>(p.lora, p.total_rows, row0 + 8 * b, row0 + n, feat, p.m_dim, lo, hi);
+    stmatrix4_t(st_addr, pack2<T>(lo[0], lo[1]), pack2<T>(lo[2], lo[3]), pack2<T>(hi[0], hi[1]),
+                pack2<T>(hi[2], hi[3]));
+    __syncwarp();
+    const uint4 w = *reinterpret_cast<const uint4*>(rd_ptr);
+    const int row = 8 * b + rd_row, col = feat + 8 * rd_blk;
+    if (row < n && col < p.m_dim)
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.out) +
+                                static_cast<int64_t>(row0 + row) * p.ldo + col) = w;
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, p.tmem_cols);
+  }
+}
+
+template <typename T, int DIR, bool LORA>
+cudaError_t launch_small(const GroupedArgs& g, const LoraTerm* lora, int num_sms, cudaStream_t s) {
+  const int feat = DIR == kGmmForward ? g.N : g.K;
+  SmallParams p{};
+  p.offsets = g.offsets;
+  p.total_rows = g.rows;
+  p.E = g.E;
+  p.m_dim = feat;
+  p.con = DIR == kGmmForward ? g.K : g.N;
+  p.m_tiles = (feat + kTileM - 1) / kTileM;
+  p.out = g.out;
+  p.ldo = feat;
+  if (lora != nullptr) p.lora = *lora;
+  // Tile cap: twice the mean rows per group (uneven groups then mostly stay one tile, and
+  // their weights are streamed once), all of them when there is one group.
+  const int64_t want = g.E == 1 ? g.rows : 2 * ((g.rows + g.E - 1) / g.E);
+  p.cap = 16;
+  while (p.cap < 256 && p.cap < want) p.cap *= 2;
+  p.box = std::min(p.cap, 64);
+  p.stage_bytes = kWBytes + p.cap * kBK * 2;
+  // Ring: two CTAs an SM up to 128 rows, one CTA with all of the memory at 256.
+  const int budget = p.cap <= 128 ? 108 * 1024 : 220 * 1024;
+  p.stages = std::min(kMaxStages, (budget - kFixed) / p.stage_bytes);
+  p.tmem_cols = static_cast<uint32_t>(std::max(32, p.cap));
+  const int64_t tiles = (g.rows / p.cap + std::min<int64_t>(g.rows, g.E)) * p.m_tiles;
+  // Splits: until the grid holds every SM's resident CTAs, with at least two slices each.
+  const int64_t fill = static_cast<int64_t>(num_sms) * (p.cap <= 128 ? 2 : 1);
+  const int slices = (p.con + kBK - 1) / kBK;
+  p.splits = 1;
+  while (p.splits < 8 && tiles * p.splits * 2 <= fill && slices >= 4 * p.splits) p.splits *= 2;
+
+  CUtensorMap mw, mx;
+  if (!grouped_map(&mw, g.dtype, g.w, g.K, g.N, g.E, DIR == kGmmForward ? 128 : 64) ||
+      !grouped_map(&mx, g.dtype, DIR == kGmmForward ? g.x : g.dy, p.con, g.rows, 1, p.box))
+    return cudaErrorInvalidValue;
+  const int smem = kFixed + p.stages * p.stage_bytes;
+  static SmemOptIn opt_in;
+  cudaError_t st = opt_in.set(grouped_small_kernel<T, DIR, LORA>, 227 * 1024);
+  if (st != cudaSuccess) return st;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.splits));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  int na = 0;
+  attr[na].id = cudaLaunchAttributeClusterDimension;
+  attr[na].val.clusterDim.x = p.splits;
+  attr[na].val.clusterDim.y = 1;
+  attr[na].val.clusterDim.z = 1;
+  ++na;
+  if (LORA) {
+    attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[na].val.programmaticStreamSerializationAllowed = 1;
+    ++na;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = na;
+  return cudaLaunchKernelEx(&cfg, grouped_small_kernel<T, DIR, LORA>, mw, mx, p);
+}
+
+template <typename T>
+cudaError_t launch_small_type(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
+                              cudaStream_t s) {
+  if (lora != nullptr) return launch_small<T, kGmmForward, true>(g, lora, num_sms, s);
+  if (g.dir == kGmmForward) return launch_small<T, kGmmForward, false>(g, nullptr, num_sms, s);
+  return launch_small<T, kGmmGradInput, false>(g, nullptr, num_sms, s);
+}
+
+}  // namespace
+
+cudaError_t launch_grouped_small(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
+                                 cudaStream_t s) {
+  if (g.dir == kGmmGradWeight) return cudaErrorInvalidValue;
+  if (g.dtype == kDtF16) return launch_small_type<__half>(g, lora, num_sms, s);
+  if (g.dtype == kDtBF16) return launch_small_type<__nv_bfloat16>(g, lora, num_sms, s);
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t take_grouped_small_error(int* err) {
+  cudaError_t st = cudaMemcpyFromSymbol(err, g_small_error, sizeof(int));
+  if (st != cudaSuccess || *err == 0) return st;
+  const int zero = 0;
+  return cudaMemcpyToSymbol(g_small_error, &zero, sizeof(int));
+}
+
+}  // namespace moe

@@ -23,7 +23,7 @@
 #include <algorithm>
 #include <mutex>
 
-#include "grouped_tc.cuh"
+#include "grouped_lora.cuh"
 
 namespace moe {
 
@@ -60,6 +60,7 @@ struct PairParams {
   int m_tiles, n_tiles;
   void* out;
   int64_t ldo;
+  LoraTerm lora;
 };
 
 struct PairTile {
@@ -128,7 +129,7 @@ __device__ __forceinline__ bool is_tail(const PairTile& t, int b) {
   return t.cnt % kTailRows != 0 && b == t.blocks - 1;
 }
 
-template <typename T, int DIR>
+template <typename T, int DIR, bool LORA>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
                     const __grid_constant__ CUtensorMap map_b,
@@ -177,7 +178,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
     tmem_alloc_pair(tmem_slot, 2 * kTileN);
     tmem_relinquish_pair();
   }
-  pdl_wait();  // grad_weight: the padded tails are written by the launch before
+  // The launch before wrote the padded tails (grad_weight) or writes t, which only the
+  // epilogue reads (the adapter projection).
+  if (!LORA) pdl_wait();
   if (warp == 2) build_group_table(p.offsets, p.E, p.rows, kTileN, table);
   tc_fence_before();
   __syncthreads();
@@ -303,6 +306,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
     const uint8_t* rd_ptr = buf + rd_row * kStageRow + ((rd_blk ^ ((rd_row >> 1) & 3)) << 4);
     T* out = static_cast<T*>(p.out);
     int i = 0;
+    if (LORA) pdl_wait();
     for (int L = pair; L < total && !*abort_flag; L += npairs, ++i) {
       const PairTile t = pair_tile<DIR>(L, table, p);
       const int acc = i & 1;
@@ -330,6 +334,14 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
           const int sel = (j & 1) * 8 * kStageRow;
           T* dst;
           bool ok;
+          if (LORA && c + 8 * j < t.n) {
+            float dl[4], dh[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { dl[k] = lo[4 * j + k]; dh[k] = hi[4 * j + k]; }
+            lora_add<T>(p.lora, p.rows, t.n0 + c + 8 * j, t.n0 + t.n, m, p.m_dim, dl, dh);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { lo[4 * j + k] = dl[k]; hi[4 * j + k] = dh[k]; }
+          }
           if (DIR == kGmmGradWeight) {
             // Eight M rows (block j of the 32) x 32 columns.
             const float(&v)[16] = j < 2 ? lo : hi;
@@ -416,16 +428,16 @@ size_t tail_bytes(int64_t E, int64_t width) {
   return (static_cast<size_t>(E) * kTailRows * static_cast<size_t>(width) * 2 + 255) & ~size_t{255};
 }
 
-template <typename T, int DIR>
-cudaError_t launch_pair(const GroupedArgs& g, int num_sms, cudaStream_t s) {
+template <typename T, int DIR, bool LORA>
+cudaError_t launch_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms, cudaStream_t s) {
   CUtensorMap ma, mb, mat, mbt;
   PairParams p{};
   p.offsets = g.offsets;
   p.rows = static_cast<int>(g.rows);
   p.E = g.E;
   p.out = g.out;
+  if (LORA) p.lora = *lora;
   bool ok;
-  int64_t tiles;
   if (DIR == kGmmGradWeight) {
     auto* ty = static_cast<uint8_t*>(g.workspace);
     uint8_t* tx = ty + tail_bytes(g.E, g.N);
@@ -457,23 +469,26 @@ cudaError_t launch_pair(const GroupedArgs& g, int num_sms, cudaStream_t s) {
     mbt = mb;
   }
   p.m_tiles = (p.m_dim + kTileM - 1) / kTileM;
-  tiles = DIR == kGmmGradWeight
+  const int64_t tiles =
+          DIR == kGmmGradWeight
               ? static_cast<int64_t>(g.E) * p.m_tiles * p.n_tiles
               : (g.rows / kTileN + std::min<int64_t>(g.rows, g.E)) * p.m_tiles;
   static SmemOptIn opt_in;
-  cudaError_t st = opt_in.set(grouped_pair_kernel<T, DIR>, kSmem);
+  cudaError_t st = opt_in.set(grouped_pair_kernel<T, DIR, LORA>, kSmem);
   if (st != cudaSuccess) return st;
   const int64_t pairs = std::min<int64_t>(tiles, num_sms / 2);
-  return launch_dependent(DIR == kGmmGradWeight, grouped_pair_kernel<T, DIR>,
+  return launch_dependent(DIR == kGmmGradWeight || LORA, grouped_pair_kernel<T, DIR, LORA>,
                           dim3(static_cast<unsigned>(2 * pairs)), dim3(kThreads), kSmem, s, ma, mb,
                           mat, mbt, p);
 }
 
 template <typename T>
-cudaError_t launch_pair_type(const GroupedArgs& g, int num_sms, cudaStream_t s) {
-  if (g.dir == kGmmForward) return launch_pair<T, kGmmForward>(g, num_sms, s);
-  if (g.dir == kGmmGradInput) return launch_pair<T, kGmmGradInput>(g, num_sms, s);
-  return launch_pair<T, kGmmGradWeight>(g, num_sms, s);
+cudaError_t launch_pair_type(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
+                             cudaStream_t s) {
+  if (lora != nullptr) return launch_pair<T, kGmmForward, true>(g, lora, num_sms, s);
+  if (g.dir == kGmmForward) return launch_pair<T, kGmmForward, false>(g, nullptr, num_sms, s);
+  if (g.dir == kGmmGradInput) return launch_pair<T, kGmmGradInput, false>(g, nullptr, num_sms, s);
+  return launch_pair<T, kGmmGradWeight, false>(g, nullptr, num_sms, s);
 }
 
 }  // namespace
@@ -506,9 +521,10 @@ bool grouped_tc_supported(const GroupedArgs& g) {
   return aligned(g.x) && aligned(g.dy) && aligned(g.w) && aligned(g.out);
 }
 
-cudaError_t launch_grouped_pair(const GroupedArgs& g, int num_sms, cudaStream_t s) {
-  if (g.dtype == kDtF16) return launch_pair_type<__half>(g, num_sms, s);
-  if (g.dtype == kDtBF16) return launch_pair_type<__nv_bfloat16>(g, num_sms, s);
+cudaError_t launch_grouped_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
+                                cudaStream_t s) {
+  if (g.dtype == kDtF16) return launch_pair_type<__half>(g, lora, num_sms, s);
+  if (g.dtype == kDtBF16) return launch_pair_type<__nv_bfloat16>(g, lora, num_sms, s);
   return cudaErrorInvalidValue;
 }
 

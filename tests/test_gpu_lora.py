@@ -75,7 +75,9 @@ def test_lora_matches_float64(pkg, orc, dev, dtype_name, T, N, K, r, L, kind):
 @pytest.mark.parametrize("dtype_name", ["float16", "bfloat16"])
 @pytest.mark.parametrize("T,N,K,r,L,kind", [
     (1, 4096, 4096, 16, 8, "one"), (64, 1024, 4096, 16, 32, "mixed"), (64, 1032, 2056, 64, 64, "mixed"),
-    (300, 1024, 2048, 16, 6, "runs"), (1100, 2048, 1024, 64, 5, "runs"), (1025, 520, 1032, 8, 100, "mixed")])
+    (300, 1024, 2048, 16, 6, "runs"), (1100, 2048, 1024, 64, 5, "runs"), (1025, 520, 1032, 8, 100, "mixed"),
+    (1500, 2568, 520, 16, 7, "runs"), (1300, 2560, 264, 24, 9, "mixed"), (3001, 1544, 136, 136, 4, "runs"),
+    (1281, 2816, 72, 8, 3, "foreign")])
 def test_larger_lora(pkg, orc, dev, dtype_name, T, N, K, r, L, kind):
     rng = np.random.default_rng(3)
     d = make(dev, T, N, K, r, L, dtype_name, ids_of(kind, T, L, rng), seed=1)
