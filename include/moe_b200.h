@@ -357,8 +357,8 @@ int moe_b200_grouped_matmul_grad_weight(int32_t dtype, int64_t num_rows, int64_t
  * a multiple of 8 for the tensor cores).  `workspace`: 256-byte aligned, at least
  * moe_b200_lora_matmul_workspace_size bytes, not shared by calls that may overlap.
  * No counterpart in the reference. */
-int moe_b200_lora_matmul_workspace_size(int32_t dtype, int64_t num_rows, int64_t k,
-                                        int64_t rank, size_t* bytes);
+int moe_b200_lora_matmul_workspace_size(int32_t dtype, int64_t num_rows, int64_t rank,
+                                        size_t* bytes);
 int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
                          int64_t num_adapters, int64_t rank, const void* x, const void* weight,
                          const void* lora_a, const void* lora_b, const int32_t* adapter_ids,

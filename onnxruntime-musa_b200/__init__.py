@@ -162,7 +162,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         ctypes.c_int, [_I32, _I64, _I64, _I64, ctypes.POINTER(_SZ)]),
     "moe_b200_grouped_matmul_grad_weight": (ctypes.c_int, [_I32, _I64, _I64, _I64, _I64, _VP, _VP,
                                                            _VP, _VP, _VP, _SZ, _VP]),
-    "moe_b200_lora_matmul_workspace_size": (ctypes.c_int, [_I32, _I64, _I64, _I64,
+    "moe_b200_lora_matmul_workspace_size": (ctypes.c_int, [_I32, _I64, _I64,
                                                            ctypes.POINTER(_SZ)]),
     "moe_b200_lora_matmul": (ctypes.c_int, [_I32, _I64, _I64, _I64, _I64, _I64, _VP, _VP, _VP, _VP,
                                             _VP, _VP, _VP, _VP, _SZ, _VP]),
@@ -924,7 +924,7 @@ def lora_matmul(x, weight, lora_a, lora_b, adapter_ids, scales, out=None, stream
         ("scales", scales, (L,), torch.float32)), out, (T, N))
     dt = elem_type_of(x)
     nbytes = _SZ()
-    check(lib().moe_b200_lora_matmul_workspace_size(dt, T, K, r, ctypes.byref(nbytes)))
+    check(lib().moe_b200_lora_matmul_workspace_size(dt, T, r, ctypes.byref(nbytes)))
     with _On(stream, (x, weight, lora_a, lora_b, adapter_ids, scales, out)) as s:
         if out is None:
             out = torch.empty((T, N), dtype=x.dtype, device=x.device)

@@ -29,13 +29,18 @@ struct GroupedArgs {
 
 // The adapter term of lora_matmul, added to the forward product of one group.
 struct LoraTerm {
-  const float* t;         // [splits][rows][rank]: partial sums of A_a x over K
-  int splits;
   int rank;               // r
   int adapters;           // L
   const void* b;          // [L, N, r]
   const int32_t* ids;     // [rows]; outside [0, L): no adapter
-  const float* scales;    // [L]
+  // FFMA kernels: t = A_a x in fp32, [rows][rank], and the adapters' scales [L].
+  const float* t;
+  const float* scales;
+  // Tensor-core kernels: s_a t in 16-bit parts, [rows][steps][4], step = 16 rank entries
+  // (grouped_lora.cuh); fp16: the power of two that each row's parts are to be scaled by.
+  const uint4* packed;
+  int steps;              // ceil(rank / 16)
+  const float* row_scale;
 };
 
 // Largest feature and contraction length, and most rows, of a call (index arithmetic of
@@ -52,23 +57,22 @@ struct LoraShrink {
   const void* x;           // [rows, K]
   const void* a;           // [L, r, K]
   const int32_t* ids;
-  float* t;                // [splits][rows][rank]
-  int splits;
+  const float* scales;     // [L]
 };
-cudaError_t launch_lora_shrink_simt(const LoraShrink& l, cudaStream_t s);  // splits = 1
-
-// The tensor-core form (16-bit types, K and rank multiples of 8, 16-byte aligned x and a)
-// leaves `splits` partial sums.
-int lora_shrink_splits(int64_t rows, int K);
+// Any type and alignment: t in fp32, [rows][rank].
+cudaError_t launch_lora_shrink_simt(const LoraShrink& l, float* t, cudaStream_t s);
+// 16-bit types, K and rank multiples of 8, 16-byte aligned x and a: the parts of
+// LoraTerm::packed and its row_scale.
 bool lora_shrink_tc_supported(const LoraShrink& l);
-cudaError_t launch_lora_shrink_tc(const LoraShrink& l, cudaStream_t s);
+cudaError_t launch_lora_shrink_tc(const LoraShrink& l, uint4* packed, float* row_scale,
+                                  int num_sms, cudaStream_t s);
 
 // Tensor-core path: 16-bit types, N and K multiples of 8, 16-byte aligned buffers.
 bool grouped_tc_supported(const GroupedArgs& g);
 size_t grouped_tc_workspace(int dtype, GroupedDir dir, int64_t N, int64_t K, int64_t E);
 // 256 x 256 tiles by CTA pairs, and weight streaming for few rows per group (not
-// grad_weight).  `lora` (forward, one group, rank % 8 == 0) may be nullptr; t is then
-// awaited with pdl_wait().
+// grad_weight).  `lora` (forward, one group, rank % 8 == 0) may be nullptr; its parts
+// are awaited with pdl_wait().
 cudaError_t launch_grouped_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
                                 cudaStream_t s);
 cudaError_t launch_grouped_small(const GroupedArgs& g, const LoraTerm* lora, int num_sms,

@@ -1,5 +1,6 @@
 // C entries of the expert products (moe_b200_grouped_matmul*) and the adapter projection
 // (moe_b200_lora_matmul): argument checks and the choice of kernel.
+#include <atomic>
 #include <cstdlib>
 
 #include "../../include/moe_b200.h"
@@ -53,10 +54,14 @@ int check_pointers(const char* what, int32_t dtype, const void* const* ptrs, int
 }
 
 int sm_count() {
+  static std::atomic<int> counts[64];
   int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  n = counts[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    counts[dev].store(n, std::memory_order_relaxed);
+  }
   return n;
 }
 
@@ -100,9 +105,13 @@ int run_grouped(const char* what, const moe::GroupedArgs& g, cudaStream_t s) {
   return rc != MOE_B200_OK ? rc : finish(what, s);
 }
 
-size_t lora_bytes(int32_t dtype, int64_t rows, int64_t k, int64_t rank) {
-  const int64_t splits = dtype == moe::kDtF32 ? 1 : moe::lora_shrink_splits(rows, static_cast<int>(k));
-  return static_cast<size_t>(rows * splits) * static_cast<size_t>(rank) * sizeof(float);
+// Workspace of lora_matmul: 64 bytes per row and 16 rank entries (the packed parts, or t in
+// fp32), then a float per row.
+size_t lora_parts_bytes(int64_t rows, int64_t rank) {
+  return static_cast<size_t>(rows) * static_cast<size_t>((rank + 15) / 16) * 64;
+}
+size_t lora_bytes(int64_t rows, int64_t rank) {
+  return lora_parts_bytes(rows, rank) + static_cast<size_t>(rows) * sizeof(float);
 }
 
 }  // namespace
@@ -214,14 +223,14 @@ int moe_b200_grouped_matmul_grad_weight(int32_t dtype, int64_t num_rows, int64_t
   return run_grouped(kWhat, g, s);
 }
 
-int moe_b200_lora_matmul_workspace_size(int32_t dtype, int64_t num_rows, int64_t k,
-                                        int64_t rank, size_t* bytes) {
+int moe_b200_lora_matmul_workspace_size(int32_t dtype, int64_t num_rows, int64_t rank,
+                                        size_t* bytes) {
   static const char* kWhat = "lora_matmul_workspace_size";
-  int rc = check_shape(kWhat, dtype, num_rows, 1, k, rank, "rank", moe::kLoraMaxRank);
+  int rc = check_shape(kWhat, dtype, num_rows, 1, 1, rank, "rank", moe::kLoraMaxRank);
   if (rc != MOE_B200_OK) return rc;
   if (bytes == nullptr)
     return set_error(MOE_B200_INVALID_ARGUMENT, "%s: bytes must be non-NULL", kWhat);
-  *bytes = lora_bytes(dtype, num_rows, k, rank);
+  *bytes = lora_bytes(num_rows, rank);
   return MOE_B200_OK;
 }
 
@@ -243,7 +252,7 @@ int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
   const void* words[] = {adapter_ids, scales};
   rc = check_pointers(kWhat, dtype, ptrs, 5, words, 2);
   if (rc != MOE_B200_OK) return rc;
-  const size_t need = lora_bytes(dtype, num_rows, k, rank);
+  const size_t need = lora_bytes(num_rows, rank);
   if (workspace_bytes < need || workspace == nullptr ||
       reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
     return set_error(MOE_B200_INVALID_ARGUMENT,
@@ -258,7 +267,7 @@ int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
   l.x = x;
   l.a = lora_a;
   l.ids = adapter_ids;
-  l.t = static_cast<float*>(workspace);
+  l.scales = scales;
   moe::GroupedArgs g{};
   g.dtype = dtype;
   g.dir = moe::kGmmForward;
@@ -271,18 +280,28 @@ int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
   g.out = y;
   const bool a16 = (reinterpret_cast<uintptr_t>(lora_b) & 15) == 0;
   const bool tc = moe::grouped_tc_supported(g) && moe::lora_shrink_tc_supported(l) && a16;
-  l.splits = tc ? moe::lora_shrink_splits(num_rows, l.K) : 1;
-  rc = cuda_status(tc ? moe::launch_lora_shrink_tc(l, s) : moe::launch_lora_shrink_simt(l, s),
-                   kWhat);
-  if (rc != MOE_B200_OK) return rc;
   moe::LoraTerm term{};
-  term.t = l.t;
-  term.splits = l.splits;
   term.rank = l.rank;
   term.adapters = l.adapters;
   term.b = lora_b;
   term.ids = adapter_ids;
-  term.scales = scales;
+  cudaError_t st;
+  if (tc) {
+    auto* packed = static_cast<uint4*>(workspace);
+    auto* row_scale = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
+                                               lora_parts_bytes(num_rows, rank));
+    st = moe::launch_lora_shrink_tc(l, packed, row_scale, sm_count(), s);
+    term.packed = packed;
+    term.steps = static_cast<int>((rank + 15) / 16);
+    term.row_scale = row_scale;
+  } else {
+    auto* t = static_cast<float*>(workspace);
+    st = moe::launch_lora_shrink_simt(l, t, s);
+    term.t = t;
+    term.scales = scales;
+  }
+  rc = cuda_status(st, kWhat);
+  if (rc != MOE_B200_OK) return rc;
   rc = cuda_status(tc ? launch_tc(g, &term, s) : moe::launch_grouped_simt(g, &term, s), kWhat);
   return rc != MOE_B200_OK ? rc : finish(kWhat, s);
 }

@@ -244,7 +244,7 @@ grouped_simt_kernel(const SimtParams p) {
     const int m = ty * 4 + (i / 4) * 64 + (i & 3);
     if (m >= nm) continue;
     if (DIR == kGmmForward && p.lora.t != nullptr) {
-      // y += s_a * sum_j t[row, j] B_a[n, j], the partial sums of t added in split order.
+      // y += s_a * sum_j t[row, j] B_a[n, j].
       const int row = row0 + m, ad = __ldg(p.lora.ids + row), r = p.lora.rank;
       if (ad >= 0 && ad < p.lora.adapters) {
         float d[TN];
@@ -252,9 +252,7 @@ grouped_simt_kernel(const SimtParams p) {
         for (int j = 0; j < TN; ++j) d[j] = 0.f;
         const T* bb = static_cast<const T*>(p.lora.b) + static_cast<int64_t>(ad) * p.N * r;
         for (int q = 0; q < r; ++q) {
-          float t = 0.f;
-          for (int sp = 0; sp < p.lora.splits; ++sp)
-            t += __ldg(p.lora.t + (static_cast<int64_t>(sp) * p.rows + row) * r + q);
+          const float t = __ldg(p.lora.t + static_cast<int64_t>(row) * r + q);
 #pragma unroll
           for (int j = 0; j < TN; ++j) {
             const int n = tx * 4 + (j / 4) * 64 + (j & 3);

@@ -60,7 +60,7 @@ __device__ __forceinline__ void st_cluster_f4(uint32_t addr, const float (&v)[4]
                : "memory");
 }
 
-template <typename T, int DIR, bool LORA>
+template <typename T, int DIR, int LORA>
 __global__ void __launch_bounds__(kThreads)
 grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
                      const __grid_constant__ CUtensorMap map_x, const SmallParams p) {
@@ -206,7 +206,7 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
     }
     cluster_sync();
   }
-  if (LORA) pdl_wait();  // t comes from the launch before this one
+  if (LORA > 0) pdl_wait();  // t comes from the launch before this one
 
   uint8_t* buf = stage_out + warp * kEpiBytes;
   const int st_row = lane & 7, st_blk = lane >> 3;
@@ -215,8 +215,16 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
   const int rd_row = lane >> 2, rd_blk = lane & 3;
   const uint8_t* rd_ptr = buf + rd_row * kStageRow + ((rd_blk ^ ((rd_row >> 1) & 3)) << 4);
   const int feat = m0 + q * 32;
+  LoraFrags<LORA == 0 ? 1 : LORA> frags;
   for (int i = pair; i * S + split < blocks; i += 2) {
     const int b = i * S + split;
+    int ad = -1;
+    uint4 parts[LORA == 0 ? 1 : LORA];
+    if constexpr (LORA > 0) {
+      const int row = 8 * b + (lane >> 2);
+      ad = lora_adapter(p.lora, row0 + row, row < n);
+      lora_rows<LORA>(p.lora, row0 + row, row < n, 0, parts);
+    }
     float lo[4] = {0.f, 0.f, 0.f, 0.f}, hi[4] = {0.f, 0.f, 0.f, 0.f};
     float own_lo[4] = {0.f, 0.f, 0.f, 0.f}, own_hi[4] = {0.f, 0.f, 0.f, 0.f};
     if (!empty_part) {
@@ -237,7 +245,8 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
         hi[0] += c.x; hi[1] += c.y; hi[2] += c.z; hi[3] += c.w;
       }
     }
-    if (LORA) lora_add<T>(p.lora, p.total_rows, row0 + 8 * b, row0 + n, feat, p.m_dim, lo, hi);
+    if constexpr (LORA > 0)
+      lora_add<T, LORA>(p.lora, ad, row0 + 8 * b + (lane >> 2), feat, p.m_dim, parts, frags, lo, hi);
     stmatrix4_t(st_addr, pack2<T>(lo[0], lo[1]), pack2<T>(lo[2], lo[3]), pack2<T>(hi[0], hi[1]),
                 pack2<T>(hi[2], hi[3]));
     __syncwarp();
@@ -256,7 +265,7 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
   }
 }
 
-template <typename T, int DIR, bool LORA>
+template <typename T, int DIR, int LORA>
 cudaError_t launch_small(const GroupedArgs& g, const LoraTerm* lora, int num_sms, cudaStream_t s) {
   const int feat = DIR == kGmmForward ? g.N : g.K;
   SmallParams p{};
@@ -307,7 +316,7 @@ cudaError_t launch_small(const GroupedArgs& g, const LoraTerm* lora, int num_sms
   attr[na].val.clusterDim.y = 1;
   attr[na].val.clusterDim.z = 1;
   ++na;
-  if (LORA) {
+  if (LORA > 0) {
     attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[na].val.programmaticStreamSerializationAllowed = 1;
     ++na;
@@ -320,9 +329,12 @@ cudaError_t launch_small(const GroupedArgs& g, const LoraTerm* lora, int num_sms
 template <typename T>
 cudaError_t launch_small_type(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
                               cudaStream_t s) {
-  if (lora != nullptr) return launch_small<T, kGmmForward, true>(g, lora, num_sms, s);
-  if (g.dir == kGmmForward) return launch_small<T, kGmmForward, false>(g, nullptr, num_sms, s);
-  return launch_small<T, kGmmGradInput, false>(g, nullptr, num_sms, s);
+  // Ranks up to 16 keep one step in registers, larger ones blocks of four.
+  if (lora != nullptr)
+    return lora->steps == 1 ? launch_small<T, kGmmForward, 1>(g, lora, num_sms, s)
+                            : launch_small<T, kGmmForward, 4>(g, lora, num_sms, s);
+  if (g.dir == kGmmForward) return launch_small<T, kGmmForward, 0>(g, nullptr, num_sms, s);
+  return launch_small<T, kGmmGradInput, 0>(g, nullptr, num_sms, s);
 }
 
 }  // namespace

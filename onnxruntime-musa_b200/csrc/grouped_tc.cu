@@ -129,7 +129,8 @@ __device__ __forceinline__ bool is_tail(const PairTile& t, int b) {
   return t.cnt % kTailRows != 0 && b == t.blocks - 1;
 }
 
-template <typename T, int DIR, bool LORA>
+// LORA: 16-entry steps of the rank per register block of the adapter term, 0 without one.
+template <typename T, int DIR, int LORA>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
                     const __grid_constant__ CUtensorMap map_b,
@@ -180,7 +181,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
   }
   // The launch before wrote the padded tails (grad_weight) or writes t, which only the
   // epilogue reads (the adapter projection).
-  if (!LORA) pdl_wait();
+  if (LORA == 0) pdl_wait();
   if (warp == 2) build_group_table(p.offsets, p.E, p.rows, kTileN, table);
   tc_fence_before();
   __syncthreads();
@@ -306,7 +307,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
     const uint8_t* rd_ptr = buf + rd_row * kStageRow + ((rd_blk ^ ((rd_row >> 1) & 3)) << 4);
     T* out = static_cast<T*>(p.out);
     int i = 0;
-    if (LORA) pdl_wait();
+    if (LORA > 0) pdl_wait();
     for (int L = pair; L < total && !*abort_flag; L += npairs, ++i) {
       const PairTile t = pair_tile<DIR>(L, table, p);
       const int acc = i & 1;
@@ -319,7 +320,20 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
       const uint32_t taddr =
           tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * kTileN;
       const int m = t.m0 + static_cast<int>(rank) * 128 + q * 32;  // first M entry of the warp
+      LoraFrags<LORA == 0 ? 1 : LORA> frags;  // of this tile's features
       for (int c = first; c < t.n; c += 64) {
+        // The chunk's adapters and packed parts are fetched ahead of the accumulators: one
+        // trip to L2 a chunk instead of one a row block.
+        int ads = -1;
+        uint4 parts[4][LORA == 0 ? 1 : LORA];
+        if constexpr (LORA > 0) {
+          ads = lora_adapter(p.lora, t.n0 + c + lane, c + lane < t.n);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int row = c + 8 * j + (lane >> 2);
+            lora_rows<LORA>(p.lora, t.n0 + row, row < t.n, 0, parts[j]);
+          }
+        }
         float lo[16], hi[16];
         if (DIR == kGmmGradWeight && t.cnt == 0) {  // an expert without rows: zeros
 #pragma unroll
@@ -334,11 +348,12 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
           const int sel = (j & 1) * 8 * kStageRow;
           T* dst;
           bool ok;
-          if (LORA && c + 8 * j < t.n) {
+          if constexpr (LORA > 0) {
             float dl[4], dh[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) { dl[k] = lo[4 * j + k]; dh[k] = hi[4 * j + k]; }
-            lora_add<T>(p.lora, p.rows, t.n0 + c + 8 * j, t.n0 + t.n, m, p.m_dim, dl, dh);
+            lora_add<T, LORA>(p.lora, __shfl_sync(0xffffffffu, ads, 8 * j + (lane >> 2)),
+                              t.n0 + c + 8 * j + (lane >> 2), m, p.m_dim, parts[j], frags, dl, dh);
 #pragma unroll
             for (int k = 0; k < 4; ++k) { lo[4 * j + k] = dl[k]; hi[4 * j + k] = dh[k]; }
           }
@@ -428,7 +443,7 @@ size_t tail_bytes(int64_t E, int64_t width) {
   return (static_cast<size_t>(E) * kTailRows * static_cast<size_t>(width) * 2 + 255) & ~size_t{255};
 }
 
-template <typename T, int DIR, bool LORA>
+template <typename T, int DIR, int LORA>
 cudaError_t launch_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms, cudaStream_t s) {
   CUtensorMap ma, mb, mat, mbt;
   PairParams p{};
@@ -436,7 +451,7 @@ cudaError_t launch_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
   p.rows = static_cast<int>(g.rows);
   p.E = g.E;
   p.out = g.out;
-  if (LORA) p.lora = *lora;
+  if (LORA > 0) p.lora = *lora;
   bool ok;
   if (DIR == kGmmGradWeight) {
     auto* ty = static_cast<uint8_t*>(g.workspace);
@@ -477,7 +492,7 @@ cudaError_t launch_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
   cudaError_t st = opt_in.set(grouped_pair_kernel<T, DIR, LORA>, kSmem);
   if (st != cudaSuccess) return st;
   const int64_t pairs = std::min<int64_t>(tiles, num_sms / 2);
-  return launch_dependent(DIR == kGmmGradWeight || LORA, grouped_pair_kernel<T, DIR, LORA>,
+  return launch_dependent(DIR == kGmmGradWeight || LORA > 0, grouped_pair_kernel<T, DIR, LORA>,
                           dim3(static_cast<unsigned>(2 * pairs)), dim3(kThreads), kSmem, s, ma, mb,
                           mat, mbt, p);
 }
@@ -485,10 +500,13 @@ cudaError_t launch_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
 template <typename T>
 cudaError_t launch_pair_type(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
                              cudaStream_t s) {
-  if (lora != nullptr) return launch_pair<T, kGmmForward, true>(g, lora, num_sms, s);
-  if (g.dir == kGmmForward) return launch_pair<T, kGmmForward, false>(g, nullptr, num_sms, s);
-  if (g.dir == kGmmGradInput) return launch_pair<T, kGmmGradInput, false>(g, nullptr, num_sms, s);
-  return launch_pair<T, kGmmGradWeight, false>(g, nullptr, num_sms, s);
+  // Ranks up to 16 keep one step in registers, larger ones blocks of four.
+  if (lora != nullptr)
+    return lora->steps == 1 ? launch_pair<T, kGmmForward, 1>(g, lora, num_sms, s)
+                            : launch_pair<T, kGmmForward, 4>(g, lora, num_sms, s);
+  if (g.dir == kGmmForward) return launch_pair<T, kGmmForward, 0>(g, nullptr, num_sms, s);
+  if (g.dir == kGmmGradInput) return launch_pair<T, kGmmGradInput, 0>(g, nullptr, num_sms, s);
+  return launch_pair<T, kGmmGradWeight, 0>(g, nullptr, num_sms, s);
 }
 
 }  // namespace

@@ -9,9 +9,10 @@
 // adapters a pass), its rows are the N, and each column keeps the lanes of its own adapter:
 // rows need no sorting, and another adapter's values never reach a row.  One prompt in a
 // chunk is one pass; a decode chunk of 8 rows is at most 8 adapters, read once each.
-// Bound: the bytes of A_a (decode) and of x (prefill); the products are few.  The splits
-// leave partial sums that the epilogue of the projection adds in order, which costs it
-// splits * r floats a row and saves a join here.
+// Bound: the bytes of A_a (decode) and of x (prefill); the products are few.  The splits of
+// a chunk are a cluster: each leaves its partial sums in shared memory, and each row's are
+// added in rank order by one warp, which scales, splits and packs them as the epilogue of
+// the projection takes them (grouped_lora.cuh).
 #include <algorithm>
 
 #include "grouped_tc.cuh"
@@ -51,11 +52,16 @@ constexpr int kM = 128;
 constexpr int kABytes = kM * kBK * 2;
 constexpr int kMaxChunk = 64;
 constexpr int kTcStages = 4;
+// Largest dynamic shared memory: align slack, ring, partial sums, barriers.
+constexpr int kTcSmemMax = 1024 + kTcStages * (kABytes + kMaxChunk * kBK * 2) +
+                           kMaxChunk * kLoraMaxRank * 4 + 256;
 constexpr int kTcThreads = 256;   // warp 0 TMA, warp 1 MMA, warps 4..7 epilogue
 
 struct ShrinkParams {
   const int32_t* ids;
-  float* t;
+  const float* scales;
+  uint4* packed;
+  float* row_scale;
   int64_t rows;
   int K, rank, adapters;
   int chunk;      // rows of a CTA: 8 or 64
@@ -64,15 +70,34 @@ struct ShrinkParams {
   int stage_bytes;
 };
 
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+// Two 16-bit parts of each of four values, {hi, hi, lo, lo}.
+template <typename T>
+__device__ __forceinline__ uint4 pack_parts(const float4& v) {
+  const float h0 = to_f(from_f<T>(v.x)), h1 = to_f(from_f<T>(v.y));
+  const float h2 = to_f(from_f<T>(v.z)), h3 = to_f(from_f<T>(v.w));
+  return make_uint4(pack2<T>(h0, h1), pack2<T>(h2, h3), pack2<T>(v.x - h0, v.y - h1),
+                    pack2<T>(v.z - h2, v.w - h3));
+}
+
+template <typename T>
 __global__ void __launch_bounds__(kTcThreads)
 lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
-                      const __grid_constant__ CUtensorMap map_a, const uint32_t format,
-                      const ShrinkParams p) {
+                      const __grid_constant__ CUtensorMap map_a, const ShrinkParams p) {
   pdl_launch_dependents();  // the projection's main loop does not read t
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kTcStages * p.stage_bytes);
+  float* part = reinterpret_cast<float*>(ring + kTcStages * p.stage_bytes);  // [chunk][rank]
+  uint64_t* full = reinterpret_cast<uint64_t*>(part + p.chunk * p.rank);
   uint64_t* empty = full + kTcStages;
   uint64_t* tfull = empty + kTcStages;   // [2]
   uint64_t* tempty = tfull + 2;          // [2]
@@ -82,7 +107,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
   __shared__ int s_distinct;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = blockIdx.x % p.splits;
+  const int split = static_cast<int>(cluster_ctarank());
   const int64_t row0 = static_cast<int64_t>(blockIdx.x / p.splits) * p.chunk;
   const int n = static_cast<int>(min(static_cast<int64_t>(p.chunk), p.rows - row0));
 
@@ -175,7 +200,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      const uint32_t idesc = idesc_f16(format, kM, p.mma_n);
+      const uint32_t idesc = idesc_f16(TcFormat<T>::kId, kM, p.mma_n);
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -218,7 +243,6 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
       const int unit = ps * per + u;
       const int j = (unit % blocks_u) * kM + j0;
       const int slot = u < per && unit < units && j < p.rank ? unit / blocks_u : -2;
-      float* dst = p.t + (static_cast<int64_t>(split) * p.rows + row0) * p.rank + j;
       for (int c = 0; c < n; c += 16) {
         float v[16];
         tmem_ld16(tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * p.mma_n + c, v);
@@ -226,7 +250,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (c + i < n && s_slot[c + i] == slot)
-            dst[static_cast<int64_t>(c + i) * p.rank] = s0 < s1 ? v[i] : 0.f;
+            part[(c + i) * p.rank + j] = s0 < s1 ? v[i] : 0.f;
       }
       tc_fence_before();
       __syncwarp();
@@ -239,6 +263,48 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
     tc_fence_after();
     tmem_dealloc(tmem, tmem_cols);
   }
+  cluster_sync();  // every split's partial sums are in its `part`
+  // Row i of the chunk is finished by CTA i % splits, one warp a row; a lane takes granules
+  // of four entries.
+  const int steps = (p.rank + 15) / 16;
+  for (int i = split + p.splits * warp; i < n; i += p.splits * (kTcThreads / 32)) {
+    if (s_slot[i] < 0) continue;
+    const float sc = __ldg(p.scales + s_id[i]);
+    float4 v[2];
+    float m = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int j = 4 * (lane + 32 * h);
+      v[h] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (j < p.rank) {
+        const uint32_t at = smem_u32(part + i * p.rank + j);
+        for (int r = 0; r < p.splits; ++r) {
+          const float4 w = ld_cluster_f4(mapa_shared(at, r));
+          v[h].x += w.x; v[h].y += w.y; v[h].z += w.z; v[h].w += w.w;
+        }
+        v[h].x *= sc; v[h].y *= sc; v[h].z *= sc; v[h].w *= sc;
+      }
+      m = fmaxf(m, fmaxf(fmaxf(fabsf(v[h].x), fabsf(v[h].y)), fmaxf(fabsf(v[h].z), fabsf(v[h].w))));
+    }
+    if (std::is_same<T, __half>::value) {
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+      float down = 1.f;
+      if (m > 0.f && m < __int_as_float(0x7f800000)) {
+        const int e = min(max((__float_as_int(m) >> 23) - 127, -120), 120);
+        const float up = __int_as_float((127 - e) << 23);
+        down = __int_as_float((127 + e) << 23);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) { v[h].x *= up; v[h].y *= up; v[h].z *= up; v[h].w *= up; }
+      }
+      if (lane == 0) p.row_scale[row0 + i] = down;
+    }
+    uint4* dst = p.packed + (row0 + i) * steps * 4;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (lane + 32 * h < steps * 4) dst[lane + 32 * h] = pack_parts<T>(v[h]);
+  }
+  cluster_sync();  // no CTA leaves while another reads its part
 }
 
 // Rows of a CTA: small chunks spread a decode batch (whose rows follow many adapters) over
@@ -246,28 +312,61 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
 int shrink_chunk(int64_t rows) { return rows <= 256 ? 8 : kMaxChunk; }
 
 template <typename T>
-cudaError_t shrink_simt(const LoraShrink& l, cudaStream_t s) {
+cudaError_t shrink_simt(const LoraShrink& l, float* t, cudaStream_t s) {
   lora_shrink_simt_kernel<T><<<static_cast<unsigned>(l.rows), kWarps * 32, 0, s>>>(
-      static_cast<const T*>(l.x), static_cast<const T*>(l.a), l.ids, l.K, l.rank, l.adapters, l.t);
+      static_cast<const T*>(l.x), static_cast<const T*>(l.a), l.ids, l.K, l.rank, l.adapters, t);
   return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t shrink_tc(const LoraShrink& l, uint4* packed, float* row_scale, int num_sms,
+                      cudaStream_t s) {
+  ShrinkParams p{};
+  p.ids = l.ids;
+  p.scales = l.scales;
+  p.packed = packed;
+  p.row_scale = row_scale;
+  p.rows = l.rows;
+  p.K = l.K;
+  p.rank = l.rank;
+  p.adapters = l.adapters;
+  p.chunk = shrink_chunk(l.rows);
+  p.mma_n = std::max(p.chunk, 16);
+  p.stage_bytes = kABytes + p.mma_n * kBK * 2;
+  // Splits: until about two CTAs an SM run, with at least two slices of K each.
+  const int64_t chunks = (l.rows + p.chunk - 1) / p.chunk;
+  const int slices = (l.K + kBK - 1) / kBK;
+  p.splits = 1;
+  while (p.splits < 8 && chunks * p.splits <= num_sms && slices >= 4 * p.splits) p.splits *= 2;
+  CUtensorMap mx, ma;
+  if (!grouped_map(&mx, l.dtype, l.x, l.K, l.rows, 1, p.chunk) ||
+      !grouped_map(&ma, l.dtype, l.a, l.K, l.rank, l.adapters, std::min(l.rank, kM)))
+    return cudaErrorInvalidValue;
+  static SmemOptIn opt_in;
+  cudaError_t st = opt_in.set(lora_shrink_tc_kernel<T>, kTcSmemMax);
+  if (st != cudaSuccess) return st;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(chunks * p.splits));
+  cfg.blockDim = dim3(kTcThreads);
+  cfg.dynamicSmemBytes = 1024 + kTcStages * p.stage_bytes + p.chunk * p.rank * 4 + 256;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, lora_shrink_tc_kernel<T>, mx, ma, p);
 }
 
 }  // namespace
 
-cudaError_t launch_lora_shrink_simt(const LoraShrink& l, cudaStream_t s) {
-  if (l.dtype == kDtF32) return shrink_simt<float>(l, s);
-  if (l.dtype == kDtF16) return shrink_simt<__half>(l, s);
-  if (l.dtype == kDtBF16) return shrink_simt<__nv_bfloat16>(l, s);
+cudaError_t launch_lora_shrink_simt(const LoraShrink& l, float* t, cudaStream_t s) {
+  if (l.dtype == kDtF32) return shrink_simt<float>(l, t, s);
+  if (l.dtype == kDtF16) return shrink_simt<__half>(l, t, s);
+  if (l.dtype == kDtBF16) return shrink_simt<__nv_bfloat16>(l, t, s);
   return cudaErrorInvalidValue;
-}
-
-int lora_shrink_splits(int64_t rows, int K) {
-  // Until about two CTAs an SM run, with at least two slices of K each.
-  const int64_t chunks = (rows + shrink_chunk(rows) - 1) / shrink_chunk(rows);
-  const int slices = (K + kBK - 1) / kBK;
-  int splits = 1;
-  while (splits < 8 && chunks * splits * 2 <= 296 && slices >= 4 * splits) splits *= 2;
-  return splits;
 }
 
 bool lora_shrink_tc_supported(const LoraShrink& l) {
@@ -277,31 +376,11 @@ bool lora_shrink_tc_supported(const LoraShrink& l) {
   return aligned(l.x) && aligned(l.a);
 }
 
-cudaError_t launch_lora_shrink_tc(const LoraShrink& l, cudaStream_t s) {
-  ShrinkParams p{};
-  p.ids = l.ids;
-  p.t = l.t;
-  p.rows = l.rows;
-  p.K = l.K;
-  p.rank = l.rank;
-  p.adapters = l.adapters;
-  p.chunk = shrink_chunk(l.rows);
-  p.mma_n = std::max(p.chunk, 16);
-  p.splits = l.splits;
-  p.stage_bytes = kABytes + p.mma_n * kBK * 2;
-  CUtensorMap mx, ma;
-  if (!grouped_map(&mx, l.dtype, l.x, l.K, l.rows, 1, p.chunk) ||
-      !grouped_map(&ma, l.dtype, l.a, l.K, l.rank, l.adapters, std::min(l.rank, kM)))
-    return cudaErrorInvalidValue;
-  const int smem = 1024 + kTcStages * p.stage_bytes + 256;
-  static SmemOptIn opt_in;
-  cudaError_t st = opt_in.set(lora_shrink_tc_kernel,
-                              1024 + kTcStages * (kABytes + kMaxChunk * kBK * 2) + 256);
-  if (st != cudaSuccess) return st;
-  const int64_t ctas = (l.rows + p.chunk - 1) / p.chunk * p.splits;
-  lora_shrink_tc_kernel<<<static_cast<unsigned>(ctas), kTcThreads, smem, s>>>(
-      mx, ma, l.dtype == kDtBF16 ? 1u : 0u, p);
-  return cudaGetLastError();
+cudaError_t launch_lora_shrink_tc(const LoraShrink& l, uint4* packed, float* row_scale,
+                                  int num_sms, cudaStream_t s) {
+  if (l.dtype == kDtF16) return shrink_tc<__half>(l, packed, row_scale, num_sms, s);
+  if (l.dtype == kDtBF16) return shrink_tc<__nv_bfloat16>(l, packed, row_scale, num_sms, s);
+  return cudaErrorInvalidValue;
 }
 
 cudaError_t take_lora_error(int* err) {

@@ -72,12 +72,12 @@ def test_no_rows_is_no_work(pkg):
 def test_workspace_sizes(pkg):
     n = SZ()
     L = pkg.lib()
-    assert L.moe_b200_lora_matmul_workspace_size(pkg.BFLOAT16, 100, 16, 16, ctypes.byref(n)) == pkg.OK
+    assert L.moe_b200_lora_matmul_workspace_size(pkg.BFLOAT16, 100, 16, ctypes.byref(n)) == pkg.OK
     assert n.value >= 100 * 16 * 4
     assert _lora(pkg, rows=100, r=16, nbytes=n.value - 1) == pkg.INVALID_ARGUMENT
-    assert L.moe_b200_lora_matmul_workspace_size(pkg.BFLOAT16, 100, 16, 0, ctypes.byref(n)) == \
+    assert L.moe_b200_lora_matmul_workspace_size(pkg.BFLOAT16, 100, 0, ctypes.byref(n)) == \
         pkg.INVALID_ARGUMENT
-    assert L.moe_b200_lora_matmul_workspace_size(pkg.BFLOAT16, 100, 16, 16, None) == \
+    assert L.moe_b200_lora_matmul_workspace_size(pkg.BFLOAT16, 100, 16, None) == \
         pkg.INVALID_ARGUMENT
     f = L.moe_b200_grouped_matmul_grad_weight_workspace_size
     assert f(pkg.BFLOAT16, 64, 64, 8, ctypes.byref(n)) == pkg.OK
