@@ -767,74 +767,87 @@ def permute(expert_idx, num_experts: int, stream=None):
 
 # ------------------------------------------------------- expert products, adapters
 
-def _operands(what: str, like, named, out, out_shape):
-    """Checks of the operators below: contiguous CUDA tensors of one device, the dtype of
-    the first (or the one named) and the expected shape.  ``named``: (name, tensor, shape,
-    dtype or None) with -1 for a free dimension; ``out`` None or a tensor of
-    ``out_shape``."""
-    dev, dt = like.device, like.dtype
-    if not like.is_cuda:
-        raise ValueError(f"{what}: tensors must be contiguous CUDA tensors")
-    if out is not None:
-        named = (*named, ("out", out, out_shape, None))
-    for name, t, shape, want in named:
-        if t.device != dev or not t.is_contiguous():
-            raise ValueError(f"{what}: {name} must be a contiguous tensor on {dev}")
-        if t.dtype != (want or dt):
-            raise TypeError(f"{what}: {name} must be {want or dt}, not {t.dtype}")
-        if t.dim() != len(shape) or any(w >= 0 and w != d for w, d in zip(shape, t.shape)):
-            raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected "
-                             f"{tuple('*' if w < 0 else w for w in shape)}")
+# The checks below run on every call of operators that take a few microseconds on the GPU,
+# so the usual case is one chained comparison per tensor and the messages are composed only
+# once something is wrong.
+
+_DT: dict[Any, int] = {}   # torch dtype -> element type, filled on first use
+_LORA_BYTES: dict[tuple[int, int, int], int] = {}
+_GRAD_WEIGHT_BYTES: dict[tuple[int, int, int, int], int] = {}
 
 
-class _On:
-    """Runs an operator on ``stream`` (None: the current stream of the tensors' device) of
-    the tensors' device: outputs and workspaces come from that stream's allocator pool, and
-    inputs used on a stream other than the current one are marked as in use there."""
-
-    __slots__ = ("handle", "_dev", "_ctx")
-
-    def __init__(self, stream, tensors):
+def _dt_code(what: str, dtype) -> int:
+    code = _DT.get(dtype)
+    if code is None:
         torch = _torch()
-        dev = tensors[0].device
-        self._dev = self._ctx = None
-        if dev.index != torch.cuda.current_device():
-            self._dev = torch.cuda.device(dev)
-            self._dev.__enter__()
-        if stream is None:
-            self.handle = torch.cuda.current_stream(dev).cuda_stream
-            return
-        if isinstance(stream, int):
-            stream = torch.cuda.ExternalStream(stream, device=dev) if stream else \
-                torch.cuda.default_stream(dev)
-        self.handle = stream.cuda_stream
-        if self.handle != torch.cuda.current_stream(dev).cuda_stream:
-            for t in tensors:
-                if t is not None:
-                    t.record_stream(stream)
-            self._ctx = torch.cuda.stream(stream)
-            self._ctx.__enter__()
+        if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise TypeError(f"{what}: unsupported dtype {dtype}")
+        code = _DT[dtype] = {torch.float32: FLOAT, torch.float16: FLOAT16,
+                             torch.bfloat16: BFLOAT16}[dtype]
+    return code
+
+
+def _require(what: str, name: str, t, shape: tuple, dtype, dev) -> None:
+    """``t`` is a contiguous tensor of this shape and dtype on ``dev``."""
+    if t.shape == shape and t.dtype is dtype and t.device == dev and t.is_contiguous():
+        return
+    if t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be a contiguous tensor on {dev}")
+    if t.dtype is not dtype:
+        raise TypeError(f"{what}: {name} must be {dtype}, not {t.dtype}")
+    raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {shape}")
+
+
+def _dims(what: str, name: str, t, n: int):
+    shape = t.shape
+    if len(shape) != n:
+        raise ValueError(f"{what}: {name} must have {n} dimensions, not {len(shape)}")
+    return shape
+
+
+def _device_of(what: str, t):
+    if not t.is_cuda:
+        raise ValueError(f"{what}: tensors must be contiguous CUDA tensors")
+    return t.device
+
+
+class _Elsewhere:
+    """A call on another device than the current one, or on a stream of the caller's: the
+    device and stream are current inside (outputs and workspaces then come from that
+    stream's allocator pool), and tensors that come from another stream are marked as in use
+    on this one."""
+
+    def __init__(self, stream, dev, tensors):
+        torch = _torch()
+        self._ctx = [torch.cuda.device(dev)]
+        if stream is not None:
+            if isinstance(stream, int):
+                stream = torch.cuda.ExternalStream(stream, device=dev) if stream else \
+                    torch.cuda.default_stream(dev)
+            if stream.device != dev:
+                raise ValueError(f"stream of {stream.device} for tensors on {dev}")
+            if stream != torch.cuda.current_stream(dev):
+                for t in tensors:
+                    if t is not None:
+                        t.record_stream(stream)
+            self._ctx.append(torch.cuda.stream(stream))
 
     def __enter__(self):
-        return self.handle
+        for c in self._ctx:
+            c.__enter__()
 
     def __exit__(self, *exc):
-        if self._ctx is not None:
-            self._ctx.__exit__(*exc)
-        if self._dev is not None:
-            self._dev.__exit__(*exc)
+        for c in reversed(self._ctx):
+            c.__exit__(*exc)
 
 
-def _rank2(what: str, name: str, t) -> tuple[int, int]:
-    if t.dim() != 2:
-        raise ValueError(f"{what}: {name} must have 2 dimensions, not {t.dim()}")
-    return t.shape
-
-
-def _rank3(what: str, name: str, t) -> tuple[int, int, int]:
-    if t.dim() != 3:
-        raise ValueError(f"{what}: {name} must have 3 dimensions, not {t.dim()}")
-    return t.shape
+def _current_stream(dev) -> int | None:
+    """The current stream of ``dev`` if it is the current device, else None.  (The raw-handle
+    query: building a Stream object takes 3 us, a third of a small call.)"""
+    torch = _torch()
+    if dev.index != torch.cuda.current_device():
+        return None
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def grouped_matmul(x, weights, expert_offsets, out=None, stream=None):
@@ -845,36 +858,40 @@ def grouped_matmul(x, weights, expert_offsets, out=None, stream=None):
     [E, N, K], ``expert_offsets`` int32 [E + 1] on the device; returns [R, N] (``out`` if
     given).  Rows from ``expert_offsets[E]`` on are neither read nor written.  float32,
     float16 or bfloat16, fp32 sums."""
-    torch = _torch()
-    R, K = _rank2("grouped_matmul", "x", x)
-    E, N, _ = _rank3("grouped_matmul", "weights", weights)
-    _operands("grouped_matmul", x, (
-        ("x", x, (R, K), None), ("weights", weights, (E, N, K), None),
-        ("expert_offsets", expert_offsets, (E + 1,), torch.int32)), out, (R, N))
-    with _On(stream, (x, weights, expert_offsets, out)) as s:
-        if out is None:
-            out = torch.empty((R, N), dtype=x.dtype, device=x.device)
-        check(lib().moe_b200_grouped_matmul(
-            elem_type_of(x), R, N, K, E, x.data_ptr(), weights.data_ptr(),
-            expert_offsets.data_ptr(), out.data_ptr(), s))
-    return out
+    what = "grouped_matmul"
+    R, K = _dims(what, "x", x, 2)
+    E, N, _ = _dims(what, "weights", weights, 3)
+    return _product(what, lib().moe_b200_grouped_matmul, x, weights, expert_offsets, out, stream,
+                    R, N, K, E, K, N)
 
 
 def grouped_matmul_grad_input(dy, weights, expert_offsets, out=None, stream=None):
     """Gradient of :func:`grouped_matmul` with respect to ``x``:
     ``dx[p] = weights[e].T @ dy[p]``; ``dy`` [R, N], returns [R, K]."""
-    torch = _torch()
-    R, N = _rank2("grouped_matmul_grad_input", "dy", dy)
-    E, _, K = _rank3("grouped_matmul_grad_input", "weights", weights)
-    _operands("grouped_matmul_grad_input", dy, (
-        ("dy", dy, (R, N), None), ("weights", weights, (E, N, K), None),
-        ("expert_offsets", expert_offsets, (E + 1,), torch.int32)), out, (R, K))
-    with _On(stream, (dy, weights, expert_offsets, out)) as s:
-        if out is None:
-            out = torch.empty((R, K), dtype=dy.dtype, device=dy.device)
-        check(lib().moe_b200_grouped_matmul_grad_input(
-            elem_type_of(dy), R, N, K, E, dy.data_ptr(), weights.data_ptr(),
-            expert_offsets.data_ptr(), out.data_ptr(), s))
+    what = "grouped_matmul_grad_input"
+    R, N = _dims(what, "dy", dy, 2)
+    E, _, K = _dims(what, "weights", weights, 3)
+    return _product(what, lib().moe_b200_grouped_matmul_grad_input, dy, weights, expert_offsets,
+                    out, stream, R, N, K, E, N, K)
+
+
+def _product(what, entry, rows, weights, offsets, out, stream, R, N, K, E, width, out_width):
+    dev, dtype = _device_of(what, rows), rows.dtype
+    code = _dt_code(what, dtype)
+    _require(what, "rows", rows, (R, width), dtype, dev)
+    _require(what, "weights", weights, (E, N, K), dtype, dev)
+    _require(what, "expert_offsets", offsets, (E + 1,), _torch().int32, dev)
+    if out is not None:
+        _require(what, "out", out, (R, out_width), dtype, dev)
+    s = _current_stream(dev) if stream is None else None
+    if s is None:
+        with _Elsewhere(stream, dev, (rows, weights, offsets, out)):
+            return _product(what, entry, rows, weights, offsets, out, None, R, N, K, E, width,
+                            out_width)
+    if out is None:
+        out = rows.new_empty((R, out_width))
+    check(entry(code, R, N, K, E, rows.data_ptr(), weights.data_ptr(), offsets.data_ptr(),
+                out.data_ptr(), s))
     return out
 
 
@@ -882,26 +899,35 @@ def grouped_matmul_grad_weight(x, dy, expert_offsets, out=None, stream=None):
     """Gradient of :func:`grouped_matmul` with respect to the weights:
     ``dw[e] = sum_p outer(dy[p], x[p])`` over the rows of expert e (zeros if it has none);
     ``x`` [R, K], ``dy`` [R, N], returns [E, N, K]."""
-    torch = _torch()
-    R, K = _rank2("grouped_matmul_grad_weight", "x", x)
-    _, N = _rank2("grouped_matmul_grad_weight", "dy", dy)
-    if expert_offsets.dim() != 1 or expert_offsets.shape[0] < 2:
-        raise ValueError("grouped_matmul_grad_weight: expert_offsets must have E + 1 >= 2 entries")
-    E = expert_offsets.shape[0] - 1
-    _operands("grouped_matmul_grad_weight", x, (
-        ("x", x, (R, K), None), ("dy", dy, (R, N), None),
-        ("expert_offsets", expert_offsets, (E + 1,), torch.int32)), out, (E, N, K))
-    dt = elem_type_of(x)
-    nbytes = _SZ()
-    check(lib().moe_b200_grouped_matmul_grad_weight_workspace_size(dt, N, K, E,
-                                                                   ctypes.byref(nbytes)))
-    with _On(stream, (x, dy, expert_offsets, out)) as s:
-        if out is None:
-            out = torch.empty((E, N, K), dtype=x.dtype, device=x.device)
-        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=x.device)
-        check(lib().moe_b200_grouped_matmul_grad_weight(
-            dt, R, N, K, E, x.data_ptr(), dy.data_ptr(), expert_offsets.data_ptr(),
-            out.data_ptr(), ws.data_ptr(), nbytes.value, s))
+    what = "grouped_matmul_grad_weight"
+    R, K = _dims(what, "x", x, 2)
+    _, N = _dims(what, "dy", dy, 2)
+    E = _dims(what, "expert_offsets", expert_offsets, 1)[0] - 1
+    if E < 1:
+        raise ValueError(f"{what}: expert_offsets must have E + 1 >= 2 entries")
+    dev, dtype = _device_of(what, x), x.dtype
+    code = _dt_code(what, dtype)
+    _require(what, "x", x, (R, K), dtype, dev)
+    _require(what, "dy", dy, (R, N), dtype, dev)
+    _require(what, "expert_offsets", expert_offsets, (E + 1,), _torch().int32, dev)
+    if out is not None:
+        _require(what, "out", out, (E, N, K), dtype, dev)
+    s = _current_stream(dev) if stream is None else None
+    if s is None:
+        with _Elsewhere(stream, dev, (x, dy, expert_offsets, out)):
+            return grouped_matmul_grad_weight(x, dy, expert_offsets, out)
+    L = lib()
+    nbytes = _GRAD_WEIGHT_BYTES.get((code, N, K, E))
+    if nbytes is None:
+        n = _SZ()
+        check(L.moe_b200_grouped_matmul_grad_weight_workspace_size(code, N, K, E, ctypes.byref(n)))
+        nbytes = _GRAD_WEIGHT_BYTES[code, N, K, E] = n.value
+    if out is None:
+        out = x.new_empty((E, N, K))
+    ws = x.new_empty((nbytes,), dtype=_torch().uint8)
+    check(L.moe_b200_grouped_matmul_grad_weight(
+        code, R, N, K, E, x.data_ptr(), dy.data_ptr(), expert_offsets.data_ptr(), out.data_ptr(),
+        ws.data_ptr(), nbytes, s))
     return out
 
 
@@ -912,25 +938,40 @@ def lora_matmul(x, weight, lora_a, lora_b, adapter_ids, scales, out=None, stream
 
     ``x`` [T, K], ``weight`` [N, K], ``lora_a`` [L, r, K], ``lora_b`` [L, N, r] (adapters of
     smaller rank padded with zeros), ``adapter_ids`` int32 [T], ``scales`` float32 [L];
-    returns [T, N].  float32, float16 or bfloat16; the intermediate stays in fp32."""
+    returns [T, N].  float32, float16 or bfloat16; the intermediate is not rounded to the
+    16-bit type."""
+    what = "lora_matmul"
+    T, K = _dims(what, "x", x, 2)
+    N, _ = _dims(what, "weight", weight, 2)
+    A, r, _ = _dims(what, "lora_a", lora_a, 3)
+    dev, dtype = _device_of(what, x), x.dtype
+    code = _dt_code(what, dtype)
     torch = _torch()
-    T, K = _rank2("lora_matmul", "x", x)
-    N, _ = _rank2("lora_matmul", "weight", weight)
-    L, r, _ = _rank3("lora_matmul", "lora_a", lora_a)
-    _operands("lora_matmul", x, (
-        ("x", x, (T, K), None), ("weight", weight, (N, K), None),
-        ("lora_a", lora_a, (L, r, K), None), ("lora_b", lora_b, (L, N, r), None),
-        ("adapter_ids", adapter_ids, (T,), torch.int32),
-        ("scales", scales, (L,), torch.float32)), out, (T, N))
-    dt = elem_type_of(x)
-    nbytes = _SZ()
-    check(lib().moe_b200_lora_matmul_workspace_size(dt, T, r, ctypes.byref(nbytes)))
-    with _On(stream, (x, weight, lora_a, lora_b, adapter_ids, scales, out)) as s:
-        if out is None:
-            out = torch.empty((T, N), dtype=x.dtype, device=x.device)
-        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=x.device)
-        check(lib().moe_b200_lora_matmul(
-            dt, T, N, K, L, r, x.data_ptr(), weight.data_ptr(), lora_a.data_ptr(),
-            lora_b.data_ptr(), adapter_ids.data_ptr(), scales.data_ptr(), out.data_ptr(),
-            ws.data_ptr(), nbytes.value, s))
+    _require(what, "x", x, (T, K), dtype, dev)
+    _require(what, "weight", weight, (N, K), dtype, dev)
+    _require(what, "lora_a", lora_a, (A, r, K), dtype, dev)
+    _require(what, "lora_b", lora_b, (A, N, r), dtype, dev)
+    _require(what, "adapter_ids", adapter_ids, (T,), torch.int32, dev)
+    _require(what, "scales", scales, (A,), torch.float32, dev)
+    if out is not None:
+        _require(what, "out", out, (T, N), dtype, dev)
+    s = _current_stream(dev) if stream is None else None
+    if s is None:
+        with _Elsewhere(stream, dev, (x, weight, lora_a, lora_b, adapter_ids, scales, out)):
+            return lora_matmul(x, weight, lora_a, lora_b, adapter_ids, scales, out)
+    L = lib()
+    nbytes = _LORA_BYTES.get((code, T, r))
+    if nbytes is None:
+        n = _SZ()
+        check(L.moe_b200_lora_matmul_workspace_size(code, T, r, ctypes.byref(n)))
+        if len(_LORA_BYTES) >= 4096:
+            _LORA_BYTES.clear()
+        nbytes = _LORA_BYTES[code, T, r] = n.value
+    if out is None:
+        out = x.new_empty((T, N))
+    ws = x.new_empty((nbytes,), dtype=torch.uint8)
+    check(L.moe_b200_lora_matmul(
+        code, T, N, K, A, r, x.data_ptr(), weight.data_ptr(), lora_a.data_ptr(),
+        lora_b.data_ptr(), adapter_ids.data_ptr(), scales.data_ptr(), out.data_ptr(),
+        ws.data_ptr(), nbytes, s))
     return out
