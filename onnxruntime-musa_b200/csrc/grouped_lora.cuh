@@ -136,4 +136,80 @@ __device__ __forceinline__ void lora_add(const LoraTerm& l, int ad, int64_t row,
   }
 }
 
+// The same for rows that may follow many adapters (decode): the fragments of BATCH adapters
+// are fetched together, so a block of eight adapters waits for memory 8 / BATCH times
+// instead of eight; gather() may run before the rows' parts exist.
+template <typename T, int STEPS, int BATCH>
+struct LoraBatch {
+  int a[BATCH];              // adapters whose fragments are held, -1: none
+  LoraFrags<STEPS> fr[BATCH];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) a[k] = -1;
+  }
+  // The first BATCH adapters of `todo` (lanes whose row still waits for its adapter `ad`).
+  __device__ __forceinline__ void gather(const LoraTerm& l, int ad, unsigned& todo, int n0, int N) {
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      int next = -1;
+      if (todo != 0) {
+        next = __shfl_sync(0xffffffffu, ad, __ffs(todo) - 1);
+        todo &= ~__ballot_sync(0xffffffffu, ad == next);
+        if (next != a[k] || l.steps > STEPS) fr[k].template load<T>(l, next, 0, n0, N);
+      }
+      a[k] = next;
+    }
+  }
+  static __device__ __forceinline__ void step(const uint2 (&f)[4], const uint4& w,
+                                              float (&d)[2][4]) {
+    mma_16816(d[0], f[0].x, f[1].x, f[0].y, f[1].y, w.x, w.y, T());
+    mma_16816(d[1], f[2].x, f[3].x, f[2].y, f[3].y, w.x, w.y, T());
+    mma_16816(d[0], f[0].x, f[1].x, f[0].y, f[1].y, w.z, w.w, T());
+    mma_16816(d[1], f[2].x, f[3].x, f[2].y, f[3].y, w.z, w.w, T());
+  }
+  // The sums of the held adapters: each column is set from its own adapter only.
+  __device__ __forceinline__ void apply(const LoraTerm& l, int ad, int64_t row, int n0, int N,
+                                        const uint4 (&v)[STEPS], float (&lo)[4], float (&hi)[4]) {
+    const int c = threadIdx.x & 3;
+    const int ad0 = __shfl_sync(0xffffffffu, ad, 8 * c);
+    const int ad1 = __shfl_sync(0xffffffffu, ad, 8 * c + 4);
+    float f0 = 1.f, f1 = 1.f;
+    if (std::is_same<T, __half>::value) {
+      const float f = ad >= 0 ? l.row_scale[row] : 1.f;
+      f0 = __shfl_sync(0xffffffffu, f, 8 * c);
+      f1 = __shfl_sync(0xffffffffu, f, 8 * c + 4);
+    }
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      if (a[k] < 0) break;
+      float d[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) step(fr[k].f[s], v[s], d);
+      if (STEPS > 1) {  // (one step is all of a rank up to 16)
+#pragma unroll 1
+        for (int s0 = STEPS; s0 < l.steps; s0 += STEPS) {
+          uint4 w[STEPS];
+          fr[k].template load<T>(l, a[k], s0, n0, N);
+          lora_rows<STEPS>(l, row, ad >= 0, s0, w);
+#pragma unroll
+          for (int s = 0; s < STEPS; ++s) step(fr[k].f[s], w[s], d);
+        }
+      }
+      if (ad0 == a[k]) {
+        lo[0] = f0 * d[0][0];
+        lo[2] = f0 * d[0][2];
+        hi[0] = f0 * d[1][0];
+        hi[2] = f0 * d[1][2];
+      }
+      if (ad1 == a[k]) {
+        lo[1] = f1 * d[0][1];
+        lo[3] = f1 * d[0][3];
+        hi[1] = f1 * d[1][1];
+        hi[3] = f1 * d[1][3];
+      }
+    }
+  }
+};
+
 }  // namespace moe

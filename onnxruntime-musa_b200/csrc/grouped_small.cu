@@ -11,6 +11,10 @@
 // through distributed shared memory -- 8-row blocks of the accumulator go to the CTA that
 // owns the block, which adds them in rank order -- so there is no global workspace, no
 // counter to clear, no second launch, and the result is the same bits on every call.
+//
+// The adapter term (LORA) does not wait for the product: while the weights stream, the
+// epilogue warps form it for the blocks that they will finish and park it in the other half
+// of the CTA's tensor memory.
 #include <algorithm>
 
 #include "grouped_lora.cuh"
@@ -23,7 +27,7 @@ __device__ int g_small_error;
 constexpr int kBK = 64;
 constexpr int kTileM = 128;
 constexpr int kWBytes = kTileM * kBK * 2;
-constexpr int kThreads = 256;
+constexpr int kThreads = 320;                    // warp 0 TMA, warp 1 MMA, warps 2.. epilogue
 constexpr int kMaxStages = 8;
 constexpr int kStageRow = 64;                    // bytes of a staged output row
 constexpr int kEpiBytes = 8 * kStageRow;         // per warp
@@ -36,10 +40,11 @@ struct SmallParams {
   int E;
   int m_dim, con;
   int m_tiles;
-  int cap;            // most rows of a tile (16, 32, 64, 128 or 256)
+  int cap, cap_log2;  // most rows of a tile (16, 32, 64, 128 or 256)
   int box;            // rows of one TMA box of the rows operand: min(cap, 64)
   int splits;         // cluster size
   int stages, stage_bytes;
+  int part_bytes;     // of the exchange behind the ring; 0: it reuses the ring
   uint32_t tmem_cols;
   void* out;
   int64_t ldo;
@@ -54,27 +59,46 @@ __device__ __forceinline__ void tmem_ld_frag1(uint32_t taddr, float (&v)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void st_cluster_f4(uint32_t addr, const float (&v)[4]) {
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v[0]),
-               "f"(v[1]), "f"(v[2]), "f"(v[3])
+__device__ __forceinline__ void tmem_st_frag1(uint32_t taddr, const float (&v)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x1.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr),
+               "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])),
+               "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3]))
                : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// 16 bytes to another CTA's shared memory, counted on that CTA's barrier `bar`.
+__device__ __forceinline__ void st_async_f4(uint32_t addr, const float (&v)[4], uint32_t bar) {
+  asm volatile(
+      "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::
+          "r"(addr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 template <typename T, int DIR, int LORA>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, LORA > 0 ? 1 : 2)
 grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
                      const __grid_constant__ CUtensorMap map_x, const SmallParams p) {
   constexpr bool kAMn = DIR == kGmmGradInput;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* stage_out = ring + p.stages * p.stage_bytes;
+  uint8_t* parts_buf = p.part_bytes ? ring + p.stages * p.stage_bytes : ring;
+  uint8_t* stage_out = ring + p.stages * p.stage_bytes + p.part_bytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(stage_out + 8 * kEpiBytes);
   uint64_t* empty = full + kMaxStages;
   uint64_t* tfull = empty + kMaxStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull + 1);
+  uint64_t* xfull = tfull + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(xfull + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((2 * kMaxStages + 1) * 8 + 8 <= 256, "barrier block");
+  static_assert((2 * kMaxStages + 2) * 8 + 8 <= 256, "barrier block");
   GroupTable table;
   table.rows = reinterpret_cast<int2*>(full + 32);
   table.tiles = reinterpret_cast<int*>(table.rows + kMaxExperts);
@@ -89,6 +113,7 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
       mbar_init(&empty[s], 1);
     }
     mbar_init(tfull, 1);
+    mbar_init(xfull, 1);
     *abort_flag = 0;
     fence_mbarrier_init();
     tma_prefetch_desc(&map_w);
@@ -98,16 +123,23 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
     tmem_alloc(tmem_slot, p.tmem_cols);
     tmem_relinquish();
   }
+  // The adapter projection's inputs were ready before the launch in front of it started;
+  // its parts are awaited below.
+  if (LORA == 0) pdl_wait();
   if (warp == 2)
-    build_group_table(p.offsets, p.E, static_cast<int>(p.total_rows), p.cap, table);
+    build_group_table(p.offsets, p.E, static_cast<int>(p.total_rows), p.cap_log2, table);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_launch_dependents();  // this CTA holds its tensor memory: see launch_small
   const uint32_t tmem = *tmem_slot;
   if (L >= table.tiles[p.E] * p.m_tiles) {  // the grid is an upper bound; whole clusters leave
     if (warp == 1) tmem_dealloc(tmem, p.tmem_cols);
     return;
   }
+
+  // From here on the cluster stays together; its CTAs' barriers are initialised.
+  if (p.splits > 1 && p.part_bytes) cluster_arrive();
 
   // Tile: the row tiles of a weight tile run side by side (the weights then come from L2).
   const int e = find_group(table.tiles, p.E, p.m_tiles, L);
@@ -172,72 +204,134 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
     tc_commit(tfull);
   }
   __syncwarp();
+
+  // Epilogue warp w reads TMEM lanes 32 (w % 4) ..; the warps of a lane quarter (two, or one
+  // in a block of 192 threads) take turns with the 8-row blocks that this CTA owns (block b
+  // belongs to CTA b % splits).
+  const int S = p.splits;
+  const int blocks = (n + 7) / 8;
+  const int owned = blocks > split ? (blocks - split + S - 1) / S : 0;
+  const bool epi = warp >= 2;
+  const int q = warp & 3, pair = (warp - 2) >> 2, turns = (blockDim.x - 64) / 128;
+  const int feat = m0 + q * 32;
+  const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16);
+  if (threadIdx.x == 64 && S > 1 && owned > 0)
+    mbar_arrive_expect_tx(xfull, owned * (S - 1) * kPartBytes);
+  if constexpr (LORA > 0) {
+    if (epi && pair < owned) {
+      // While the weights stream, a load takes microseconds: the fragments of B are under way
+      // before the parts exist, and each block's parts before the block in front is done.
+      // One copy of the code for all of it: a warp runs it a few times only, and fetching
+      // instructions waits in the same queues (with gather and apply at three places each it
+      // took 8 us longer).
+      LoraBatch<T, LORA, 6 / LORA> batch;
+      batch.clear();
+      const int g = lane >> 2;
+      int i = pair;
+      int row = (i * S + split) * 8 + g;
+      int ad = lora_adapter(p.lora, row0 + row, row < n);
+      unsigned todo = __ballot_sync(0xffffffffu, ad >= 0);
+      uint4 parts[LORA], parts_next[LORA];
+      int row_next = 0, ad_next = -1;
+      float lo[4] = {0.f, 0.f, 0.f, 0.f}, hi[4] = {0.f, 0.f, 0.f, 0.f};
+      bool first = true, fresh = true;
+#pragma unroll 1
+      while (true) {
+        batch.gather(p.lora, ad, todo, feat, p.m_dim);
+        if (first) {
+          pdl_wait();  // the packed parts come from the launch before this one
+          lora_rows<LORA>(p.lora, row0 + row, row < n, 0, parts);
+          first = false;
+        }
+        if (fresh) {
+          row_next = ((i + turns) * S + split) * 8 + g;
+          const bool more = i + turns < owned && row_next < n;
+          ad_next = lora_adapter(p.lora, row0 + row_next, more);
+          lora_rows<LORA>(p.lora, row0 + row_next, more, 0, parts_next);
+          fresh = false;
+        }
+        batch.apply(p.lora, ad, row0 + row, feat, p.m_dim, parts, lo, hi);
+        if (todo != 0) continue;
+        tmem_st_frag1(taddr + p.cap + 8 * i, lo);
+        tmem_st_frag1(taddr + (16u << 16) + p.cap + 8 * i, hi);
+        i += turns;
+        if (i >= owned) break;
+        row = row_next;
+        ad = ad_next;
+#pragma unroll
+        for (int s = 0; s < LORA; ++s) parts[s] = parts_next[s];
+        todo = __ballot_sync(0xffffffffu, ad >= 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lo[j] = hi[j] = 0.f;
+        fresh = true;
+      }
+      tmem_st_wait();
+    } else {
+      pdl_wait();
+    }
+    __syncwarp();
+  }
+
   const bool ok = mbar_wait(tfull, 0);
   if (!ok) {
     atomicExch(&g_small_error, kErrTimeoutEpilogue);
     *abort_flag = 1;
   }
   tc_fence_after();
-
-  // Warp w reads TMEM lanes 32 (w % 4) ..; the warps of a lane quarter take alternate
-  // 8-row blocks of those this CTA owns (block b belongs to CTA b % splits).
-  const int q = warp & 3, pair = warp >> 2;
-  const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16);
-  const int blocks = (n + 7) / 8;
   const bool empty_part = s0 == s1 || !ok;  // nothing accumulated: the part is zero
-  const int S = p.splits;
   if (S > 1) {
-    cluster_sync();  // every CTA's MMAs have read its ring: the rings take the parts now
-    for (int b = pair; b < blocks; b += 2) {
-      const int owner = b % S;
-      if (owner == split) continue;
-      float lo[4] = {0.f, 0.f, 0.f, 0.f}, hi[4] = {0.f, 0.f, 0.f, 0.f};
-      if (!empty_part) {
-        tmem_ld_frag1(taddr + 8 * b, lo);
-        tmem_ld_frag1(taddr + (16u << 16) + 8 * b, hi);
-        tmem_ld_wait();
-      }
-      // Slot of this sender among the owner's S - 1, block b / S of the owner's.
-      const int slot = split < owner ? split : split - 1;
-      const uint32_t dst = smem_u32(ring) + ((b / S) * (S - 1) + slot) * kPartBytes +
-                           q * (kPartBytes / 4) + lane * 16;
-      st_cluster_f4(mapa_shared(dst, owner), lo);
-      st_cluster_f4(mapa_shared(dst + 512, owner), hi);
+    if (p.part_bytes) {
+      cluster_wait();  // every CTA of the cluster has initialised its barriers
+    } else {
+      cluster_sync();  // ... and its MMAs have read its ring, which takes the parts now
     }
-    cluster_sync();
+    if (epi)
+      for (int b = pair; b < blocks; b += turns) {
+        const int owner = b % S;
+        if (owner == split) continue;
+        float lo[4] = {0.f, 0.f, 0.f, 0.f}, hi[4] = {0.f, 0.f, 0.f, 0.f};
+        if (!empty_part) {
+          tmem_ld_frag1(taddr + 8 * b, lo);
+          tmem_ld_frag1(taddr + (16u << 16) + 8 * b, hi);
+          tmem_ld_wait();
+        }
+        // Slot of this sender among the owner's S - 1, block b / S of the owner's.
+        const int slot = split < owner ? split : split - 1;
+        const uint32_t dst = smem_u32(parts_buf) + ((b / S) * (S - 1) + slot) * kPartBytes +
+                             q * (kPartBytes / 4) + lane * 16;
+        const uint32_t bar = mapa_shared(smem_u32(xfull), owner);
+        st_async_f4(mapa_shared(dst, owner), lo, bar);
+        st_async_f4(mapa_shared(dst + 512, owner), hi, bar);
+      }
+    if (owned > 0 && !mbar_wait_cluster(xfull, 0)) atomicExch(&g_small_error, kErrTimeoutEpilogue);
   }
-  if (LORA > 0) pdl_wait();  // t comes from the launch before this one
 
-  uint8_t* buf = stage_out + warp * kEpiBytes;
+  uint8_t* buf = stage_out + (warp & 7) * kEpiBytes;
   const int st_row = lane & 7, st_blk = lane >> 3;
   const uint32_t st_addr =
       smem_u32(buf) + st_row * kStageRow + ((st_blk ^ ((st_row >> 1) & 3)) << 4);
   const int rd_row = lane >> 2, rd_blk = lane & 3;
   const uint8_t* rd_ptr = buf + rd_row * kStageRow + ((rd_blk ^ ((rd_row >> 1) & 3)) << 4);
-  const int feat = m0 + q * 32;
-  LoraFrags<LORA == 0 ? 1 : LORA> frags;
-  for (int i = pair; i * S + split < blocks; i += 2) {
+  for (int i = pair; epi && i < owned; i += turns) {
     const int b = i * S + split;
-    int ad = -1;
-    uint4 parts[LORA == 0 ? 1 : LORA];
-    if constexpr (LORA > 0) {
-      const int row = 8 * b + (lane >> 2);
-      ad = lora_adapter(p.lora, row0 + row, row < n);
-      lora_rows<LORA>(p.lora, row0 + row, row < n, 0, parts);
-    }
     float lo[4] = {0.f, 0.f, 0.f, 0.f}, hi[4] = {0.f, 0.f, 0.f, 0.f};
     float own_lo[4] = {0.f, 0.f, 0.f, 0.f}, own_hi[4] = {0.f, 0.f, 0.f, 0.f};
+    float add_lo[4] = {0.f, 0.f, 0.f, 0.f}, add_hi[4] = {0.f, 0.f, 0.f, 0.f};
     if (!empty_part) {
       tmem_ld_frag1(taddr + 8 * b, own_lo);
       tmem_ld_frag1(taddr + (16u << 16) + 8 * b, own_hi);
-      tmem_ld_wait();
     }
+    if constexpr (LORA > 0) {
+      tmem_ld_frag1(taddr + p.cap + 8 * i, add_lo);
+      tmem_ld_frag1(taddr + (16u << 16) + p.cap + 8 * i, add_hi);
+    }
+    tmem_ld_wait();
     for (int r = 0; r < S; ++r) {  // the parts in rank order
       if (r == split) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) { lo[j] += own_lo[j]; hi[j] += own_hi[j]; }
       } else {
-        const uint8_t* src = ring + (i * (S - 1) + (r < split ? r : r - 1)) * kPartBytes +
+        const uint8_t* src = parts_buf + (i * (S - 1) + (r < split ? r : r - 1)) * kPartBytes +
                              q * (kPartBytes / 4) + lane * 16;
         const float4 a = *reinterpret_cast<const float4*>(src);
         const float4 c = *reinterpret_cast<const float4*>(src + 512);
@@ -245,8 +339,10 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
         hi[0] += c.x; hi[1] += c.y; hi[2] += c.z; hi[3] += c.w;
       }
     }
-    if constexpr (LORA > 0)
-      lora_add<T, LORA>(p.lora, ad, row0 + 8 * b + (lane >> 2), feat, p.m_dim, parts, frags, lo, hi);
+    if constexpr (LORA > 0) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { lo[j] += add_lo[j]; hi[j] += add_hi[j]; }
+    }
     stmatrix4_t(st_addr, pack2<T>(lo[0], lo[1]), pack2<T>(lo[2], lo[3]), pack2<T>(hi[0], hi[1]),
                 pack2<T>(hi[2], hi[3]));
     __syncwarp();
@@ -281,58 +377,54 @@ cudaError_t launch_small(const GroupedArgs& g, const LoraTerm* lora, int num_sms
   // Tile cap: twice the mean rows per group (uneven groups then mostly stay one tile, and
   // their weights are streamed once), all of them when there is one group.
   const int64_t want = g.E == 1 ? g.rows : 2 * ((g.rows + g.E - 1) / g.E);
-  p.cap = 16;
-  while (p.cap < 256 && p.cap < want) p.cap *= 2;
+  p.cap_log2 = 4;
+  while (p.cap_log2 < 8 && (1 << p.cap_log2) < want) ++p.cap_log2;
+  p.cap = 1 << p.cap_log2;
   p.box = std::min(p.cap, 64);
   p.stage_bytes = kWBytes + p.cap * kBK * 2;
-  // Ring: two CTAs an SM up to 128 rows, one CTA with all of the memory at 256.
-  const int budget = p.cap <= 128 ? 108 * 1024 : 220 * 1024;
-  p.stages = std::min(kMaxStages, (budget - kFixed) / p.stage_bytes);
-  p.tmem_cols = static_cast<uint32_t>(std::max(32, p.cap));
+  // Tensor memory of the CTAs that fit an SM together never exceeds its 512 columns (a CTA
+  // of these kernels takes at least 90 KB of shared memory per 256 columns), so an
+  // allocation never waits for a CTA that waits for its own cluster.
+  p.tmem_cols = static_cast<uint32_t>(std::max(32, p.cap * (LORA > 0 ? 2 : 1)));
   const int64_t tiles = (g.rows / p.cap + std::min<int64_t>(g.rows, g.E)) * p.m_tiles;
-  // Splits: until the grid holds every SM's resident CTAs, with at least two slices each.
-  const int64_t fill = static_cast<int64_t>(num_sms) * (p.cap <= 128 ? 2 : 1);
+  // CTAs an SM: two, sharing its memory, up to 128 rows; one at 256.  (One alone with 130 KB
+  // was slower: clusters of such CTAs do not all find room at once, 16.5 against 13.4 us for
+  // 64 rows, 4096 x 4096.)  With adapters two need blocks of 192 threads for their registers.
+  const int resident = p.cap > 128 ? 1 : 2;
+  const int budget = p.cap > 128 ? 220 * 1024 : 113 * 1024;
+  const int threads = LORA > 0 && resident == 2 ? 192 : kThreads;
+  // Splits: until the grid fills these, with at least two slices each.  With adapters, one
+  // CTA an SM, so that all find room beside those of the kernel that forms the parts.
+  const int64_t fill = static_cast<int64_t>(num_sms) * (LORA > 0 ? 1 : resident);
   const int slices = (p.con + kBK - 1) / kBK;
   p.splits = 1;
   while (p.splits < 8 && tiles * p.splits * 2 <= fill && slices >= 4 * p.splits) p.splits *= 2;
-
+  // The exchange has its own memory up to 64 rows (at most 28 KB); above, it reuses the ring
+  // and the cluster meets once more before it.
+  const int blocks_owned = (p.cap / 8 + p.splits - 1) / p.splits;
+  p.part_bytes = p.cap <= 64 ? blocks_owned * (p.splits - 1) * kPartBytes : 0;
+  p.stages = std::min(kMaxStages, (budget - kFixed - p.part_bytes) / p.stage_bytes);
   CUtensorMap mw, mx;
   if (!grouped_map(&mw, g.dtype, g.w, g.K, g.N, g.E, DIR == kGmmForward ? 128 : 64) ||
       !grouped_map(&mx, g.dtype, DIR == kGmmForward ? g.x : g.dy, p.con, g.rows, 1, p.box))
     return cudaErrorInvalidValue;
-  const int smem = kFixed + p.stages * p.stage_bytes;
+  const int smem = kFixed + p.stages * p.stage_bytes + p.part_bytes;
   static SmemOptIn opt_in;
   cudaError_t st = opt_in.set(grouped_small_kernel<T, DIR, LORA>, 227 * 1024);
   if (st != cudaSuccess) return st;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.splits));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  int na = 0;
-  attr[na].id = cudaLaunchAttributeClusterDimension;
-  attr[na].val.clusterDim.x = p.splits;
-  attr[na].val.clusterDim.y = 1;
-  attr[na].val.clusterDim.z = 1;
-  ++na;
-  if (LORA > 0) {
-    attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[na].val.programmaticStreamSerializationAllowed = 1;
-    ++na;
-  }
-  cfg.attrs = attr;
-  cfg.numAttrs = na;
-  return cudaLaunchKernelEx(&cfg, grouped_small_kernel<T, DIR, LORA>, mw, mx, p);
+  return launch_overlapped(grouped_small_kernel<T, DIR, LORA>,
+                           static_cast<unsigned>(tiles * p.splits), threads, smem, p.splits, s,
+                           mw, mx, p);
 }
 
 template <typename T>
 cudaError_t launch_small_type(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
                               cudaStream_t s) {
-  // Ranks up to 16 keep one step in registers, larger ones blocks of four.
+  // Register blocks of the adapter term: one step (ranks up to 16) of four adapters, or two
+  // steps of two.
   if (lora != nullptr)
     return lora->steps == 1 ? launch_small<T, kGmmForward, 1>(g, lora, num_sms, s)
-                            : launch_small<T, kGmmForward, 4>(g, lora, num_sms, s);
+                            : launch_small<T, kGmmForward, 2>(g, lora, num_sms, s);
   if (g.dir == kGmmForward) return launch_small<T, kGmmForward, 0>(g, nullptr, num_sms, s);
   return launch_small<T, kGmmGradInput, 0>(g, nullptr, num_sms, s);
 }

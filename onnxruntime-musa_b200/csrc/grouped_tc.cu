@@ -179,14 +179,15 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
     tmem_alloc_pair(tmem_slot, 2 * kTileN);
     tmem_relinquish_pair();
   }
-  // The launch before wrote the padded tails (grad_weight) or writes t, which only the
-  // epilogue reads (the adapter projection).
+  // The adapter projection's inputs were ready before the launch in front of it started;
+  // its parts are awaited by the epilogue.
   if (LORA == 0) pdl_wait();
-  if (warp == 2) build_group_table(p.offsets, p.E, p.rows, kTileN, table);
+  if (warp == 2) build_group_table(p.offsets, p.E, p.rows, 8, table);
   tc_fence_before();
   __syncthreads();
   cluster_sync();  // both CTAs' barriers are initialised before any remote signal
   tc_fence_after();
+  pdl_launch_dependents();
   const uint32_t tmem_base = *tmem_slot;
   const int total =
       DIR == kGmmGradWeight ? p.E * p.m_tiles * p.n_tiles : table.tiles[p.E] * p.m_tiles;
@@ -400,6 +401,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
 __global__ void __launch_bounds__(256)
 tail_kernel(const int32_t* __restrict__ offsets, int rows, const uint4* __restrict__ dy, int nv,
             const uint4* __restrict__ x, int kv, uint4* __restrict__ ty, uint4* __restrict__ tx) {
+  pdl_wait();
   pdl_launch_dependents();
   const int e = blockIdx.y;
   const int begin = min(max(__ldg(offsets + e), 0), rows);
@@ -466,11 +468,11 @@ cudaError_t launch_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
          grouped_map(&mbt, g.dtype, tx, g.K, static_cast<int64_t>(g.E) * kTailRows, 1, kTailRows);
     if (!ok) return cudaErrorInvalidValue;
     const int vecs = kTailRows * (g.N + g.K) / 8;
-    tail_kernel<<<dim3(std::min(32, (vecs + 255) / 256), g.E), 256, 0, s>>>(
-        g.offsets, p.rows, static_cast<const uint4*>(g.dy), g.N / 8,
-        static_cast<const uint4*>(g.x), g.K / 8, reinterpret_cast<uint4*>(ty),
-        reinterpret_cast<uint4*>(tx));
-    cudaError_t st = cudaGetLastError();
+    cudaError_t st = launch_dependent(true, tail_kernel,
+                                      dim3(std::min(32, (vecs + 255) / 256), g.E), dim3(256), 0, s, g.offsets,
+                                      p.rows, static_cast<const uint4*>(g.dy), g.N / 8,
+                                      static_cast<const uint4*>(g.x), g.K / 8,
+                                      reinterpret_cast<uint4*>(ty), reinterpret_cast<uint4*>(tx));
     if (st != cudaSuccess) return st;
   } else {
     const int feat = DIR == kGmmForward ? g.N : g.K;
@@ -492,9 +494,8 @@ cudaError_t launch_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
   cudaError_t st = opt_in.set(grouped_pair_kernel<T, DIR, LORA>, kSmem);
   if (st != cudaSuccess) return st;
   const int64_t pairs = std::min<int64_t>(tiles, num_sms / 2);
-  return launch_dependent(DIR == kGmmGradWeight || LORA > 0, grouped_pair_kernel<T, DIR, LORA>,
-                          dim3(static_cast<unsigned>(2 * pairs)), dim3(kThreads), kSmem, s, ma, mb,
-                          mat, mbt, p);
+  return launch_overlapped(grouped_pair_kernel<T, DIR, LORA>, static_cast<unsigned>(2 * pairs),
+                           kThreads, kSmem, 0, s, ma, mb, mat, mbt, p);
 }
 
 template <typename T>

@@ -51,10 +51,11 @@ constexpr int kBK = 64;
 constexpr int kM = 128;
 constexpr int kABytes = kM * kBK * 2;
 constexpr int kMaxChunk = 64;
-constexpr int kTcStages = 4;
+constexpr int kTcStages = 8;   // most stages of the ring
 // Largest dynamic shared memory: align slack, ring, partial sums, barriers.
-constexpr int kTcSmemMax = 1024 + kTcStages * (kABytes + kMaxChunk * kBK * 2) +
+constexpr int kTcSmemMax = 1024 + 3 * (kABytes + kMaxChunk * kBK * 2) +
                            kMaxChunk * kLoraMaxRank * 4 + 256;
+static_assert(1024 + 92 * 1024 + kABytes + 8 * kLoraMaxRank * 4 + 256 <= kTcSmemMax, "");
 constexpr int kTcThreads = 256;   // warp 0 TMA, warp 1 MMA, warps 4..7 epilogue
 
 struct ShrinkParams {
@@ -64,10 +65,12 @@ struct ShrinkParams {
   float* row_scale;
   int64_t rows;
   int K, rank, adapters;
-  int chunk;      // rows of a CTA: 8 or 64
+  int chunk;      // rows of a CTA: 4, 8 or 64
   int mma_n;      // max(chunk, 16)
   int splits;
-  int stage_bytes;
+  int a_bytes;    // rows of A_a in a stage (the MMA reads on behind them, in other stages
+                  // or the slack after the ring: lanes that nobody reads)
+  int stages, stage_bytes;
 };
 
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
@@ -92,11 +95,10 @@ template <typename T>
 __global__ void __launch_bounds__(kTcThreads)
 lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
                       const __grid_constant__ CUtensorMap map_a, const ShrinkParams p) {
-  pdl_launch_dependents();  // the projection's main loop does not read t
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  float* part = reinterpret_cast<float*>(ring + kTcStages * p.stage_bytes);  // [chunk][rank]
+  float* part = reinterpret_cast<float*>(ring + p.stages * p.stage_bytes + kABytes - p.a_bytes);  // [chunk][rank]
   uint64_t* full = reinterpret_cast<uint64_t*>(part + p.chunk * p.rank);
   uint64_t* empty = full + kTcStages;
   uint64_t* tfull = empty + kTcStages;   // [2]
@@ -112,7 +114,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
   const int n = static_cast<int>(min(static_cast<int64_t>(p.chunk), p.rows - row0));
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kTcStages; ++s) {
+    for (int s = 0; s < p.stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -129,6 +131,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
     tmem_alloc(tmem_slot, tmem_cols);
     tmem_relinquish();
   }
+  pdl_wait();
   // Distinct adapters of the chunk in order of first appearance.
   const int tok = static_cast<int>(threadIdx.x) - 64;  // warps 2 and 3
   const bool mine = tok >= 0 && tok < kMaxChunk;
@@ -143,6 +146,10 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // The projection's main loop does not read the parts, so it may start now -- not before
+  // this CTA holds its tensor memory, which the projection could otherwise take and keep
+  // until this kernel is done.
+  pdl_launch_dependents();
   if (mine) {
     const int id = s_id[tok];
     int first = -1;
@@ -177,25 +184,34 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
   const int s1 = static_cast<int>(static_cast<int64_t>(slices) * (split + 1) / p.splits);
 
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int ps = 0; ps < passes && !*abort_flag; ++ps) {
-        const int u0 = ps * per, nu = min(per, units - u0);
-        for (int s = s0; s < s1; ++s) {
-          if (!mbar_wait(&empty[stage], phase ^ 1)) {
+    // Lane 0 waits for the slot and loads x; lane u loads the rows of unit u (up to 16 boxes
+    // a slice: issued by one thread they took longer than the transfer).
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int ps = 0; ps < passes && ok; ++ps) {
+      const int u0 = ps * per, nu = min(per, units - u0);
+      const int unit = u0 + lane;
+      const bool mine_u = lane < nu;
+      const int a_row = mine_u ? (unit % blocks_u) * kM : 0;
+      const int a_id = mine_u ? s_adapter[unit / blocks_u] : 0;
+      for (int s = s0; s < s1; ++s) {
+        uint8_t* w = ring + stage * p.stage_bytes;
+        if (lane == 0) {
+          ok = mbar_wait(&empty[stage], phase ^ 1);
+          if (ok) {
+            mbar_arrive_expect_tx(&full[stage], (nu * rows_u + p.chunk) * kBK * 2);
+            tma_load_3d(w + p.a_bytes, &map_x, &full[stage], s * kBK, static_cast<int>(row0), 0);
+          } else {
             atomicExch(&g_shrink_error, kErrTimeoutProducer);
             *abort_flag = 1;
-            break;
           }
-          uint8_t* w = ring + stage * p.stage_bytes;
-          mbar_arrive_expect_tx(&full[stage], (nu * rows_u + p.chunk) * kBK * 2);
-          for (int u = 0; u < nu; ++u)
-            tma_load_3d(w + u * rows_u * kBK * 2, &map_a, &full[stage], s * kBK,
-                        ((u0 + u) % blocks_u) * kM, s_adapter[(u0 + u) / blocks_u]);
-          tma_load_3d(w + kABytes, &map_x, &full[stage], s * kBK, static_cast<int>(row0), 0);
-          if (++stage == kTcStages) { stage = 0; phase ^= 1; }
         }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        if (!ok) break;
+        if (mine_u)
+          tma_load_3d(w + lane * rows_u * kBK * 2, &map_a, &full[stage], s * kBK, a_row, a_id);
+        if (++stage == p.stages) { stage = 0; phase ^= 1; }
       }
     }
   } else if (warp == 1) {
@@ -216,10 +232,10 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
 #pragma unroll
           for (int k = 0; k < kBK / 16; ++k)
             tc_mma_f16(tmem + acc * p.mma_n, smem_desc_k_sw128(w + k * 32),
-                       smem_desc_k_sw128(w + kABytes + k * 32), idesc,
+                       smem_desc_k_sw128(w + p.a_bytes + k * 32), idesc,
                        (s != s0 || k != 0) ? 1u : 0u);
           tc_commit(&empty[stage]);
-          if (++stage == kTcStages) { stage = 0; phase ^= 1; }
+          if (++stage == p.stages) { stage = 0; phase ^= 1; }
         }
         tc_commit(&tfull[acc]);  // after a timeout too: it waits for the MMAs issued
       }
@@ -278,9 +294,13 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
       v[h] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (j < p.rank) {
         const uint32_t at = smem_u32(part + i * p.rank + j);
-        for (int r = 0; r < p.splits; ++r) {
-          const float4 w = ld_cluster_f4(mapa_shared(at, r));
-          v[h].x += w.x; v[h].y += w.y; v[h].z += w.z; v[h].w += w.w;
+        float4 w[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          w[r] = r < p.splits ? ld_cluster_f4(mapa_shared(at, r)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          v[h].x += w[r].x; v[h].y += w[r].y; v[h].z += w[r].z; v[h].w += w[r].w;
         }
         v[h].x *= sc; v[h].y *= sc; v[h].z *= sc; v[h].w *= sc;
       }
@@ -309,7 +329,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
 
 // Rows of a CTA: small chunks spread a decode batch (whose rows follow many adapters) over
 // the GPU, tall ones read A_a once per 64 rows of a prompt.
-int shrink_chunk(int64_t rows) { return rows <= 256 ? 8 : kMaxChunk; }
+int shrink_chunk(int64_t rows) { return rows <= 128 ? 4 : rows <= 256 ? 8 : kMaxChunk; }
 
 template <typename T>
 cudaError_t shrink_simt(const LoraShrink& l, float* t, cudaStream_t s) {
@@ -332,7 +352,14 @@ cudaError_t shrink_tc(const LoraShrink& l, uint4* packed, float* row_scale, int 
   p.adapters = l.adapters;
   p.chunk = shrink_chunk(l.rows);
   p.mma_n = std::max(p.chunk, 16);
-  p.stage_bytes = kABytes + p.mma_n * kBK * 2;
+  // A stage holds the adapters that a chunk can have (one token: r rows), so that a short
+  // K is in flight as a whole; two CTAs an SM with the partial sums of rank 64.
+  const int unit = std::min(l.rank, kM);
+  p.a_bytes = static_cast<int>(std::min<int64_t>(kM / unit, std::min<int64_t>(l.rows, p.chunk))) *
+              unit * kBK * 2;
+  p.stage_bytes = p.a_bytes + p.mma_n * kBK * 2;
+  p.stages = std::min(kTcStages, 92 * 1024 / p.stage_bytes);
+  if (p.chunk == kMaxChunk) p.stages = std::min(p.stages, 3);
   // Splits: until about two CTAs an SM run, with at least two slices of K each.
   const int64_t chunks = (l.rows + p.chunk - 1) / p.chunk;
   const int slices = (l.K + kBK - 1) / kBK;
@@ -345,19 +372,10 @@ cudaError_t shrink_tc(const LoraShrink& l, uint4* packed, float* row_scale, int 
   static SmemOptIn opt_in;
   cudaError_t st = opt_in.set(lora_shrink_tc_kernel<T>, kTcSmemMax);
   if (st != cudaSuccess) return st;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(chunks * p.splits));
-  cfg.blockDim = dim3(kTcThreads);
-  cfg.dynamicSmemBytes = 1024 + kTcStages * p.stage_bytes + p.chunk * p.rank * 4 + 256;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.splits;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, lora_shrink_tc_kernel<T>, mx, ma, p);
+  const size_t smem =
+      1024 + p.stages * p.stage_bytes + kABytes - p.a_bytes + p.chunk * p.rank * 4 + 256;
+  return launch_overlapped(lora_shrink_tc_kernel<T>, static_cast<unsigned>(chunks * p.splits),
+                           kTcThreads, smem, p.splits, s, mx, ma, p);
 }
 
 }  // namespace
