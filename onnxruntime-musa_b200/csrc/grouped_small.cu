@@ -40,7 +40,7 @@ struct SmallParams {
   int E;
   int m_dim, con;
   int m_tiles;
-  int cap, cap_log2;  // most rows of a tile (16, 32, 64, 128 or 256)
+  int cap;            // most rows of a tile (16, 32, 64, 128 or 256)
   int box;            // rows of one TMA box of the rows operand: min(cap, 64)
   int splits;         // cluster size
   int stages, stage_bytes;
@@ -127,7 +127,7 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
   // its parts are awaited below.
   if (LORA == 0) pdl_wait();
   if (warp == 2)
-    build_group_table(p.offsets, p.E, static_cast<int>(p.total_rows), p.cap_log2, table);
+    build_group_table(p.offsets, p.E, static_cast<int>(p.total_rows), p.cap, table);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -378,9 +378,8 @@ cudaError_t launch_small(const GroupedArgs& g, const LoraTerm* lora, int num_sms
   // Tile cap: twice the mean rows per group (uneven groups then mostly stay one tile, and
   // their weights are streamed once), all of them when there is one group.
   const int64_t want = g.E == 1 ? g.rows : 2 * ((g.rows + g.E - 1) / g.E);
-  p.cap_log2 = 4;
-  while (p.cap_log2 < 8 && (1 << p.cap_log2) < want) ++p.cap_log2;
-  p.cap = 1 << p.cap_log2;
+  p.cap = 16;
+  while (p.cap < 256 && p.cap < want) p.cap *= 2;
   p.box = std::min(p.cap, 64);
   p.stage_bytes = kWBytes + p.cap * kBK * 2;
   // Tensor memory of the CTAs that fit an SM together never exceeds its 512 columns (a CTA

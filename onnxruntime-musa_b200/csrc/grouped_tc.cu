@@ -58,6 +58,7 @@ struct PairParams {
   int n_dim;      // grad_weight: K
   int con;        // contraction length (not grad_weight)
   int m_tiles, n_tiles;
+  int tile_rows;   // most rows of a tile (forward, grad_input)
   void* out;
   int64_t ldo;
   LoraTerm lora;
@@ -113,6 +114,15 @@ __device__ __forceinline__ PairTile pair_tile(int L, const GroupTable& g, const 
     t.begin = t.cnt = 0;
   }
   return t;
+}
+
+// Tile of turn `i`: rounds of one tile per pair, walked forth and back.  (Tiles of grad_weight
+// cost what their expert has rows; walked forth only, the first pairs got the dearer tile of
+// every round: 366 us against 337 for 16384 tokens over 64 experts by a power law, [768, 2048].
+// Claiming tiles from a counter took 349 us, and 301 against 235 for a short batch, whose tiles
+// are two slices long.)
+__device__ __forceinline__ int turn_tile(int i, int pair, int npairs) {
+  return i * npairs + ((i & 1) ? npairs - 1 - pair : pair);
 }
 
 // MMA steps of 16 in slice `b` of the tile.
@@ -182,7 +192,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
   // The adapter projection's inputs were ready before the launch in front of it started;
   // its parts are awaited by the epilogue.
   if (LORA == 0) pdl_wait();
-  if (warp == 2) build_group_table(p.offsets, p.E, p.rows, 8, table);
+  if (warp == 2) build_group_table(p.offsets, p.E, p.rows, p.tile_rows, table);
   tc_fence_before();
   __syncthreads();
   cluster_sync();  // both CTAs' barriers are initialised before any remote signal
@@ -200,7 +210,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
-      for (int L = pair; L < total && !*abort_flag; L += npairs) {
+      for (int i = 0;; ++i) {
+        const int L = turn_tile(i, pair, npairs);
+        if (L >= total || *abort_flag) break;
         const PairTile t = pair_tile<DIR>(L, table, p);
         const int a0 = t.m0 + static_cast<int>(rank) * 128;
         // Rows of this CTA's half of the MMA's N, in boxes of 64.
@@ -248,9 +260,11 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
   } else if (warp == 1) {
     // ------------------------------------------------- MMA issuer (leader CTA only)
     if (lane == 0 && leader) {
-      int stage = 0, i = 0;
+      int stage = 0;
       uint32_t phase = 0;
-      for (int L = pair; L < total && !*abort_flag; L += npairs, ++i) {
+      for (int i = 0;; ++i) {
+        const int L = turn_tile(i, pair, npairs);
+        if (L >= total || *abort_flag) break;
         const PairTile t = pair_tile<DIR>(L, table, p);
         const uint32_t idesc = idesc_f16(TcFormat<T>::kId, kTileM, t.nt) |
                                (kAMn ? kIdescAMn : 0) | (kBMn ? kIdescBMn : 0);
@@ -307,9 +321,10 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
     const int rd_row = lane >> 2, rd_blk = lane & 3;
     const uint8_t* rd_ptr = buf + rd_row * kStageRow + ((rd_blk ^ ((rd_row >> 1) & 3)) << 4);
     T* out = static_cast<T*>(p.out);
-    int i = 0;
     if (LORA > 0) pdl_wait();
-    for (int L = pair; L < total && !*abort_flag; L += npairs, ++i) {
+    for (int i = 0;; ++i) {
+      const int L = turn_tile(i, pair, npairs);
+      if (L >= total || *abort_flag) break;
       const PairTile t = pair_tile<DIR>(L, table, p);
       const int acc = i & 1;
       if (!mbar_wait(&tfull[acc], (i >> 1) & 1)) {
@@ -321,43 +336,23 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
       const uint32_t taddr =
           tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * kTileN;
       const int m = t.m0 + static_cast<int>(rank) * 128 + q * 32;  // first M entry of the warp
-      LoraFrags<LORA == 0 ? 1 : LORA> frags;  // of this tile's features
-      for (int c = first; c < t.n; c += 64) {
-        // The chunk's adapters and packed parts are fetched ahead of the accumulators: one
-        // trip to L2 a chunk instead of one a row block.
-        int ads = -1;
-        uint4 parts[4][LORA == 0 ? 1 : LORA];
-        if constexpr (LORA > 0) {
-          ads = lora_adapter(p.lora, t.n0 + c + lane, c + lane < t.n);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int row = c + 8 * j + (lane >> 2);
-            lora_rows<LORA>(p.lora, t.n0 + row, row < t.n, 0, parts[j]);
-          }
-        }
-        float lo[16], hi[16];
-        if (DIR == kGmmGradWeight && t.cnt == 0) {  // an expert without rows: zeros
-#pragma unroll
-          for (int j = 0; j < 16; ++j) lo[j] = hi[j] = 0.f;
-        } else {
-          tmem_ld_frag4(taddr + c, lo);
-          tmem_ld_frag4(taddr + (16u << 16) + c, hi);
-          tmem_ld_wait();
-        }
+      const bool zero = DIR == kGmmGradWeight && t.cnt == 0;  // an expert without rows
+      auto release = [&] {  // this warp has read the accumulator
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));
+      };
+      auto fetch = [&](int c, float (&lo)[16], float (&hi)[16]) {
+        tmem_ld_frag4(taddr + c, lo);
+        tmem_ld_frag4(taddr + (16u << 16) + c, hi);
+      };
+      // Stores 32 columns of the accumulator, c .. c + 31.
+      auto store = [&](int c, float (&lo)[16], float (&hi)[16]) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int sel = (j & 1) * 8 * kStageRow;
           T* dst;
           bool ok;
-          if constexpr (LORA > 0) {
-            float dl[4], dh[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) { dl[k] = lo[4 * j + k]; dh[k] = hi[4 * j + k]; }
-            lora_add<T, LORA>(p.lora, __shfl_sync(0xffffffffu, ads, 8 * j + (lane >> 2)),
-                              t.n0 + c + 8 * j + (lane >> 2), m, p.m_dim, parts[j], frags, dl, dh);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) { lo[4 * j + k] = dl[k]; hi[4 * j + k] = dh[k]; }
-          }
           if (DIR == kGmmGradWeight) {
             // Eight M rows (block j of the 32) x 32 columns.
             const float(&v)[16] = j < 2 ? lo : hi;
@@ -380,10 +375,63 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
           const uint4 w = *reinterpret_cast<const uint4*>(rd_ptr + sel);
           if (ok) *reinterpret_cast<uint4*>(dst) = w;
         }
+      };
+      if constexpr (LORA > 0) {
+        LoraFrags<LORA> frags;  // of this tile's features
+        for (int c = first; c < t.n; c += 64) {
+          // The chunk's adapters and packed parts are fetched ahead of the accumulators: one
+          // trip to L2 a chunk instead of one a row block.
+          const int ads = lora_adapter(p.lora, t.n0 + c + lane, c + lane < t.n);
+          uint4 parts[4][LORA];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int row = c + 8 * j + (lane >> 2);
+            lora_rows<LORA>(p.lora, t.n0 + row, row < t.n, 0, parts[j]);
+          }
+          float lo[16], hi[16];
+          fetch(c, lo, hi);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float dl[4], dh[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { dl[k] = lo[4 * j + k]; dh[k] = hi[4 * j + k]; }
+            lora_add<T, LORA>(p.lora, __shfl_sync(0xffffffffu, ads, 8 * j + (lane >> 2)),
+                              t.n0 + c + 8 * j + (lane >> 2), m, p.m_dim, parts[j], frags, dl, dh);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { lo[4 * j + k] = dl[k]; hi[4 * j + k] = dh[k]; }
+          }
+          store(c, lo, hi);
+        }
+        release();
+      } else {
+        // The next columns are on their way from tensor memory while these are stored, and
+        // the accumulator goes back before the last ones are.
+        float lo[16] = {}, hi[16] = {}, lo2[16] = {}, hi2[16] = {};
+        int c = first;
+        if (c < t.n && !zero) fetch(c, lo, hi);
+        tmem_ld_wait();
+        if (c >= t.n) release();
+        while (c < t.n) {
+          if (c + 64 < t.n) {
+            if (!zero) fetch(c + 64, lo2, hi2);
+          } else {
+            release();
+          }
+          store(c, lo, hi);
+          c += 64;
+          if (c >= t.n) break;
+          tmem_ld_wait();
+          if (c + 64 < t.n) {
+            if (!zero) fetch(c + 64, lo, hi);
+          } else {
+            release();
+          }
+          store(c, lo2, hi2);
+          c += 64;
+          tmem_ld_wait();
+        }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));
     }
   }
 
@@ -445,6 +493,26 @@ size_t tail_bytes(int64_t E, int64_t width) {
   return (static_cast<size_t>(E) * kTailRows * static_cast<size_t>(width) * 2 + 255) & ~size_t{255};
 }
 
+// Tile height for one group of `rows`: the tiles run in rounds of one per SM pair, and a
+// round that is nearly empty costs a whole one, so the height (a multiple of 16) is the one
+// with the shortest rounds x slice time.  A slice takes 2 h cycles of MMA or, below about
+// 215 rows, the (16 KB + 64 h) bytes a CTA reads from L2 at some 70 a cycle.  (4001 rows,
+// 4096 features: 224 instead of 256, four rounds of 224 rows instead of 3.5 that cost four.)
+int tile_rows_one_group(int64_t rows, int m_tiles, int pairs) {
+  int best = kTileN;
+  double best_cost = 1e300;
+  for (int h = kTileN; h >= 128; h -= 16) {
+    const int64_t tiles = (rows + h - 1) / h * m_tiles;
+    const double cost = static_cast<double>((tiles + pairs - 1) / pairs) *
+                        std::max(2.0 * h, (16384.0 + 64.0 * h) / 70.0);
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = h;
+    }
+  }
+  return best;
+}
+
 template <typename T, int DIR, int LORA>
 cudaError_t launch_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms, cudaStream_t s) {
   CUtensorMap ma, mb, mat, mbt;
@@ -484,12 +552,14 @@ cudaError_t launch_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
     if (!ok) return cudaErrorInvalidValue;
     mat = ma;
     mbt = mb;
+    p.tile_rows = kTileN;
+    if (g.E == 1) p.tile_rows = tile_rows_one_group(g.rows, (feat + kTileM - 1) / kTileM, num_sms / 2);
   }
   p.m_tiles = (p.m_dim + kTileM - 1) / kTileM;
   const int64_t tiles =
           DIR == kGmmGradWeight
               ? static_cast<int64_t>(g.E) * p.m_tiles * p.n_tiles
-              : (g.rows / kTileN + std::min<int64_t>(g.rows, g.E)) * p.m_tiles;
+              : (g.rows / p.tile_rows + std::min<int64_t>(g.rows, g.E)) * p.m_tiles;
   static SmemOptIn opt_in;
   cudaError_t st = opt_in.set(grouped_pair_kernel<T, DIR, LORA>, kSmem);
   if (st != cudaSuccess) return st;

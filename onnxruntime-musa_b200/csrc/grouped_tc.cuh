@@ -72,17 +72,17 @@ struct GroupTable {
 
 // Filled by one full warp.  offsets == nullptr: one group of all rows.  Offsets are clamped
 // to [0, rows] and a group never ends before it begins, whatever the caller's array holds.
-// Tiles are 1 << shift rows.  A lane takes ceil(E / 32) adjacent groups, so that all loads
+// A lane takes ceil(E / 32) adjacent groups, so that all loads
 // are in flight together (a short kernel waits for this before anything else).
 __device__ __forceinline__ void build_group_table(const int32_t* offsets, int E, int rows,
-                                                  int shift, const GroupTable& t) {
+                                                  int tile_rows, const GroupTable& t) {
   constexpr int kPer = kMaxExperts / 32;
   const int lane = threadIdx.x & 31;
   if (offsets == nullptr) {
     if (lane == 0) {
       t.rows[0] = make_int2(0, rows);
       t.tiles[0] = 0;
-      t.tiles[1] = (rows + (1 << shift) - 1) >> shift;
+      t.tiles[1] = (rows + tile_rows - 1) / tile_rows;
     }
     return;
   }
@@ -98,7 +98,7 @@ __device__ __forceinline__ void build_group_table(const int32_t* offsets, int E,
       const int b = min(max(v[i], 0), rows);
       const int c = max(min(v[i + 1], rows), b);
       t.rows[e0 + i] = make_int2(b, c);
-      v[i] = (c - b + (1 << shift) - 1) >> shift;
+      v[i] = (c - b + tile_rows - 1) / tile_rows;
       sum += v[i];
     }
   int incl = sum;
