@@ -36,11 +36,13 @@ struct LoraTerm {
   // FFMA kernels: t = A_a x in fp32, [rows][rank], and the adapters' scales [L].
   const float* t;
   const float* scales;
-  // Tensor-core kernels: s_a t in 16-bit parts, [rows][steps][4], step = 16 rank entries
-  // (grouped_lora.cuh); fp16: the power of two that each row's parts are to be scaled by.
-  const uint4* packed;
+  // Tensor-core kernels: s_a t in two 16-bit parts, [2][rows][rank] (grouped_lora.cuh);
+  // fp16: the power of two that each row's parts are to be scaled by; and each row's adapter,
+  // -1 for none, with kLoraScaled set where that power is not 1.
+  const uint16_t* parts;
   int steps;              // ceil(rank / 16)
   const float* row_scale;
+  const int* row_code;
 };
 
 // Largest feature and contraction length, and most rows, of a call (index arithmetic of
@@ -48,6 +50,7 @@ struct LoraTerm {
 constexpr int64_t kGmmMaxDim = 1 << 20;
 constexpr int64_t kGmmMaxRows = 1 << 30;
 constexpr int kLoraMaxRank = 256;
+constexpr int kLoraScaled = 1 << 24;  // above every adapter number
 
 // t[row, j] = sum_k A_a[j, k] x[row, k] for rows with an adapter a (others are left).
 struct LoraShrink {
@@ -62,10 +65,10 @@ struct LoraShrink {
 // Any type and alignment: t in fp32, [rows][rank].
 cudaError_t launch_lora_shrink_simt(const LoraShrink& l, float* t, cudaStream_t s);
 // 16-bit types, K and rank multiples of 8, 16-byte aligned x and a: the parts of
-// LoraTerm::packed and its row_scale.
+// LoraTerm, its row_scale and row_code.
 bool lora_shrink_tc_supported(const LoraShrink& l);
-cudaError_t launch_lora_shrink_tc(const LoraShrink& l, uint4* packed, float* row_scale,
-                                  int num_sms, cudaStream_t s);
+cudaError_t launch_lora_shrink_tc(const LoraShrink& l, uint16_t* parts, float* row_scale,
+                                  int* row_code, int num_sms, cudaStream_t s);
 
 // Tensor-core path: 16-bit types, N and K multiples of 8, 16-byte aligned buffers.
 bool grouped_tc_supported(const GroupedArgs& g);

@@ -105,13 +105,13 @@ int run_grouped(const char* what, const moe::GroupedArgs& g, cudaStream_t s) {
   return rc != MOE_B200_OK ? rc : finish(what, s);
 }
 
-// Workspace of lora_matmul: 64 bytes per row and 16 rank entries (the packed parts, or t in
-// fp32), then a float per row.
+// Workspace of lora_matmul: four bytes per row and rank entry (two 16-bit parts, or t in
+// fp32), then a float and an int per row.
 size_t lora_parts_bytes(int64_t rows, int64_t rank) {
-  return static_cast<size_t>(rows) * static_cast<size_t>((rank + 15) / 16) * 64;
+  return (static_cast<size_t>(rows) * static_cast<size_t>(rank) * 4 + 15) & ~size_t{15};
 }
 size_t lora_bytes(int64_t rows, int64_t rank) {
-  return lora_parts_bytes(rows, rank) + static_cast<size_t>(rows) * sizeof(float);
+  return lora_parts_bytes(rows, rank) + static_cast<size_t>(rows) * 8;
 }
 
 }  // namespace
@@ -287,13 +287,15 @@ int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
   term.ids = adapter_ids;
   cudaError_t st;
   if (tc) {
-    auto* packed = static_cast<uint4*>(workspace);
+    auto* parts = static_cast<uint16_t*>(workspace);
     auto* row_scale = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
                                                lora_parts_bytes(num_rows, rank));
-    st = moe::launch_lora_shrink_tc(l, packed, row_scale, sm_count(), s);
-    term.packed = packed;
+    auto* row_code = reinterpret_cast<int*>(row_scale + num_rows);
+    st = moe::launch_lora_shrink_tc(l, parts, row_scale, row_code, sm_count(), s);
+    term.parts = parts;
     term.steps = static_cast<int>((rank + 15) / 16);
     term.row_scale = row_scale;
+    term.row_code = row_code;
   } else {
     auto* t = static_cast<float*>(workspace);
     st = moe::launch_lora_shrink_simt(l, t, s);

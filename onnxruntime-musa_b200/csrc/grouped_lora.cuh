@@ -5,8 +5,8 @@
 // The rank-sized intermediate enters mma.m16n8k16 as the sum of two 16-bit parts,
 // hi = round(s_a t) and lo = round(s_a t - hi), which keeps 16 (bf16) or 22 (fp16) of its
 // bits; one part would leave an error of half an output step of the term itself.  fp16
-// rows are first scaled by a power of two to |s_a t| < 2 (t may exceed fp16's range),
-// undone on the fp32 sum.  The shrink kernel (lora.cu) leaves them as the lanes take them.
+// rows outside [2^-8, 2^15) are first scaled by a power of two to |s_a t| < 2 (t may exceed
+// fp16's range), undone on the fp32 sum.  The shrink kernel (lora.cu) forms the parts.
 // The eight rows of a fragment may follow different adapters: the products of each adapter
 // among them are formed for all eight columns in a sum of their own, and a column takes
 // only its own adapter's, so nothing of another adapter (an infinity, say) reaches a row.
@@ -59,16 +59,23 @@ struct LoraFrags {
   }
 };
 
-// The packed parts of row `row` for this lane, 16 STEPS entries from step s0 on: entries
+// The parts of row `row` for this lane, 16 STEPS entries from step s0 on: entries
 // 4 (l % 4) + [0, 4) of each step as {hi, hi, lo, lo}.  (The order of the entries inside a
 // step is free as long as both operands agree, and four in a row make the loads wide.)
 template <int STEPS>
-__device__ __forceinline__ void lora_rows(const LoraTerm& l, int64_t row, bool ok, int s0,
-                                          uint4 (&v)[STEPS]) {
-  const uint4* q = l.packed + (row * l.steps + s0) * 4 + (threadIdx.x & 3);
+__device__ __forceinline__ void lora_rows(const LoraTerm& l, int64_t rows, int64_t row, bool ok,
+                                          int s0, uint4 (&v)[STEPS]) {
+  const int j = s0 * 16 + 4 * (threadIdx.x & 3);
+  const uint16_t* q = l.parts + row * l.rank + j;
 #pragma unroll
-  for (int s = 0; s < STEPS; ++s)
-    v[s] = ok && s0 + s < l.steps ? q[s * 4] : make_uint4(0, 0, 0, 0);
+  for (int s = 0; s < STEPS; ++s) {
+    uint2 hi = make_uint2(0, 0), lo = make_uint2(0, 0);
+    if (ok && j + 16 * s < l.rank) {
+      hi = *reinterpret_cast<const uint2*>(q + 16 * s);
+      lo = *reinterpret_cast<const uint2*>(q + 16 * s + rows * l.rank);
+    }
+    v[s] = make_uint4(hi.x, hi.y, lo.x, lo.y);
+  }
 }
 
 // Adapter of row `row` (-1: none).
@@ -79,9 +86,10 @@ __device__ __forceinline__ int lora_adapter(const LoraTerm& l, int64_t row, bool
 
 // Adds the adapter term of eight rows and features n0 .. n0 + 31 to lo (features 0..15) and
 // hi (16..31).  This lane's row (of the fragment's column l / 4): adapter `ad`, number
-// `row`, its first 16 STEPS packed entries `v`.
+// `row`, its first 16 STEPS entries `v`.
 template <typename T, int STEPS>
-__device__ __forceinline__ void lora_add(const LoraTerm& l, int ad, int64_t row, int n0, int N,
+__device__ __forceinline__ void lora_add(const LoraTerm& l, int64_t rows, int ad, int64_t row,
+                                         int n0, int N,
                                          const uint4 (&v)[STEPS], LoraFrags<STEPS>& fr,
                                          float (&lo)[4], float (&hi)[4]) {
   unsigned todo = __ballot_sync(0xffffffffu, ad >= 0);
@@ -108,7 +116,7 @@ __device__ __forceinline__ void lora_add(const LoraTerm& l, int ad, int64_t row,
         for (int s = 0; s < STEPS; ++s) w[s] = v[s];
       } else {
         fr.template load<T>(l, a, s0, n0, N);
-        lora_rows<STEPS>(l, row, ad >= 0, s0, w);
+        lora_rows<STEPS>(l, rows, row, ad >= 0, s0, w);
       }
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
@@ -169,8 +177,8 @@ struct LoraBatch {
     mma_16816(d[1], f[2].x, f[3].x, f[2].y, f[3].y, w.z, w.w, T());
   }
   // The sums of the held adapters: each column is set from its own adapter only.
-  __device__ __forceinline__ void apply(const LoraTerm& l, int ad, int64_t row, int n0, int N,
-                                        const uint4 (&v)[STEPS], float (&lo)[4], float (&hi)[4]) {
+  __device__ __forceinline__ void apply(const LoraTerm& l, int64_t rows, int ad, int64_t row, int n0,
+                                        int N, const uint4 (&v)[STEPS], float (&lo)[4], float (&hi)[4]) {
     const int c = threadIdx.x & 3;
     const int ad0 = __shfl_sync(0xffffffffu, ad, 8 * c);
     const int ad1 = __shfl_sync(0xffffffffu, ad, 8 * c + 4);
@@ -191,7 +199,7 @@ struct LoraBatch {
         for (int s0 = STEPS; s0 < l.steps; s0 += STEPS) {
           uint4 w[STEPS];
           fr[k].template load<T>(l, a[k], s0, n0, N);
-          lora_rows<STEPS>(l, row, ad >= 0, s0, w);
+          lora_rows<STEPS>(l, rows, row, ad >= 0, s0, w);
 #pragma unroll
           for (int s = 0; s < STEPS; ++s) step(fr[k].f[s], w[s], d);
         }

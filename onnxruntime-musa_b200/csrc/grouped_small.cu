@@ -241,17 +241,17 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
         batch.gather(p.lora, ad, todo, feat, p.m_dim);
         if (first) {
           pdl_wait();  // the packed parts come from the launch before this one
-          lora_rows<LORA>(p.lora, row0 + row, row < n, 0, parts);
+          lora_rows<LORA>(p.lora, p.total_rows, row0 + row, row < n, 0, parts);
           first = false;
         }
         if (fresh) {
           row_next = ((i + turns) * S + split) * 8 + g;
           const bool more = i + turns < owned && row_next < n;
           ad_next = lora_adapter(p.lora, row0 + row_next, more);
-          lora_rows<LORA>(p.lora, row0 + row_next, more, 0, parts_next);
+          lora_rows<LORA>(p.lora, p.total_rows, row0 + row_next, more, 0, parts_next);
           fresh = false;
         }
-        batch.apply(p.lora, ad, row0 + row, feat, p.m_dim, parts, lo, hi);
+        batch.apply(p.lora, p.total_rows, ad, row0 + row, feat, p.m_dim, parts, lo, hi);
         if (todo != 0) continue;
         tmem_st_frag1(taddr + p.cap + 8 * i, lo);
         tmem_st_frag1(taddr + (16u << 16) + p.cap + 8 * i, hi);

@@ -20,6 +20,14 @@
 // (32 KB, six stages); two 256-column accumulators, so the epilogue of a tile overlaps the
 // MMAs of the next.  Bound: the tensor pipe; a slice of the pair is 512 cycles of MMA
 // for 64 KB from L2.
+//
+// The adapter projection is the forward product of one group, and its adapter term more
+// slices of the same accumulator where sixteen adjacent rows (counted from the tile's first)
+// follow one adapter: B_a as the M operand, the rows' parts (grouped_lora.cuh) as the N
+// operand, on the accumulator columns of the run of such rows.  Warp 10 finds the runs.  The
+// rows in between -- sixteen that follow several adapters, fp16 rows scaled against overflow
+// -- get it in the epilogue, which mma.sync makes slow beside tcgen05 (all of it there: 33 us
+// a tile of 224 rows, rank 64, beside 24 us of MMA).
 #include <algorithm>
 #include <mutex>
 
@@ -42,12 +50,13 @@ constexpr int kABytes = 128 * kBK * 2;
 constexpr int kBBytes = 128 * kBK * 2;
 constexpr int kBox = 64 * kBK * 2;       // one 64 x 64 box of a 16-bit operand
 constexpr int kThreads = 320;
+constexpr int kLoraThreads = 352;        // warp 10: the tile's runs of rows
 constexpr int kEpiWarps = 8;
 constexpr int kStageRow = 64;            // bytes of one staged output row (32 elements)
 constexpr int kEpiBytes = 2 * 8 * kStageRow;  // per warp: two buffers of 8 rows
 constexpr int kRaster = 8;               // M-fastest runs of this many tiles (L2 reuse)
 constexpr int kTailRows = 16;
-constexpr int kSmem = 1024 + kStages * (kABytes + kBBytes) + kEpiWarps * kEpiBytes + 256 +
+constexpr int kSmem = 1024 + kStages * (kABytes + kBBytes) + kEpiWarps * kEpiBytes + 384 +
                       kMaxExperts * 8 + (kMaxExperts + 1) * 4;
 static_assert(kSmem <= 227 * 1024, "shared memory of the pair kernel");
 
@@ -62,6 +71,7 @@ struct PairParams {
   void* out;
   int64_t ldo;
   LoraTerm lora;
+  int rank_blocks;  // of 64
 };
 
 struct PairTile {
@@ -125,6 +135,33 @@ __device__ __forceinline__ int turn_tile(int i, int pair, int npairs) {
   return i * npairs + ((i & 1) ? npairs - 1 - pair : pair);
 }
 
+// Adapter projection: what a group of sixteen rows follows -- an adapter, none (-1), several
+// (kMixedCode; also rows scaled against overflow) or, past the last row, anything.
+constexpr int kMixedCode = -2;
+constexpr int kAnyCode = -3;
+__device__ __forceinline__ int join_codes(int a, int b) {
+  return a == b || b == kAnyCode ? a : a == kAnyCode ? b : kMixedCode;
+}
+// Runs of groups that follow the same adapter, in order.
+struct RunWalk {
+  const volatile int* code_of;
+  int groups, at = 0;
+  int code = -1, begin = 0, count = 0;
+  __device__ RunWalk(const volatile int* c, int n) : code_of(c), groups(n) {}
+  __device__ __forceinline__ bool next() {
+    while (at < groups && code_of[at] < 0) ++at;
+    if (at >= groups) return false;
+    begin = at;
+    code = code_of[at];
+    while (at < groups && code_of[at] == code) ++at;
+    count = at - begin;
+    return true;
+  }
+};
+__device__ __forceinline__ void fence_proxy_async_all() {
+  asm volatile("fence.proxy.async;" ::: "memory");
+}
+
 // MMA steps of 16 in slice `b` of the tile.
 template <int DIR>
 __device__ __forceinline__ int block_steps(const PairTile& t, int b) {
@@ -141,7 +178,7 @@ __device__ __forceinline__ bool is_tail(const PairTile& t, int b) {
 
 // LORA: 16-entry steps of the rank per register block of the adapter term, 0 without one.
 template <typename T, int DIR, int LORA>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LORA > 0 ? kLoraThreads : kThreads, 1)
 grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
                     const __grid_constant__ CUtensorMap map_b,
                     const __grid_constant__ CUtensorMap map_at,
@@ -160,9 +197,14 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
   uint64_t* done = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((2 * kStages + 5) * 8 + 8 <= 256, "barrier block");
+  // Adapter projection: what each 16-row group of a tile follows, for the tile of turn i in
+  // slot i % 2.
+  uint64_t* cfull = done + 2;
+  uint64_t* cempty = cfull + 2;
+  volatile int* codes = reinterpret_cast<volatile int*>(cempty + 2);  // [2][16]
+  static_assert((2 * kStages + 10) * 8 + 2 * 16 * 4 <= 384, "barrier block");
   GroupTable table;
-  table.rows = reinterpret_cast<int2*>(bars + 32);
+  table.rows = reinterpret_cast<int2*>(bars + 48);
   table.tiles = reinterpret_cast<int*>(table.rows + kMaxExperts);
 
   const int warp = threadIdx.x >> 5;
@@ -178,6 +220,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
       mbar_init(&tempty[a], 2 * kEpiWarps);
+      mbar_init(&cfull[a], 1);
+      mbar_init(&cempty[a], kEpiWarps + (leader ? 2 : 1));  // and the producer, the MMA warp
     }
     mbar_init(done, 1);
     *abort_flag = 0;
@@ -255,6 +299,37 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
           }
           if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
+        if (LORA > 0) {
+          if (i == 0) {  // the parts come from the launch before
+            pdl_wait();
+            fence_proxy_async_all();
+          }
+          if (!mbar_wait(&cfull[i & 1], (i >> 1) & 1)) {
+            atomicExch(&g_pair_error, kErrTimeoutProducer);
+            *abort_flag = 1;
+          }
+          RunWalk w(codes + (i & 1) * 16, (t.n + 15) / 16);
+          while (!*abort_flag && w.next()) {
+            const int rows_half = w.count * 8;  // this CTA's half of the run's rows
+            const int boxes = (rows_half + 63) / 64;
+            const int r0 = t.n0 + w.begin * 16 + static_cast<int>(rank) * rows_half;
+            for (int b = 0; b < 2 * p.rank_blocks; ++b) {
+              if (!mbar_wait(&empty[stage], phase ^ 1)) {
+                atomicExch(&g_pair_error, kErrTimeoutProducer);
+                *abort_flag = 1;
+                break;
+              }
+              const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);
+              if (leader) mbar_arrive_expect_tx(&full[stage], 2 * (kABytes + boxes * kBox));
+              tma_load_3d_pair(sA + stage * kABytes, &map_at, bar, (b >> 1) * kBK, a0, w.code);
+              for (int j = 0; j < boxes; ++j)
+                tma_load_3d_pair(sB + stage * kBBytes + j * kBox, &map_bt, bar, (b >> 1) * kBK,
+                                 r0 + j * 64, b & 1);
+              if (++stage == kStages) { stage = 0; phase ^= 1; }
+            }
+          }
+          mbar_arrive(&cempty[i & 1]);
+        }
       }
     }
   } else if (warp == 1) {
@@ -302,11 +377,63 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
           tc_commit_pair(&empty[stage], 0x3);
           if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
+        if (LORA > 0 && ok) {
+          ok = mbar_wait(&cfull[i & 1], (i >> 1) & 1);
+          RunWalk w(codes + (i & 1) * 16, (t.n + 15) / 16);
+          while (ok && w.next()) {
+            const uint32_t run_desc = idesc_f16(TcFormat<T>::kId, kTileM, w.count * 16);
+            for (int b = 0; b < 2 * p.rank_blocks && ok; ++b) {
+              ok = mbar_wait(&full[stage], phase);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t a = smem_u32(sA + stage * kABytes);
+              const uint32_t bb = smem_u32(sB + stage * kBBytes);
+              const int left = p.lora.rank - (b >> 1) * kBK;
+#pragma unroll
+              for (int k = 0; k < kBK / 16; ++k) {
+                if (k * 16 >= left) break;
+                tc_mma_f16_pair(d + w.begin * 16, smem_desc_k_sw128(a + k * 32),
+                                smem_desc_k_sw128(bb + k * 32), run_desc, 1u);
+              }
+              tc_commit_pair(&empty[stage], 0x3);
+              if (++stage == kStages) { stage = 0; phase ^= 1; }
+            }
+          }
+          mbar_arrive(&cempty[i & 1]);
+          if (!ok) {
+            atomicExch(&g_pair_error, kErrTimeoutMma);
+            *abort_flag = 1;
+          }
+        }
         if (!ok) break;
         tc_commit_pair(&tfull[acc], 0x3);
       }
       tc_commit_pair(done, 0x1);
       mbar_wait(done, 0);
+    }
+  } else if (LORA > 0 && warp == 2 + kEpiWarps) {
+    // ------------------------------------- what the tile's rows follow (both CTAs)
+    pdl_wait();
+    for (int i = 0;; ++i) {
+      const int L = turn_tile(i, pair, npairs);
+      if (L >= total || *abort_flag) break;
+      const PairTile t = pair_tile<DIR>(L, table, p);
+      if (!mbar_wait(&cempty[i & 1], ((i >> 1) & 1) ^ 1)) {
+        atomicExch(&g_pair_error, kErrTimeoutProducer);
+        *abort_flag = 1;
+        break;
+      }
+      // Eight rows a lane, then the two lanes of a group.
+      int code = kAnyCode;
+      for (int k = 0; k < 8; ++k) {
+        const int r = lane * 8 + k;
+        code = join_codes(code, r < t.n ? p.lora.row_code[t.n0 + r] : kAnyCode);
+      }
+      code = join_codes(code, __shfl_xor_sync(0xffffffffu, code, 1));
+      if (code >= kLoraScaled) code = kMixedCode;
+      if ((lane & 1) == 0) codes[(i & 1) * 16 + lane / 2] = code;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&cfull[i & 1]);
     }
   } else {
     // ----------------------------------------------------- epilogue (both CTAs)
@@ -378,31 +505,47 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
       };
       if constexpr (LORA > 0) {
         LoraFrags<LORA> frags;  // of this tile's features
+        if (!mbar_wait(&cfull[i & 1], (i >> 1) & 1)) {
+          atomicExch(&g_pair_error, kErrTimeoutEpilogue);
+          *abort_flag = 1;
+          break;
+        }
         for (int c = first; c < t.n; c += 64) {
-          // The chunk's adapters and packed parts are fetched ahead of the accumulators: one
-          // trip to L2 a chunk instead of one a row block.
-          const int ads = lora_adapter(p.lora, t.n0 + c + lane, c + lane < t.n);
+          const volatile int* code = codes + (i & 1) * 16 + c / 16;
+          const bool mixed0 = code[0] == kMixedCode, mixed1 = code[1] == kMixedCode;
+          // The rows' parts are fetched ahead of the accumulators: one trip to L2 a chunk
+          // instead of one a row block.
+          int ads = -1;
           uint4 parts[4][LORA];
+          if (mixed0 || mixed1) {
+            if (c + lane < t.n) {
+              const int rc = p.lora.row_code[t.n0 + c + lane];
+              ads = rc < 0 ? -1 : rc & (kLoraScaled - 1);
+            }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int row = c + 8 * j + (lane >> 2);
-            lora_rows<LORA>(p.lora, t.n0 + row, row < t.n, 0, parts[j]);
+            for (int j = 0; j < 4; ++j) {
+              const int row = c + 8 * j + (lane >> 2);
+              lora_rows<LORA>(p.lora, p.rows, t.n0 + row, row < t.n, 0, parts[j]);
+            }
           }
           float lo[16], hi[16];
           fetch(c, lo, hi);
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
+            if (j < 2 ? !mixed0 : !mixed1) continue;
             float dl[4], dh[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) { dl[k] = lo[4 * j + k]; dh[k] = hi[4 * j + k]; }
-            lora_add<T, LORA>(p.lora, __shfl_sync(0xffffffffu, ads, 8 * j + (lane >> 2)),
+            lora_add<T, LORA>(p.lora, p.rows, __shfl_sync(0xffffffffu, ads, 8 * j + (lane >> 2)),
                               t.n0 + c + 8 * j + (lane >> 2), m, p.m_dim, parts[j], frags, dl, dh);
 #pragma unroll
             for (int k = 0; k < 4; ++k) { lo[4 * j + k] = dl[k]; hi[4 * j + k] = dh[k]; }
           }
           store(c, lo, hi);
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&cempty[i & 1]);
         release();
       } else {
         // The next columns are on their way from tensor memory while these are stored, and
@@ -552,6 +695,12 @@ cudaError_t launch_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
     if (!ok) return cudaErrorInvalidValue;
     mat = ma;
     mbt = mb;
+    if (LORA > 0) {
+      p.rank_blocks = (lora->rank + kBK - 1) / kBK;
+      if (!grouped_map(&mat, g.dtype, lora->b, lora->rank, g.N, lora->adapters, 128) ||
+          !grouped_map(&mbt, g.dtype, lora->parts, lora->rank, g.rows, 2, 64))
+        return cudaErrorInvalidValue;
+    }
     p.tile_rows = kTileN;
     if (g.E == 1) p.tile_rows = tile_rows_one_group(g.rows, (feat + kTileM - 1) / kTileM, num_sms / 2);
   }
@@ -565,7 +714,7 @@ cudaError_t launch_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
   if (st != cudaSuccess) return st;
   const int64_t pairs = std::min<int64_t>(tiles, num_sms / 2);
   return launch_overlapped(grouped_pair_kernel<T, DIR, LORA>, static_cast<unsigned>(2 * pairs),
-                           kThreads, kSmem, 0, s, ma, mb, mat, mbt, p);
+                           LORA > 0 ? kLoraThreads : kThreads, kSmem, 0, s, ma, mb, mat, mbt, p);
 }
 
 template <typename T>

@@ -11,8 +11,8 @@
 // chunk is one pass; a decode chunk of 8 rows is at most 8 adapters, read once each.
 // Bound: the bytes of A_a (decode) and of x (prefill); the products are few.  The splits of
 // a chunk are a cluster: each leaves its partial sums in shared memory, and each row's are
-// added in rank order by one warp, which scales, splits and packs them as the epilogue of
-// the projection takes them (grouped_lora.cuh).
+// added in rank order by one warp, which scales them and splits them into the 16-bit parts
+// that the projection takes (grouped_lora.cuh).
 #include <algorithm>
 
 #include "grouped_tc.cuh"
@@ -61,8 +61,9 @@ constexpr int kTcThreads = 256;   // warp 0 TMA, warp 1 MMA, warps 4..7 epilogue
 struct ShrinkParams {
   const int32_t* ids;
   const float* scales;
-  uint4* packed;
+  uint16_t* parts;
   float* row_scale;
+  int* row_code;
   int64_t rows;
   int K, rank, adapters;
   int chunk;      // rows of a CTA: 4, 8 or 64
@@ -82,13 +83,13 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   return v;
 }
 
-// Two 16-bit parts of each of four values, {hi, hi, lo, lo}.
+// Two 16-bit parts of each of four values.
 template <typename T>
-__device__ __forceinline__ uint4 pack_parts(const float4& v) {
+__device__ __forceinline__ void split_parts(const float4& v, uint2& hi, uint2& lo) {
   const float h0 = to_f(from_f<T>(v.x)), h1 = to_f(from_f<T>(v.y));
   const float h2 = to_f(from_f<T>(v.z)), h3 = to_f(from_f<T>(v.w));
-  return make_uint4(pack2<T>(h0, h1), pack2<T>(h2, h3), pack2<T>(v.x - h0, v.y - h1),
-                    pack2<T>(v.z - h2, v.w - h3));
+  hi = make_uint2(pack2<T>(h0, h1), pack2<T>(h2, h3));
+  lo = make_uint2(pack2<T>(v.x - h0, v.y - h1), pack2<T>(v.z - h2, v.w - h3));
 }
 
 template <typename T>
@@ -282,9 +283,11 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
   cluster_sync();  // every split's partial sums are in its `part`
   // Row i of the chunk is finished by CTA i % splits, one warp a row; a lane takes granules
   // of four entries.
-  const int steps = (p.rank + 15) / 16;
   for (int i = split + p.splits * warp; i < n; i += p.splits * (kTcThreads / 32)) {
-    if (s_slot[i] < 0) continue;
+    if (s_slot[i] < 0) {
+      if (lane == 0) p.row_code[row0 + i] = -1;
+      continue;
+    }
     const float sc = __ldg(p.scales + s_id[i]);
     float4 v[2];
     float m = 0.f;
@@ -306,23 +309,34 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
       }
       m = fmaxf(m, fmaxf(fmaxf(fabsf(v[h].x), fabsf(v[h].y)), fmaxf(fabsf(v[h].z), fabsf(v[h].w))));
     }
+    int code = s_id[i];
     if (std::is_same<T, __half>::value) {
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
       float down = 1.f;
-      if (m > 0.f && m < __int_as_float(0x7f800000)) {
+      // Inside [2^-8, 2^15) the parts keep 16 bits of the row's largest entry as they are.
+      if ((m > 0.f && m < 0.00390625f) || (m >= 32768.f && m < __int_as_float(0x7f800000))) {
         const int e = min(max((__float_as_int(m) >> 23) - 127, -120), 120);
         const float up = __int_as_float((127 - e) << 23);
         down = __int_as_float((127 + e) << 23);
+        code |= kLoraScaled;
 #pragma unroll
         for (int h = 0; h < 2; ++h) { v[h].x *= up; v[h].y *= up; v[h].z *= up; v[h].w *= up; }
       }
       if (lane == 0) p.row_scale[row0 + i] = down;
     }
-    uint4* dst = p.packed + (row0 + i) * steps * 4;
+    if (lane == 0) p.row_code[row0 + i] = code;
+    uint16_t* dst = p.parts + (row0 + i) * p.rank;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (lane + 32 * h < steps * 4) dst[lane + 32 * h] = pack_parts<T>(v[h]);
+    for (int h = 0; h < 2; ++h) {
+      const int j = 4 * (lane + 32 * h);
+      if (j < p.rank) {
+        uint2 hi, lo;
+        split_parts<T>(v[h], hi, lo);
+        *reinterpret_cast<uint2*>(dst + j) = hi;
+        *reinterpret_cast<uint2*>(dst + j + p.rows * p.rank) = lo;
+      }
+    }
   }
   cluster_sync();  // no CTA leaves while another reads its part
 }
@@ -339,13 +353,14 @@ cudaError_t shrink_simt(const LoraShrink& l, float* t, cudaStream_t s) {
 }
 
 template <typename T>
-cudaError_t shrink_tc(const LoraShrink& l, uint4* packed, float* row_scale, int num_sms,
-                      cudaStream_t s) {
+cudaError_t shrink_tc(const LoraShrink& l, uint16_t* parts, float* row_scale, int* row_code,
+                      int num_sms, cudaStream_t s) {
   ShrinkParams p{};
   p.ids = l.ids;
   p.scales = l.scales;
-  p.packed = packed;
+  p.parts = parts;
   p.row_scale = row_scale;
+  p.row_code = row_code;
   p.rows = l.rows;
   p.K = l.K;
   p.rank = l.rank;
@@ -394,10 +409,11 @@ bool lora_shrink_tc_supported(const LoraShrink& l) {
   return aligned(l.x) && aligned(l.a);
 }
 
-cudaError_t launch_lora_shrink_tc(const LoraShrink& l, uint4* packed, float* row_scale,
-                                  int num_sms, cudaStream_t s) {
-  if (l.dtype == kDtF16) return shrink_tc<__half>(l, packed, row_scale, num_sms, s);
-  if (l.dtype == kDtBF16) return shrink_tc<__nv_bfloat16>(l, packed, row_scale, num_sms, s);
+cudaError_t launch_lora_shrink_tc(const LoraShrink& l, uint16_t* parts, float* row_scale,
+                                  int* row_code, int num_sms, cudaStream_t s) {
+  if (l.dtype == kDtF16) return shrink_tc<__half>(l, parts, row_scale, row_code, num_sms, s);
+  if (l.dtype == kDtBF16)
+    return shrink_tc<__nv_bfloat16>(l, parts, row_scale, row_code, num_sms, s);
   return cudaErrorInvalidValue;
 }
 
