@@ -9,17 +9,19 @@
 //   grad_input   A = dy rows (c contiguous)   B = W[e][c, n]  (n contiguous)
 //   grad_weight  A = dy[c, m] (m contiguous)  B = x[c, n]     (n contiguous), c = rows of e
 // Bound: FFMA issue.  Each thread owns TM x TN sums, so a step of c costs TM + TN shared
-// loads for TM * TN FMAs; the next 16-deep slice is loaded to registers while the current
-// one is multiplied (double-buffered shared memory, one barrier per slice).
+// loads for TM * TN FMAs; the next slice is loaded to registers while the current one is
+// multiplied (double-buffered shared memory, one barrier per slice).  A call with few tiles
+// waits for memory instead, slice after slice; there the contraction is split over a cluster
+// of up to four CTAs, whose partial sums meet in distributed shared memory: each owns some of
+// the tile's rows and adds the parts in rank order.
 #include <algorithm>
 
-#include "grouped.h"
+#include "grouped_tc.cuh"
 
 namespace moe {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kDepth = 16;  // contraction depth of one shared slice
 
 struct SimtParams {
   const void* a;
@@ -29,6 +31,7 @@ struct SimtParams {
   int64_t rows;
   int N, K, E;
   int a_vec, b_vec;  // 4-element loads are aligned and rows are a multiple of 4 long
+  int splits;        // cluster size along the contraction (not grad_weight)
   LoraTerm lora;
 };
 
@@ -101,9 +104,9 @@ __device__ __forceinline__ float4 load4(const T* p, int n, int vec) {
   return make_float4(v[0], v[1], v[2], v[3]);
 }
 
-// One operand's slice: X rows x kDepth into s[kDepth][X + pad].  CONTIG_C: element (i, c)
+// One operand's slice: X rows x kDepth contraction entries into s[kDepth][X + pad].  CONTIG_C: element (i, c)
 // at p[i * ld + c], else at p[c * ld + i]; i < ni and c < nc are valid.
-template <typename T, int X, bool CONTIG_C>
+template <typename T, int X, int kDepth, bool CONTIG_C>
 struct Slice {
   static constexpr int kPitch = X + 4;
   static constexpr int kQuads = X * kDepth / 4 / kThreads;
@@ -149,13 +152,15 @@ template <typename T, int DIR, int TM, int TN>
 __global__ void __launch_bounds__(kThreads)
 grouped_simt_kernel(const SimtParams p) {
   constexpr int BM = 16 * TM, BN = 16 * TN;
+  constexpr int kDepth = TM == 4 ? 32 : 16;
   constexpr bool kAC = DIR != kGmmGradWeight;  // contraction contiguous in A
   constexpr bool kBC = DIR == kGmmForward;
-  using SA = Slice<T, BM, kAC>;
-  using SB = Slice<T, BN, kBC>;
+  using SA = Slice<T, BM, kDepth, kAC>;
+  using SB = Slice<T, BN, kDepth, kBC>;
   __shared__ __align__(16) float sa[2][kDepth * SA::kPitch];
   __shared__ __align__(16) float sb[2][kDepth * SB::kPitch];
 
+  pdl_wait();
   const int rows = static_cast<int>(p.rows);
   const T* a;
   const T* b;
@@ -202,16 +207,21 @@ grouped_simt_kernel(const SimtParams p) {
 
   SA fa;
   SB fb;
-  const int slices = (nc + kDepth - 1) / kDepth;
-  if (slices > 0) {
-    fa.load(a, lda, nm, 0, nc, p.a_vec);
-    fb.load(b, ldb, nn, 0, nc, p.b_vec);
+  // This CTA's slices (all of them unless the contraction is split).
+  constexpr bool kSplit = DIR != kGmmGradWeight && TM == 4;
+  const int S = kSplit ? p.splits : 1;
+  const int me = S > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int all = (nc + kDepth - 1) / kDepth;
+  const int from = all * me / S, slices = all * (me + 1) / S;
+  if (slices > from) {
+    fa.load(a, lda, nm, from * kDepth, nc, p.a_vec);
+    fb.load(b, ldb, nn, from * kDepth, nc, p.b_vec);
     fa.store(sa[0]);
     fb.store(sb[0]);
   }
   __syncthreads();
-  for (int s = 0; s < slices; ++s) {
-    const int cur = s & 1;
+  for (int s = from; s < slices; ++s) {
+    const int cur = (s - from) & 1;
     if (s + 1 < slices) {
       fa.load(a, lda, nm, (s + 1) * kDepth, nc, p.a_vec);
       fb.load(b, ldb, nn, (s + 1) * kDepth, nc, p.b_vec);
@@ -239,8 +249,43 @@ grouped_simt_kernel(const SimtParams p) {
     __syncthreads();
   }
 
+  if constexpr (kSplit) {
+    if (S > 1) {
+      // Row i of each thread's four goes to CTA i S / 4, which adds the parts in rank order.
+      static_assert(sizeof(sa) >= 3 * 256 * 16, "parts fit the operand slices");
+      float4* parts = reinterpret_cast<float4*>(&sa[0][0]);  // [S - 1][4 / S][256]
+      const int per = TM / S;
+      cluster_sync();  // every CTA has read its slices
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const int owner = i / per;
+        if (owner == me) continue;
+        const int slot = me < owner ? me : me - 1;
+        const uint32_t at = smem_u32(parts + (slot * per + i % per) * kThreads + threadIdx.x);
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
+                         mapa_shared(at, owner)),
+                     "f"(acc[i][0]), "f"(acc[i][1]), "f"(acc[i][2]), "f"(acc[i][3])
+                     : "memory");
+      }
+      cluster_sync();
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        if (i / per != me) continue;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int r = 0; r < S; ++r) {
+          const float4 v = r == me ? make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3])
+                                   : parts[((r < me ? r : r - 1) * per + i % per) * kThreads +
+                                           threadIdx.x];
+          sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+        }
+        acc[i][0] = sum.x; acc[i][1] = sum.y; acc[i][2] = sum.z; acc[i][3] = sum.w;
+      }
+    }
+  }
+
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
+    if (kSplit && S > 1 && i / (TM / S) != me) continue;
     const int m = ty * 4 + (i / 4) * 64 + (i & 3);
     if (m >= nm) continue;
     if (DIR == kGmmForward && p.lora.t != nullptr) {
@@ -273,9 +318,10 @@ grouped_simt_kernel(const SimtParams p) {
 }
 
 template <typename T, int DIR, int TM>
-cudaError_t launch_tile(const GroupedArgs& g, const SimtParams& p, cudaStream_t s) {
+cudaError_t launch_tile(const GroupedArgs& g, SimtParams p, cudaStream_t s) {
   constexpr int B = 16 * TM;
   dim3 grid;
+  p.splits = 1;
   if (DIR == kGmmGradWeight) {
     grid = dim3((g.K + B - 1) / B, (g.N + B - 1) / B, g.E);
   } else {
@@ -283,9 +329,27 @@ cudaError_t launch_tile(const GroupedArgs& g, const SimtParams& p, cudaStream_t 
     const int feat = DIR == kGmmForward ? g.N : g.K;
     const int64_t tiles = g.rows / B + std::min<int64_t>(g.rows, g.E);
     grid = dim3(static_cast<unsigned>(tiles), (feat + B - 1) / B, 1);
+    // Split until about four CTAs an SM run, with at least two slices of 32 each.
+    const int con = DIR == kGmmForward ? g.K : g.N;
+    if (TM == 4)
+      while (p.splits < 4 && tiles * grid.y * p.splits * 2 <= 4 * 148 && con >= 128 * p.splits)
+        p.splits *= 2;
+    grid.z = p.splits;
   }
-  grouped_simt_kernel<T, DIR, TM, TM><<<grid, kThreads, 0, s>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = static_cast<unsigned>(p.splits);
+  cfg.attrs = attr;
+  cfg.numAttrs = p.splits > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, grouped_simt_kernel<T, DIR, TM, TM>, p);
 }
 
 template <typename T, int DIR>
