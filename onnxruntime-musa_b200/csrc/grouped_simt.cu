@@ -31,7 +31,7 @@ struct SimtParams {
   int64_t rows;
   int N, K, E;
   int a_vec, b_vec;  // 4-element loads are aligned and rows are a multiple of 4 long
-  int splits;        // cluster size along the contraction (not grad_weight)
+  int splits;        // cluster size along the contraction
   LoraTerm lora;
 };
 
@@ -109,14 +109,15 @@ __device__ __forceinline__ float4 load4(const T* p, int n, int vec) {
 template <typename T, int X, int kDepth, bool CONTIG_C>
 struct Slice {
   static constexpr int kPitch = X + 4;
-  static constexpr int kQuads = X * kDepth / 4 / kThreads;
-  static_assert(kQuads >= 1, "");
+  static constexpr int kAll = X * kDepth / 4;
+  static constexpr int kQuads = (kAll + kThreads - 1) / kThreads;
   float4 v[kQuads];
 
   __device__ __forceinline__ void load(const T* p, int64_t ld, int ni, int c0, int nc, int vec) {
 #pragma unroll
     for (int j = 0; j < kQuads; ++j) {
       const int q = threadIdx.x + j * kThreads;
+      if (kAll % kThreads != 0 && q >= kAll) continue;
       if (CONTIG_C) {
         const int i = q / (kDepth / 4), c = c0 + (q % (kDepth / 4)) * 4;
         v[j] = i < ni && c < nc ? load4<T>(p + i * ld + c, nc - c, vec)
@@ -132,6 +133,7 @@ struct Slice {
 #pragma unroll
     for (int j = 0; j < kQuads; ++j) {
       const int q = threadIdx.x + j * kThreads;
+      if (kAll % kThreads != 0 && q >= kAll) continue;
       if (CONTIG_C) {
         const int i = q / (kDepth / 4), c = (q % (kDepth / 4)) * 4;
         s[(c + 0) * kPitch + i] = v[j].x;
@@ -146,13 +148,28 @@ struct Slice {
   }
 };
 
-// CTA tile (16 TM) x (16 TN) with TM, TN multiples of 4: thread (ty, tx) owns rows
-// ty * 4 + 64 i + [0, 4) and columns tx * 4 + 64 j + [0, 4).
+// Two fp32 values in a register pair, and the packed FMA on them (each half rounds as fmaf).
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// CTA tile (16 TM) x (16 TN), TN a multiple of 4 and TM too or 1: thread (ty, tx) owns rows
+// ty * 4 + 64 i + [0, 4) (TM = 1: row ty) and columns tx * 4 + 64 j + [0, 4).
 template <typename T, int DIR, int TM, int TN>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, TM <= 4 ? 4 : 2)
 grouped_simt_kernel(const SimtParams p) {
   constexpr int BM = 16 * TM, BN = 16 * TN;
-  constexpr int kDepth = TM == 4 ? 32 : 16;
+  constexpr int kDepth = TM <= 4 ? 32 : 16;
   constexpr bool kAC = DIR != kGmmGradWeight;  // contraction contiguous in A
   constexpr bool kBC = DIR == kGmmForward;
   using SA = Slice<T, BM, kDepth, kAC>;
@@ -169,7 +186,7 @@ grouped_simt_kernel(const SimtParams p) {
   int nm, nn, nc, row0 = 0;  // valid rows, columns and contraction length of this tile
   const int col0 = (DIR == kGmmGradWeight ? blockIdx.x : blockIdx.y) * BN;
   if (DIR == kGmmGradWeight) {
-    const int e = blockIdx.z, m0 = blockIdx.y * BM;
+    const int e = blockIdx.z / p.splits, m0 = blockIdx.y * BM;
     const int begin = group_begin(p.offsets, e, rows);
     nc = group_end(p.offsets, e, rows, begin) - begin;
     lda = p.N;
@@ -199,16 +216,17 @@ grouped_simt_kernel(const SimtParams p) {
   nn = min(nn, BN);
 
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[TM][TN];
+  const bool busy = (ty & ~1) * (TM == 1 ? 1 : 4) < nm;  // some row of this warp is valid
+  uint64_t acc2[TM][TN / 2];  // two adjacent columns each
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = 0.f;
+    for (int j = 0; j < TN / 2; ++j) acc2[i][j] = 0;
 
   SA fa;
   SB fb;
   // This CTA's slices (all of them unless the contraction is split).
-  constexpr bool kSplit = DIR != kGmmGradWeight && TM == 4;
+  constexpr bool kSplit = TM <= 4;
   const int S = kSplit ? p.splits : 1;
   const int me = S > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int all = (nc + kDepth - 1) / kDepth;
@@ -226,21 +244,30 @@ grouped_simt_kernel(const SimtParams p) {
       fa.load(a, lda, nm, (s + 1) * kDepth, nc, p.a_vec);
       fb.load(b, ldb, nn, (s + 1) * kDepth, nc, p.b_vec);
     }
+    if (busy) {
 #pragma unroll
-    for (int c = 0; c < kDepth; ++c) {
-      float ra[TM], rb[TN];
+      for (int c = 0; c < kDepth; ++c) {
+        float ra[TM];
+        uint64_t rb[TN / 2];
+        if constexpr (TM == 1) {
+          ra[0] = sa[cur][c * SA::kPitch + ty];
+        } else {
 #pragma unroll
-      for (int i = 0; i < TM; i += 4)
-        *reinterpret_cast<float4*>(ra + i) =
-            *reinterpret_cast<const float4*>(&sa[cur][c * SA::kPitch + ty * 4 + i * 16]);
+          for (int i = 0; i < TM; i += 4)
+            *reinterpret_cast<float4*>(ra + i) =
+                *reinterpret_cast<const float4*>(&sa[cur][c * SA::kPitch + ty * 4 + i * 16]);
+        }
 #pragma unroll
-      for (int j = 0; j < TN; j += 4)
-        *reinterpret_cast<float4*>(rb + j) =
-            *reinterpret_cast<const float4*>(&sb[cur][c * SB::kPitch + tx * 4 + j * 16]);
+        for (int j = 0; j < TN; j += 4)
+          *reinterpret_cast<ulonglong2*>(rb + j / 2) =
+              *reinterpret_cast<const ulonglong2*>(&sb[cur][c * SB::kPitch + tx * 4 + j * 16]);
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TM; ++i) {
+          const uint64_t aa = pair2(ra[i], ra[i]);
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = fmaf(ra[i], rb[j], acc[i][j]);
+          for (int j = 0; j < TN / 2; ++j) acc2[i][j] = fma2(aa, rb[j], acc2[i][j]);
+        }
+      }
     }
     if (s + 1 < slices) {
       fa.store(sa[cur ^ 1]);
@@ -249,16 +276,23 @@ grouped_simt_kernel(const SimtParams p) {
     __syncthreads();
   }
 
+  float acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN / 2; ++j) unpair2(acc2[i][j], acc[i][2 * j], acc[i][2 * j + 1]);
+
   if constexpr (kSplit) {
     if (S > 1) {
-      // Row i of each thread's four goes to CTA i S / 4, which adds the parts in rank order.
-      static_assert(sizeof(sa) >= 3 * 256 * 16, "parts fit the operand slices");
-      float4* parts = reinterpret_cast<float4*>(&sa[0][0]);  // [S - 1][4 / S][256]
-      const int per = TM / S;
+      // Row i of each thread's four goes to CTA i S / 4 (TM = 1: the thread's row to CTA
+      // ty % S), which adds the parts in rank order.
+      float4* parts = reinterpret_cast<float4*>(&sb[0][0]);  // [S - 1][rows owned][256]
+      static_assert(sizeof(sb) >= 3 * kThreads * 16, "parts fit the operand slices");
+      const int per = TM == 1 ? 1 : TM / S;
       cluster_sync();  // every CTA has read its slices
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        const int owner = i / per;
+        const int owner = TM == 1 ? ty % S : i / per;
         if (owner == me) continue;
         const int slot = me < owner ? me : me - 1;
         const uint32_t at = smem_u32(parts + (slot * per + i % per) * kThreads + threadIdx.x);
@@ -270,7 +304,7 @@ grouped_simt_kernel(const SimtParams p) {
       cluster_sync();
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        if (i / per != me) continue;
+        if ((TM == 1 ? ty % S : i / per) != me) continue;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int r = 0; r < S; ++r) {
           const float4 v = r == me ? make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3])
@@ -285,8 +319,8 @@ grouped_simt_kernel(const SimtParams p) {
 
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
-    if (kSplit && S > 1 && i / (TM / S) != me) continue;
-    const int m = ty * 4 + (i / 4) * 64 + (i & 3);
+    if (kSplit && S > 1 && (TM == 1 ? ty % S : i * S / TM) != me) continue;
+    const int m = TM == 1 ? ty : ty * 4 + (i / 4) * 64 + (i & 3);
     if (m >= nm) continue;
     if (DIR == kGmmForward && p.lora.t != nullptr) {
       // y += s_a * sum_j t[row, j] B_a[n, j].
@@ -317,25 +351,28 @@ grouped_simt_kernel(const SimtParams p) {
   }
 }
 
-template <typename T, int DIR, int TM>
+template <typename T, int DIR, int TM, int TN>
 cudaError_t launch_tile(const GroupedArgs& g, SimtParams p, cudaStream_t s) {
-  constexpr int B = 16 * TM;
+  constexpr int BM = 16 * TM, BN = 16 * TN;
   dim3 grid;
   p.splits = 1;
+  int64_t tiles, con;
   if (DIR == kGmmGradWeight) {
-    grid = dim3((g.K + B - 1) / B, (g.N + B - 1) / B, g.E);
+    grid = dim3((g.K + BN - 1) / BN, (g.N + BM - 1) / BM, g.E);
+    tiles = static_cast<int64_t>(grid.x) * grid.y * grid.z;
+    con = g.rows / g.E;
   } else {
     // The tile count lives on the device; ragged groups add at most one tile each.
     const int feat = DIR == kGmmForward ? g.N : g.K;
-    const int64_t tiles = g.rows / B + std::min<int64_t>(g.rows, g.E);
-    grid = dim3(static_cast<unsigned>(tiles), (feat + B - 1) / B, 1);
-    // Split until about four CTAs an SM run, with at least two slices of 32 each.
-    const int con = DIR == kGmmForward ? g.K : g.N;
-    if (TM == 4)
-      while (p.splits < 4 && tiles * grid.y * p.splits * 2 <= 4 * 148 && con >= 128 * p.splits)
-        p.splits *= 2;
-    grid.z = p.splits;
+    const int64_t rows_tiles = g.rows / BM + std::min<int64_t>(g.rows, g.E);
+    grid = dim3(static_cast<unsigned>(rows_tiles), (feat + BN - 1) / BN, 1);
+    tiles = rows_tiles * grid.y;
+    con = DIR == kGmmForward ? g.K : g.N;
   }
+  // Split until about four CTAs an SM run, with at least two slices of 32 each.
+  if (TM <= 4)
+    while (p.splits < 4 && tiles * p.splits * 2 <= 4 * 148 && con >= 128 * p.splits) p.splits *= 2;
+  grid.z *= p.splits;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(kThreads);
@@ -349,7 +386,7 @@ cudaError_t launch_tile(const GroupedArgs& g, SimtParams p, cudaStream_t s) {
   attr[1].val.clusterDim.z = static_cast<unsigned>(p.splits);
   cfg.attrs = attr;
   cfg.numAttrs = p.splits > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, grouped_simt_kernel<T, DIR, TM, TM>, p);
+  return cudaLaunchKernelEx(&cfg, grouped_simt_kernel<T, DIR, TM, TN>, p);
 }
 
 template <typename T, int DIR>
@@ -371,13 +408,16 @@ cudaError_t launch_dir(const GroupedArgs& g, const LoraTerm* lora, cudaStream_t 
   if (lora != nullptr) p.lora = *lora;
   // 128 x 128 tiles once they fill the GPU twice over (each thread then does 64 FMAs per
   // 16 shared loads instead of 16 per 8); below that the 64 x 64 tiles' four times as many
-  // CTAs win.
+  // CTAs win.  Groups of a few rows take tiles of 16 rows, which multiply less padding.
   const int64_t feat = DIR == kGmmForward ? g.N : g.K;
   const int64_t big = DIR == kGmmGradWeight
                           ? static_cast<int64_t>(g.E) * ((g.N + 127) / 128) * ((g.K + 127) / 128)
                           : (g.rows / 128) * ((feat + 127) / 128);
-  if (big >= 2 * 148) return launch_tile<T, DIR, 8>(g, p, s);
-  return launch_tile<T, DIR, 4>(g, p, s);
+  if (big >= 2 * 148) return launch_tile<T, DIR, 8, 8>(g, p, s);
+  if constexpr (DIR != kGmmGradWeight) {
+    if (g.rows <= 16 * static_cast<int64_t>(g.E)) return launch_tile<T, DIR, 1, 4>(g, p, s);
+  }
+  return launch_tile<T, DIR, 4, 4>(g, p, s);
 }
 
 template <typename T>
