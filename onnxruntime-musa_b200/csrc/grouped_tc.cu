@@ -53,7 +53,7 @@ constexpr int kThreads = 320;
 constexpr int kLoraThreads = 352;        // warp 10: the tile's runs of rows
 constexpr int kEpiWarps = 8;
 constexpr int kStageRow = 64;            // bytes of one staged output row (32 elements)
-constexpr int kEpiBytes = 2 * 8 * kStageRow;  // per warp: two buffers of 8 rows
+constexpr int kEpiBytes = 4 * 8 * kStageRow;  // per warp: four blocks of 8 rows
 constexpr int kRaster = 8;               // M-fastest runs of this many tiles (L2 reuse)
 constexpr int kTailRows = 16;
 constexpr int kSmem = 1024 + kStages * (kABytes + kBBytes) + kEpiWarps * kEpiBytes + 384 +
@@ -473,34 +473,46 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
         tmem_ld_frag4(taddr + c, lo);
         tmem_ld_frag4(taddr + (16u << 16) + c, hi);
       };
-      // Stores 32 columns of the accumulator, c .. c + 31.
+      // Stores 32 columns of the accumulator, c .. c + 31: four 8 x 32 blocks go through the
+      // warp's staging memory and leave as 16-byte pieces of 64-byte rows.  The four go
+      // together, so their latencies overlap.
       auto store = [&](int c, float (&lo)[16], float (&hi)[16]) {
+        __syncwarp();  // the staged blocks before have been read
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int sel = (j & 1) * 8 * kStageRow;
-          T* dst;
-          bool ok;
           if (DIR == kGmmGradWeight) {
             // Eight M rows (block j of the 32) x 32 columns.
             const float(&v)[16] = j < 2 ? lo : hi;
             const int o = (j & 1) * 2;
-            stmatrix4(st_addr + sel, pack2<T>(v[o], v[o + 1]), pack2<T>(v[4 + o], v[5 + o]),
-                      pack2<T>(v[8 + o], v[9 + o]), pack2<T>(v[12 + o], v[13 + o]));
-            const int row = m + 8 * j + rd_row, col = c + 8 * rd_blk;
-            ok = row < p.m_dim && col < t.n;
-            dst = out + (static_cast<int64_t>(t.e) * p.m_dim + row) * p.ldo + t.n0 + col;
+            stmatrix4(st_addr + j * 8 * kStageRow, pack2<T>(v[o], v[o + 1]),
+                      pack2<T>(v[4 + o], v[5 + o]), pack2<T>(v[8 + o], v[9 + o]),
+                      pack2<T>(v[12 + o], v[13 + o]));
           } else {
             // Eight rows of the output (accumulator columns) x 32 features, transposed.
-            stmatrix4_t(st_addr + sel, pack2<T>(lo[4 * j], lo[4 * j + 1]),
+            stmatrix4_t(st_addr + j * 8 * kStageRow, pack2<T>(lo[4 * j], lo[4 * j + 1]),
                         pack2<T>(lo[4 * j + 2], lo[4 * j + 3]), pack2<T>(hi[4 * j], hi[4 * j + 1]),
                         pack2<T>(hi[4 * j + 2], hi[4 * j + 3]));
-            const int row = c + 8 * j + rd_row, col = m + 8 * rd_blk;
-            ok = row < t.n && col < p.m_dim;
-            dst = out + static_cast<int64_t>(t.n0 + row) * p.ldo + col;
           }
-          __syncwarp();
-          const uint4 w = *reinterpret_cast<const uint4*>(rd_ptr + sel);
-          if (ok) *reinterpret_cast<uint4*>(dst) = w;
+        }
+        __syncwarp();
+        uint4 w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          w[j] = *reinterpret_cast<const uint4*>(rd_ptr + j * 8 * kStageRow);
+        if (DIR == kGmmGradWeight) {
+          const int row = m + rd_row, col = c + 8 * rd_blk;
+          T* dst = out + (static_cast<int64_t>(t.e) * p.m_dim + row) * p.ldo + t.n0 + col;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (row + 8 * j < p.m_dim && col < t.n)
+              *reinterpret_cast<uint4*>(dst + 8 * j * p.ldo) = w[j];
+        } else {
+          const int row = c + rd_row, col = m + 8 * rd_blk;
+          T* dst = out + static_cast<int64_t>(t.n0 + row) * p.ldo + col;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (row + 8 * j < t.n && col < p.m_dim)
+              *reinterpret_cast<uint4*>(dst + 8 * j * p.ldo) = w[j];
         }
       };
       if constexpr (LORA > 0) {
