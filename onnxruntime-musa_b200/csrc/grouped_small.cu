@@ -83,7 +83,7 @@ __device__ __forceinline__ void cluster_wait() {
 }
 
 template <typename T, int DIR, int LORA>
-__global__ void __launch_bounds__(kThreads, LORA > 0 ? 1 : 2)
+__global__ void __launch_bounds__(LORA > 0 ? 512 : kThreads, LORA > 0 ? 1 : 2)  // 128 / 96 registers
 grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
                      const __grid_constant__ CUtensorMap map_x, const SmallParams p) {
   constexpr bool kAMn = DIR == kGmmGradInput;
@@ -225,7 +225,7 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
       // One copy of the code for all of it: a warp runs it a few times only, and fetching
       // instructions waits in the same queues (with gather and apply at three places each it
       // took 8 us longer).
-      LoraBatch<T, LORA, 6 / LORA> batch;
+      LoraBatch<T, LORA, 4 / LORA> batch;
       batch.clear();
       const int g = lane >> 2;
       int i = pair;
@@ -389,9 +389,11 @@ cudaError_t launch_small(const GroupedArgs& g, const LoraTerm* lora, int num_sms
   const int64_t tiles = (g.rows / p.cap + std::min<int64_t>(g.rows, g.E)) * p.m_tiles;
   // CTAs an SM: two, sharing its memory, up to 128 rows; one at 256.  (One alone with 130 KB
   // was slower: clusters of such CTAs do not all find room at once, 16.5 against 13.4 us for
-  // 64 rows, 4096 x 4096.)  With adapters two need blocks of 192 threads for their registers.
+  // 64 rows, 4096 x 4096.)  With adapters two have 192 threads, and of 32 or 64 rows 85 KB, which
+  // leaves room for a CTA of the kernel that forms the parts, so that the weights stream
+  // while that runs (up to 16 rows that has few CTAs, and more bytes in flight count).
   const int resident = p.cap > 128 ? 1 : 2;
-  const int budget = p.cap > 128 ? 220 * 1024 : 113 * 1024;
+  const int budget = (p.cap > 128 ? 220 : LORA > 0 && (p.cap == 32 || p.cap == 64) ? 86 : 113) * 1024;
   const int threads = LORA > 0 && resident == 2 ? 192 : kThreads;
   // Splits: until the grid fills these, with at least two slices each.
   const int64_t fill = static_cast<int64_t>(num_sms) * resident;

@@ -8,7 +8,7 @@
 // of K.  The A_a of the chunk's distinct adapters are stacked as the MMA's M (128 / r
 // adapters a pass), its rows are the N, and each column keeps the lanes of its own adapter:
 // rows need no sorting, and another adapter's values never reach a row.  One prompt in a
-// chunk is one pass; a decode chunk of 8 rows is at most 8 adapters, read once each.
+// chunk is one pass; a decode chunk of 4 rows is at most 4 adapters, read once each.
 // Bound: the bytes of A_a (decode) and of x (prefill); the products are few.  The splits of
 // a chunk are a cluster: each leaves its partial sums in shared memory, and each row's are
 // added in rank order by one warp, which scales them and splits them into the 16-bit parts
@@ -56,7 +56,7 @@ constexpr int kTcStages = 8;   // most stages of the ring
 constexpr int kTcSmemMax = 1024 + 3 * (kABytes + kMaxChunk * kBK * 2) +
                            kMaxChunk * kLoraMaxRank * 4 + 256;
 static_assert(1024 + 92 * 1024 + kABytes + 8 * kLoraMaxRank * 4 + 256 <= kTcSmemMax, "");
-constexpr int kTcThreads = 256;   // warp 0 TMA, warp 1 MMA, warps 4..7 epilogue
+constexpr int kTcThreads = 192;   // warp 0 TMA, warp 1 MMA, warps 2..5 epilogue
 
 struct ShrinkParams {
   const int32_t* ids;
@@ -66,7 +66,7 @@ struct ShrinkParams {
   int* row_code;
   int64_t rows;
   int K, rank, adapters;
-  int chunk;      // rows of a CTA: 4, 8 or 64
+  int chunk;      // rows of a CTA: 4 or 64
   int mma_n;      // max(chunk, 16)
   int splits;
   int a_bytes;    // rows of A_a in a stage (the MMA reads on behind them, in other stages
@@ -134,7 +134,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
   }
   pdl_wait();
   // Distinct adapters of the chunk in order of first appearance.
-  const int tok = static_cast<int>(threadIdx.x) - 64;  // warps 2 and 3
+  const int tok = static_cast<int>(threadIdx.x) - 64;  // warps 2 and 3: a thread a row
   const bool mine = tok >= 0 && tok < kMaxChunk;
   if (mine) {
     int id = -1;
@@ -245,29 +245,32 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
         *abort_flag = 1;
       }
     }
-  } else if (warp >= 4) {
+  } else {
     const int q = warp & 3;
     const int lane_row = q * 32 + lane;
     const int u = lane_row / rows_u, j0 = lane_row - u * rows_u;
     for (int ps = 0; ps < passes && !*abort_flag; ++ps) {
       const int acc = ps & 1;
+      const int unit = ps * per + u;
+      const int j = (unit % blocks_u) * kM + j0;
+      const int slot = u < per && unit < units && j < p.rank ? unit / blocks_u : -2;
+      uint64_t own = 0;  // the rows that follow this lane's adapter
+      for (int i = 0; i < n; ++i)
+        if (s_slot[i] == slot) own |= uint64_t{1} << i;
       if (!mbar_wait(&tfull[acc], (ps >> 1) & 1)) {
         atomicExch(&g_shrink_error, kErrTimeoutEpilogue);
         *abort_flag = 1;
         break;
       }
       tc_fence_after();
-      const int unit = ps * per + u;
-      const int j = (unit % blocks_u) * kM + j0;
-      const int slot = u < per && unit < units && j < p.rank ? unit / blocks_u : -2;
       for (int c = 0; c < n; c += 16) {
         float v[16];
         tmem_ld16(tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * p.mma_n + c, v);
         tmem_ld_wait();
+        const unsigned bits = static_cast<unsigned>(own >> c);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (c + i < n && s_slot[c + i] == slot)
-            part[(c + i) * p.rank + j] = s0 < s1 ? v[i] : 0.f;
+          if (bits & (1u << i)) part[(c + i) * p.rank + j] = s0 < s1 ? v[i] : 0.f;
       }
       tc_fence_before();
       __syncwarp();
@@ -343,7 +346,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
 
 // Rows of a CTA: small chunks spread a decode batch (whose rows follow many adapters) over
 // the GPU, tall ones read A_a once per 64 rows of a prompt.
-int shrink_chunk(int64_t rows) { return rows <= 128 ? 4 : rows <= 256 ? 8 : kMaxChunk; }
+int shrink_chunk(int64_t rows) { return rows <= 256 ? 4 : kMaxChunk; }
 
 template <typename T>
 cudaError_t shrink_simt(const LoraShrink& l, float* t, cudaStream_t s) {
@@ -368,13 +371,13 @@ cudaError_t shrink_tc(const LoraShrink& l, uint16_t* parts, float* row_scale, in
   p.chunk = shrink_chunk(l.rows);
   p.mma_n = std::max(p.chunk, 16);
   // A stage holds the adapters that a chunk can have (one token: r rows), so that a short
-  // K is in flight as a whole; two CTAs an SM with the partial sums of rank 64.
+  // K is in flight as a whole.  Small chunks stay at 56 KB, which fits an SM beside two CTAs of
+  // the projection; of tall ones with the partial sums of rank 64, two fit an SM.
   const int unit = std::min(l.rank, kM);
   p.a_bytes = static_cast<int>(std::min<int64_t>(kM / unit, std::min<int64_t>(l.rows, p.chunk))) *
               unit * kBK * 2;
   p.stage_bytes = p.a_bytes + p.mma_n * kBK * 2;
-  p.stages = std::min(kTcStages, 92 * 1024 / p.stage_bytes);
-  if (p.chunk == kMaxChunk) p.stages = std::min(p.stages, 3);
+  p.stages = p.chunk == kMaxChunk ? 3 : std::max(2, std::min(kTcStages, 40 * 1024 / p.stage_bytes));
   // Splits: until about two CTAs an SM run, with at least two slices of K each.
   const int64_t chunks = (l.rows + p.chunk - 1) / p.chunk;
   const int slices = (l.K + kBK - 1) / kBK;
