@@ -84,6 +84,13 @@ cudaError_t launch_grouped_small(const GroupedArgs& g, const LoraTerm* lora, int
 cudaError_t take_grouped_pair_error(int* err);
 cudaError_t take_grouped_small_error(int* err);
 cudaError_t take_lora_error(int* err);
+cudaError_t take_lora_few_error(int* err);
+
+// The whole adapter projection of a few rows in one launch (same types, sizes and alignment as
+// the two launches; b: lora_b).
+bool lora_few_supported(int64_t rows, int64_t rank);
+cudaError_t launch_lora_few(const GroupedArgs& g, const LoraShrink& l, const void* b, int num_sms,
+                            cudaStream_t s);
 
 // FFMA kernels: any size, alignment and float type.
 cudaError_t launch_grouped_simt(const GroupedArgs& g, const LoraTerm* lora, cudaStream_t s);

@@ -72,7 +72,7 @@ int finish(const char* what, cudaStream_t s) {
   int rc = cuda_status(cudaStreamSynchronize(s), what);
   if (rc != MOE_B200_OK) return rc;
   for (auto take : {moe::take_grouped_pair_error, moe::take_grouped_small_error,
-                    moe::take_lora_error}) {
+                    moe::take_lora_error, moe::take_lora_few_error}) {
     int err = 0;
     rc = cuda_status(take(&err), what);
     if (rc == MOE_B200_OK && err != 0)
@@ -280,6 +280,10 @@ int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
   g.out = y;
   const bool a16 = (reinterpret_cast<uintptr_t>(lora_b) & 15) == 0;
   const bool tc = moe::grouped_tc_supported(g) && moe::lora_shrink_tc_supported(l) && a16;
+  if (tc && moe::lora_few_supported(num_rows, rank)) {
+    rc = cuda_status(moe::launch_lora_few(g, l, lora_b, sm_count(), s), kWhat);
+    return rc != MOE_B200_OK ? rc : finish(kWhat, s);
+  }
   moe::LoraTerm term{};
   term.rank = l.rank;
   term.adapters = l.adapters;

@@ -63,7 +63,8 @@ def ids_of(kind, T, L, rng):
     (1, 64, 64, 8, 1), (1, 264, 520, 16, 3), (7, 72, 136, 8, 4), (16, 128, 256, 32, 5),
     (33, 136, 200, 16, 9), (65, 264, 328, 64, 3), (130, 520, 264, 24, 40), (257, 128, 128, 128, 2),
     (600, 264, 136, 16, 7), (5, 33, 41, 3, 2), (70, 130, 66, 5, 6), (300, 64, 72, 256, 3),
-    (9, 8, 8, 1, 2)])
+    (9, 8, 8, 1, 2), (1, 136, 72, 128, 2), (2, 1032, 264, 64, 3), (3, 520, 136, 40, 2),
+    (8, 264, 2056, 16, 5), (8, 64, 64, 8, 3), (4, 4104, 520, 24, 6)])
 @pytest.mark.parametrize("kind", ["none", "one", "mixed", "foreign", "runs"])
 def test_lora_matches_float64(pkg, orc, dev, dtype_name, T, N, K, r, L, kind):
     rng = np.random.default_rng(T * 7 + r)
