@@ -33,9 +33,8 @@ struct LoraTerm {
   int adapters;           // L
   const void* b;          // [L, N, r]
   const int32_t* ids;     // [rows]; outside [0, L): no adapter
-  // FFMA kernels: t = A_a x in fp32, [rows][rank], and the adapters' scales [L].
+  // FFMA kernels: t = s_a A_a x in fp32, [rows][rank].
   const float* t;
-  const float* scales;
   // Tensor-core kernels: s_a t in two 16-bit parts, [2][rows][rank] (grouped_lora.cuh);
   // fp16: the power of two that each row's parts are to be scaled by; and each row's adapter,
   // -1 for none, with kLoraScaled set where that power is not 1.
@@ -62,7 +61,7 @@ struct LoraShrink {
   const int32_t* ids;
   const float* scales;     // [L]
 };
-// Any type and alignment: t in fp32, [rows][rank].
+// Any type and alignment: s_a t in fp32, [rows][rank].
 cudaError_t launch_lora_shrink_simt(const LoraShrink& l, float* t, cudaStream_t s);
 // 16-bit types, K and rank multiples of 8, 16-byte aligned x and a: the parts of
 // LoraTerm, its row_scale and row_code.

@@ -304,7 +304,6 @@ int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
     auto* t = static_cast<float*>(workspace);
     st = moe::launch_lora_shrink_simt(l, t, s);
     term.t = t;
-    term.scales = scales;
   }
   rc = cuda_status(st, kWhat);
   if (rc != MOE_B200_OK) return rc;

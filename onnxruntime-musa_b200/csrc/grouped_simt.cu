@@ -165,7 +165,9 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 
 // CTA tile (16 TM) x (16 TN), TN a multiple of 4 and TM too or 1: thread (ty, tx) owns rows
 // ty * 4 + 64 i + [0, 4) (TM = 1: row ty) and columns tx * 4 + 64 j + [0, 4).
-template <typename T, int DIR, int TM, int TN>
+// SPLIT: the contraction may be split over a cluster; LORA: with the adapter term.  (Both in
+// every kernel spilled registers in the main loop of the 128 x 128 tiles: 10% of its time.)
+template <typename T, int DIR, int TM, int TN, bool SPLIT, bool LORA>
 __global__ void __launch_bounds__(kThreads, TM <= 4 ? 4 : 2)
 grouped_simt_kernel(const SimtParams p) {
   constexpr int BM = 16 * TM, BN = 16 * TN;
@@ -174,8 +176,10 @@ grouped_simt_kernel(const SimtParams p) {
   constexpr bool kBC = DIR == kGmmForward;
   using SA = Slice<T, BM, kDepth, kAC>;
   using SB = Slice<T, BN, kDepth, kBC>;
-  __shared__ __align__(16) float sa[2][kDepth * SA::kPitch];
-  __shared__ __align__(16) float sb[2][kDepth * SB::kPitch];
+  constexpr int kSlice = kDepth * (SA::kPitch + SB::kPitch);
+  __shared__ __align__(16) float operands[2 * kSlice];
+  auto sa = [&](int buf) { return operands + buf * kSlice; };
+  auto sb = [&](int buf) { return operands + buf * kSlice + kDepth * SA::kPitch; };
 
   pdl_wait();
   const int rows = static_cast<int>(p.rows);
@@ -226,16 +230,15 @@ grouped_simt_kernel(const SimtParams p) {
   SA fa;
   SB fb;
   // This CTA's slices (all of them unless the contraction is split).
-  constexpr bool kSplit = TM <= 4;
-  const int S = kSplit ? p.splits : 1;
+  const int S = SPLIT ? p.splits : 1;
   const int me = S > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int all = (nc + kDepth - 1) / kDepth;
   const int from = all * me / S, slices = all * (me + 1) / S;
   if (slices > from) {
     fa.load(a, lda, nm, from * kDepth, nc, p.a_vec);
     fb.load(b, ldb, nn, from * kDepth, nc, p.b_vec);
-    fa.store(sa[0]);
-    fb.store(sb[0]);
+    fa.store(sa(0));
+    fb.store(sb(0));
   }
   __syncthreads();
   for (int s = from; s < slices; ++s) {
@@ -244,23 +247,24 @@ grouped_simt_kernel(const SimtParams p) {
       fa.load(a, lda, nm, (s + 1) * kDepth, nc, p.a_vec);
       fb.load(b, ldb, nn, (s + 1) * kDepth, nc, p.b_vec);
     }
+    const float *a_now = sa(cur), *b_now = sb(cur);
     if (busy) {
 #pragma unroll
       for (int c = 0; c < kDepth; ++c) {
         float ra[TM];
         uint64_t rb[TN / 2];
         if constexpr (TM == 1) {
-          ra[0] = sa[cur][c * SA::kPitch + ty];
+          ra[0] = a_now[c * SA::kPitch + ty];
         } else {
 #pragma unroll
           for (int i = 0; i < TM; i += 4)
             *reinterpret_cast<float4*>(ra + i) =
-                *reinterpret_cast<const float4*>(&sa[cur][c * SA::kPitch + ty * 4 + i * 16]);
+                *reinterpret_cast<const float4*>(&a_now[c * SA::kPitch + ty * 4 + i * 16]);
         }
 #pragma unroll
         for (int j = 0; j < TN; j += 4)
           *reinterpret_cast<ulonglong2*>(rb + j / 2) =
-              *reinterpret_cast<const ulonglong2*>(&sb[cur][c * SB::kPitch + tx * 4 + j * 16]);
+              *reinterpret_cast<const ulonglong2*>(&b_now[c * SB::kPitch + tx * 4 + j * 16]);
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
           const uint64_t aa = pair2(ra[i], ra[i]);
@@ -270,8 +274,8 @@ grouped_simt_kernel(const SimtParams p) {
       }
     }
     if (s + 1 < slices) {
-      fa.store(sa[cur ^ 1]);
-      fb.store(sb[cur ^ 1]);
+      fa.store(sa(cur ^ 1));
+      fb.store(sb(cur ^ 1));
     }
     __syncthreads();
   }
@@ -282,14 +286,15 @@ grouped_simt_kernel(const SimtParams p) {
 #pragma unroll
     for (int j = 0; j < TN / 2; ++j) unpair2(acc2[i][j], acc[i][2 * j], acc[i][2 * j + 1]);
 
-  if constexpr (kSplit) {
-    if (S > 1) {
-      // Row i of each thread's four goes to CTA i S / 4 (TM = 1: the thread's row to CTA
-      // ty % S), which adds the parts in rank order.
-      float4* parts = reinterpret_cast<float4*>(&sb[0][0]);  // [S - 1][rows owned][256]
-      static_assert(sizeof(sb) >= 3 * kThreads * 16, "parts fit the operand slices");
-      const int per = TM == 1 ? 1 : TM / S;
-      cluster_sync();  // every CTA has read its slices
+  if (SPLIT && S > 1) {
+    // The cluster's parts: row i of each thread goes to CTA i S / TM (TM = 1: the thread's row to CTA ty % S), which
+    // adds the parts in rank order; four columns at a time.
+    float4* parts = reinterpret_cast<float4*>(operands);  // [S - 1][rows owned][256]
+    static_assert(sizeof(operands) >= 3 * ((TM + 3) / 4) * kThreads * 16, "parts fit the operands");
+    const int per = TM == 1 ? 1 : TM / S;
+#pragma unroll
+    for (int j = 0; j < TN; j += 4) {
+      cluster_sync();  // every CTA has read its slices, or the parts of the columns before
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         const int owner = TM == 1 ? ty % S : i / per;
@@ -298,7 +303,7 @@ grouped_simt_kernel(const SimtParams p) {
         const uint32_t at = smem_u32(parts + (slot * per + i % per) * kThreads + threadIdx.x);
         asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
                          mapa_shared(at, owner)),
-                     "f"(acc[i][0]), "f"(acc[i][1]), "f"(acc[i][2]), "f"(acc[i][3])
+                     "f"(acc[i][j]), "f"(acc[i][j + 1]), "f"(acc[i][j + 2]), "f"(acc[i][j + 3])
                      : "memory");
       }
       cluster_sync();
@@ -307,42 +312,100 @@ grouped_simt_kernel(const SimtParams p) {
         if ((TM == 1 ? ty % S : i / per) != me) continue;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int r = 0; r < S; ++r) {
-          const float4 v = r == me ? make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3])
-                                   : parts[((r < me ? r : r - 1) * per + i % per) * kThreads +
-                                           threadIdx.x];
+          const float4 v =
+              r == me ? make_float4(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3])
+                      : parts[((r < me ? r : r - 1) * per + i % per) * kThreads + threadIdx.x];
           sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
         }
-        acc[i][0] = sum.x; acc[i][1] = sum.y; acc[i][2] = sum.z; acc[i][3] = sum.w;
+        acc[i][j] = sum.x; acc[i][j + 1] = sum.y; acc[i][j + 2] = sum.z; acc[i][j + 3] = sum.w;
+      }
+    }
+  }
+
+  // Whether this CTA finishes row i of each thread.
+  auto owned = [&](int i) { return S == 1 || (TM == 1 ? ty % S : i * S / TM) == me; };
+  auto row_of = [&](int i) { return TM == 1 ? ty : ty * 4 + (i / 4) * 64 + (i & 3); };
+  if constexpr (LORA) {
+    // The adapter term (t holds s_a A_a x).  Rows of other adapters skip an adapter's FMAs, so
+    // that what it holds (an infinity, say) stays with its own rows.
+    __shared__ int s_ad[BM], s_list[BM];
+    __shared__ int s_count;
+    if (threadIdx.x == 0) s_count = 0;
+    const int r = p.lora.rank;
+    for (int m = threadIdx.x; m < BM; m += kThreads) {
+      const int id = m < nm ? __ldg(p.lora.ids + row0 + m) : -1;
+      s_ad[m] = id >= 0 && id < p.lora.adapters ? id : -1;
+    }
+    __syncthreads();
+    for (int m = threadIdx.x; m < BM; m += kThreads) {
+      const int id = s_ad[m];
+      int k = 0;
+      if (id >= 0)
+        while (s_ad[k] != id) ++k;
+      if (id >= 0 && k == m) s_list[atomicAdd(&s_count, 1)] = id;
+    }
+    __syncthreads();
+    const float* t = p.lora.t + static_cast<int64_t>(row0) * r;
+    const T* b0 = static_cast<const T*>(p.lora.b) + static_cast<int64_t>(col0) * r;
+    const int64_t per = static_cast<int64_t>(p.N) * r;
+    const bool tv = r % 4 == 0;
+    const bool bv = tv && reinterpret_cast<uintptr_t>(p.lora.b) % (4 * sizeof(T)) == 0;
+    if (s_count > 4) {
+      // Many adapters (decode): each thread walks its own rows' t and B.
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const int m = row_of(i);
+        if (!owned(i) || s_ad[m] < 0) continue;
+        const T* bb = b0 + s_ad[m] * per;
+        for (int q = 0; q < r; q += 4) {
+          const float4 u = load4<float>(t + static_cast<int64_t>(m) * r + q, r - q, tv);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            const int n = tx * 4 + (j / 4) * 64 + (j & 3);
+            if (n >= nn) continue;
+            const float4 v = load4<T>(bb + static_cast<int64_t>(n) * r + q, r - q, bv);
+            acc[i][j] = fmaf(u.x, v.x, fmaf(u.y, v.y, fmaf(u.z, v.z, fmaf(u.w, v.w, acc[i][j]))));
+          }
+        }
+      }
+    } else {
+      // Few (prompts): slices of t against B_a, adapter by adapter.  (A row's sums come from one
+      // adapter, so the list's order does not show.)
+      Slice<float, BM, kDepth, true> ft;
+      Slice<T, BN, kDepth, true> fl;
+      const float *a_now = sa(0), *b_now = sb(0);
+      for (int d = 0; d < s_count; ++d) {
+        const int ad = s_list[d];
+        for (int c0 = 0; c0 < r; c0 += kDepth) {
+          ft.load(t, r, nm, c0, r, tv);
+          fl.load(b0 + ad * per, r, nn, c0, r, bv);
+          __syncthreads();
+          ft.store(sa(0));
+          fl.store(sb(0));
+          __syncthreads();
+          const int depth = min(kDepth, r - c0);
+          for (int c = 0; c < depth; ++c) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+              const float u = a_now[c * SA::kPitch + row_of(i)];
+              if (owned(i) && s_ad[row_of(i)] == ad) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+                  acc[i][j] = fmaf(u, b_now[c * SB::kPitch + tx * 4 + (j / 4) * 64 + (j & 3)],
+                                   acc[i][j]);
+              }
+            }
+          }
+        }
       }
     }
   }
 
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
-    if (kSplit && S > 1 && (TM == 1 ? ty % S : i * S / TM) != me) continue;
-    const int m = TM == 1 ? ty : ty * 4 + (i / 4) * 64 + (i & 3);
+    if (!owned(i)) continue;
+    const int m = row_of(i);
     if (m >= nm) continue;
-    if (DIR == kGmmForward && p.lora.t != nullptr) {
-      // y += s_a * sum_j t[row, j] B_a[n, j].
-      const int row = row0 + m, ad = __ldg(p.lora.ids + row), r = p.lora.rank;
-      if (ad >= 0 && ad < p.lora.adapters) {
-        float d[TN];
-#pragma unroll
-        for (int j = 0; j < TN; ++j) d[j] = 0.f;
-        const T* bb = static_cast<const T*>(p.lora.b) + static_cast<int64_t>(ad) * p.N * r;
-        for (int q = 0; q < r; ++q) {
-          const float t = __ldg(p.lora.t + static_cast<int64_t>(row) * r + q);
-#pragma unroll
-          for (int j = 0; j < TN; ++j) {
-            const int n = tx * 4 + (j / 4) * 64 + (j & 3);
-            if (n < nn) d[j] = fmaf(t, to_f(bb[static_cast<int64_t>(col0 + n) * r + q]), d[j]);
-          }
-        }
-        const float sc = __ldg(p.lora.scales + ad);
-#pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = fmaf(sc, d[j], acc[i][j]);
-      }
-    }
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int n = tx * 4 + (j / 4) * 64 + (j & 3);
@@ -351,7 +414,89 @@ grouped_simt_kernel(const SimtParams p) {
   }
 }
 
-template <typename T, int DIR, int TM, int TN>
+// Forward product of groups of a few rows: streaming the weights through the lanes.  A warp
+// takes kGemvCols output features and up to kGemvRows rows of the group at a time; its lanes
+// stride over the contraction, four entries each, and meet in a butterfly sum.  Bound: the
+// weights' bytes (a 64-row tile of the kernel above would multiply 64 rows whatever the group
+// has: 97 us for one row of [4096, 4096] fp32).
+constexpr int kGemvRows = 8;
+constexpr int kGemvCols = 2;
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+grouped_gemv_kernel(const SimtParams p) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int rows = static_cast<int>(p.rows), e = blockIdx.y, K = p.K;
+  const int begin = group_begin(p.offsets, e, rows), end = group_end(p.offsets, e, rows, begin);
+  const int n0 = (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kGemvCols;
+  if (n0 >= p.N) return;
+  const T* w0 = static_cast<const T*>(p.b) + (static_cast<int64_t>(e) * p.N + n0) * K;
+  const T* x = static_cast<const T*>(p.a);
+  for (int r0 = begin; r0 < end; r0 += kGemvRows) {
+    const int nr = min(kGemvRows, end - r0);
+    float acc[kGemvCols][kGemvRows] = {};
+    const T* xr = x + static_cast<int64_t>(r0) * K;
+#pragma unroll 4
+    for (int c = lane * 4; c < K; c += 128) {
+      float4 w[kGemvCols];
+#pragma unroll
+      for (int j = 0; j < kGemvCols; ++j)
+        w[j] = n0 + j < p.N ? load4<T>(w0 + static_cast<int64_t>(j) * K + c, K - c, p.b_vec)
+                            : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < kGemvRows; ++i) {
+        if (i >= nr) break;
+        const float4 v = load4<T>(xr + static_cast<int64_t>(i) * K + c, K - c, p.a_vec);
+#pragma unroll
+        for (int j = 0; j < kGemvCols; ++j) {
+          acc[j][i] = fmaf(w[j].x, v.x, acc[j][i]);
+          acc[j][i] = fmaf(w[j].y, v.y, acc[j][i]);
+          acc[j][i] = fmaf(w[j].z, v.z, acc[j][i]);
+          acc[j][i] = fmaf(w[j].w, v.w, acc[j][i]);
+        }
+      }
+    }
+    if (p.lora.t != nullptr) {  // y += B_a t, the lanes striding over the rank
+      const int r = p.lora.rank;
+#pragma unroll
+      for (int i = 0; i < kGemvRows; ++i) {
+        if (i >= nr) break;
+        const int ad = __ldg(p.lora.ids + r0 + i);
+        if (ad < 0 || ad >= p.lora.adapters) continue;
+        const float* t = p.lora.t + static_cast<int64_t>(r0 + i) * r;
+        const T* bb = static_cast<const T*>(p.lora.b) + (static_cast<int64_t>(ad) * p.N + n0) * r;
+        for (int q = lane; q < r; q += 32) {
+          const float tq = t[q];
+#pragma unroll
+          for (int j = 0; j < kGemvCols; ++j)
+            if (n0 + j < p.N) acc[j][i] = fmaf(to_f(bb[j * r + q]), tq, acc[j][i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kGemvRows; ++i) {
+      if (i >= nr) break;
+#pragma unroll
+      for (int j = 0; j < kGemvCols; ++j) {
+        float v = acc[j][i];
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+        if (lane == 0 && n0 + j < p.N)
+          static_cast<T*>(p.out)[static_cast<int64_t>(r0 + i) * p.N + n0 + j] = from_f<T>(v);
+      }
+    }
+  }
+}
+
+template <typename T>
+cudaError_t launch_gemv(const SimtParams& p, cudaStream_t s) {
+  const int per = kThreads / 32 * kGemvCols;
+  return launch_dependent(true, grouped_gemv_kernel<T>, dim3((p.N + per - 1) / per, p.E),
+                          dim3(kThreads), 0, s, p);
+}
+
+template <typename T, int DIR, int TM, int TN, bool LORA>
 cudaError_t launch_tile(const GroupedArgs& g, SimtParams p, cudaStream_t s) {
   constexpr int BM = 16 * TM, BN = 16 * TN;
   dim3 grid;
@@ -369,9 +514,10 @@ cudaError_t launch_tile(const GroupedArgs& g, SimtParams p, cudaStream_t s) {
     tiles = rows_tiles * grid.y;
     con = DIR == kGmmForward ? g.K : g.N;
   }
-  // Split until about four CTAs an SM run, with at least two slices of 32 each.
-  if (TM <= 4)
-    while (p.splits < 4 && tiles * p.splits * 2 <= 4 * 148 && con >= 128 * p.splits) p.splits *= 2;
+  // Split until the SMs' resident CTAs run (four, of 128 x 128 tiles two), with a contraction
+  // of at least 64 each.
+  const int64_t fill = 148 * (TM <= 4 ? 4 : 2);
+  while (p.splits < 4 && tiles * p.splits * 2 <= fill && con >= 128 * p.splits) p.splits *= 2;
   grid.z *= p.splits;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
@@ -386,10 +532,12 @@ cudaError_t launch_tile(const GroupedArgs& g, SimtParams p, cudaStream_t s) {
   attr[1].val.clusterDim.z = static_cast<unsigned>(p.splits);
   cfg.attrs = attr;
   cfg.numAttrs = p.splits > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, grouped_simt_kernel<T, DIR, TM, TN>, p);
+  if (TM <= 4 || p.splits > 1)
+    return cudaLaunchKernelEx(&cfg, grouped_simt_kernel<T, DIR, TM, TN, true, LORA>, p);
+  return cudaLaunchKernelEx(&cfg, grouped_simt_kernel<T, DIR, TM, TN, TM <= 4, LORA>, p);
 }
 
-template <typename T, int DIR>
+template <typename T, int DIR, bool LORA>
 cudaError_t launch_dir(const GroupedArgs& g, const LoraTerm* lora, cudaStream_t s) {
   SimtParams p{};
   p.a = DIR == kGmmForward ? g.x : g.dy;
@@ -406,25 +554,32 @@ cudaError_t launch_dir(const GroupedArgs& g, const LoraTerm* lora, cudaStream_t 
   p.a_vec = vec(p.a, DIR == kGmmForward ? g.K : g.N);
   p.b_vec = vec(p.b, g.K);
   if (lora != nullptr) p.lora = *lora;
-  // 128 x 128 tiles once they fill the GPU twice over (each thread then does 64 FMAs per
-  // 16 shared loads instead of 16 per 8); below that the 64 x 64 tiles' four times as many
-  // CTAs win.  Groups of a few rows take tiles of 16 rows, which multiply less padding.
+  if constexpr (DIR == kGmmForward) {
+    if (g.rows <= (g.E == 1 ? kGemvRows : 4 * static_cast<int64_t>(g.E))) return launch_gemv<T>(p, s);
+  }
+  // 128 x 128 tiles where groups fill them and they, split four ways, fill the GPU (each thread
+  // then does 64 FMAs per 16 shared loads instead of 16 per 8); else 64 x 64, and 16 rows for
+  // groups of a few rows, which multiply less padding.
   const int64_t feat = DIR == kGmmForward ? g.N : g.K;
   const int64_t big = DIR == kGmmGradWeight
                           ? static_cast<int64_t>(g.E) * ((g.N + 127) / 128) * ((g.K + 127) / 128)
-                          : (g.rows / 128) * ((feat + 127) / 128);
-  if (big >= 2 * 148) return launch_tile<T, DIR, 8, 8>(g, p, s);
+                          : ((g.rows + 127) / 128) * ((feat + 127) / 128);
+  const int64_t height = DIR == kGmmGradWeight ? g.N : g.rows / g.E;
+  // (With element-wise loads the small tiles win until the big ones fill the GPU unsplit.)
+  const int64_t ways = p.a_vec && p.b_vec ? 4 : 1;
+  if (height >= 96 && feat >= 96 && ways * big >= 148) return launch_tile<T, DIR, 8, 8, LORA>(g, p, s);
   if constexpr (DIR != kGmmGradWeight) {
-    if (g.rows <= 16 * static_cast<int64_t>(g.E)) return launch_tile<T, DIR, 1, 4>(g, p, s);
+    if (g.rows <= 16 * static_cast<int64_t>(g.E)) return launch_tile<T, DIR, 1, 4, LORA>(g, p, s);
   }
-  return launch_tile<T, DIR, 4, 4>(g, p, s);
+  return launch_tile<T, DIR, 4, 4, LORA>(g, p, s);
 }
 
 template <typename T>
 cudaError_t launch_type(const GroupedArgs& g, const LoraTerm* lora, cudaStream_t s) {
-  if (g.dir == kGmmForward) return launch_dir<T, kGmmForward>(g, lora, s);
-  if (g.dir == kGmmGradInput) return launch_dir<T, kGmmGradInput>(g, lora, s);
-  return launch_dir<T, kGmmGradWeight>(g, lora, s);
+  if (lora != nullptr) return launch_dir<T, kGmmForward, true>(g, lora, s);
+  if (g.dir == kGmmForward) return launch_dir<T, kGmmForward, false>(g, nullptr, s);
+  if (g.dir == kGmmGradInput) return launch_dir<T, kGmmGradInput, false>(g, nullptr, s);
+  return launch_dir<T, kGmmGradWeight, false>(g, nullptr, s);
 }
 
 }  // namespace

@@ -22,26 +22,74 @@ namespace {
 
 constexpr int kWarps = 8;
 
-// Any type and alignment: one CTA per row, a warp per rank entry, the lanes striding over
-// K.  The row comes from L1 after the first warp's pass; A_a is read once per row.
+// Any type and alignment: a CTA takes kRows adjacent rows and kWarps rank entries, a warp
+// each, the lanes striding over K.  One pass over an A row serves all rows that follow its
+// adapter (rows of a prompt; A_a is what is read most).
+constexpr int kRows = 4;
+
+template <typename T>
+__device__ __forceinline__ void load_vec(const T* p, int n, bool vec, float (&v)[4]) {
+  if (vec && n >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p);
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      const T* q = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = to_f(q[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? to_f(p[i]) : 0.f;
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kWarps * 32)
 lora_shrink_simt_kernel(const T* __restrict__ x, const T* __restrict__ a,
-                        const int32_t* __restrict__ ids, int K, int rank, int adapters,
+                        const int32_t* __restrict__ ids, const float* __restrict__ scales,
+                        int64_t rows, int K, int rank, int adapters, bool vec,
                         float* __restrict__ t) {
-  const int64_t row = blockIdx.x;
-  const int ad = ids[row];
-  if (ad < 0 || ad >= adapters) return;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const T* xr = x + row * K;
-  for (int j = warp; j < rank; j += kWarps) {
-    const T* ar = a + (static_cast<int64_t>(ad) * rank + j) * K;
-    float sum = 0.f;
-#pragma unroll 4
-    for (int k = lane; k < K; k += 32) sum = fmaf(to_f(ar[k]), to_f(xr[k]), sum);
+  const int j = blockIdx.y * kWarps + warp;
+  if (j >= rank) return;
+  int ad[kRows];
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) t[row * rank + j] = sum;
+  for (int i = 0; i < kRows; ++i) {
+    ad[i] = row0 + i < rows ? ids[row0 + i] : -1;
+    if (ad[i] >= adapters) ad[i] = -1;
+  }
+#pragma unroll
+  for (int f = 0; f < kRows; ++f) {
+    // The first row of each adapter leads; the rows after it that follow the same join.
+    bool lead = ad[f] >= 0;
+#pragma unroll
+    for (int i = 0; i < f; ++i) lead = lead && ad[i] != ad[f];
+    if (!lead) continue;
+    const T* ar = a + (static_cast<int64_t>(ad[f]) * rank + j) * K;
+    float sum[kRows] = {};
+#pragma unroll 8
+    for (int k = lane * 4; k < K; k += 128) {
+      float w[4], v[4];
+      load_vec(ar + k, K - k, vec, w);
+#pragma unroll
+      for (int i = f; i < kRows; ++i) {
+        if (ad[i] != ad[f]) continue;
+        load_vec(x + (row0 + i) * K + k, K - k, vec, v);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sum[i] = fmaf(w[q], v[q], sum[i]);
+      }
+    }
+#pragma unroll
+    for (int i = f; i < kRows; ++i) {
+      if (ad[i] != ad[f]) continue;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], d);
+      if (lane == 0) t[(row0 + i) * rank + j] = scales[ad[f]] * sum[i];
+    }
   }
 }
 
@@ -350,9 +398,15 @@ int shrink_chunk(int64_t rows) { return rows <= 256 ? 4 : kMaxChunk; }
 
 template <typename T>
 cudaError_t shrink_simt(const LoraShrink& l, float* t, cudaStream_t s) {
-  lora_shrink_simt_kernel<T><<<static_cast<unsigned>(l.rows), kWarps * 32, 0, s>>>(
-      static_cast<const T*>(l.x), static_cast<const T*>(l.a), l.ids, l.K, l.rank, l.adapters, t);
-  return cudaGetLastError();
+  const bool vec = l.K % 4 == 0 &&
+                   (reinterpret_cast<uintptr_t>(l.x) | reinterpret_cast<uintptr_t>(l.a)) %
+                           (4 * sizeof(T)) == 0;
+  return launch_dependent(true, lora_shrink_simt_kernel<T>,
+                          dim3(static_cast<unsigned>((l.rows + kRows - 1) / kRows),
+                               (l.rank + kWarps - 1) / kWarps),
+                          dim3(kWarps * 32), 0, s, static_cast<const T*>(l.x),
+                          static_cast<const T*>(l.a), l.ids, l.scales, l.rows, l.K, l.rank,
+                          l.adapters, vec, t);
 }
 
 template <typename T>
