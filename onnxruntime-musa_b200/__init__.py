@@ -861,8 +861,8 @@ def grouped_matmul(x, weights, expert_offsets, out=None, stream=None):
     what = "grouped_matmul"
     R, K = _dims(what, "x", x, 2)
     E, N, _ = _dims(what, "weights", weights, 3)
-    return _product(what, lib().moe_b200_grouped_matmul, x, weights, expert_offsets, out, stream,
-                    R, N, K, E, K, N)
+    return _product(what, "x", lib().moe_b200_grouped_matmul, x, weights, expert_offsets, out,
+                    stream, R, N, K, E, K, N)
 
 
 def grouped_matmul_grad_input(dy, weights, expert_offsets, out=None, stream=None):
@@ -871,14 +871,14 @@ def grouped_matmul_grad_input(dy, weights, expert_offsets, out=None, stream=None
     what = "grouped_matmul_grad_input"
     R, N = _dims(what, "dy", dy, 2)
     E, _, K = _dims(what, "weights", weights, 3)
-    return _product(what, lib().moe_b200_grouped_matmul_grad_input, dy, weights, expert_offsets,
-                    out, stream, R, N, K, E, N, K)
+    return _product(what, "dy", lib().moe_b200_grouped_matmul_grad_input, dy, weights,
+                    expert_offsets, out, stream, R, N, K, E, N, K)
 
 
-def _product(what, entry, rows, weights, offsets, out, stream, R, N, K, E, width, out_width):
+def _product(what, name, entry, rows, weights, offsets, out, stream, R, N, K, E, width, out_width):
     dev, dtype = _device_of(what, rows), rows.dtype
     code = _dt_code(what, dtype)
-    _require(what, "rows", rows, (R, width), dtype, dev)
+    _require(what, name, rows, (R, width), dtype, dev)
     _require(what, "weights", weights, (E, N, K), dtype, dev)
     _require(what, "expert_offsets", offsets, (E + 1,), _torch().int32, dev)
     if out is not None:
@@ -886,8 +886,8 @@ def _product(what, entry, rows, weights, offsets, out, stream, R, N, K, E, width
     s = _current_stream(dev) if stream is None else None
     if s is None:
         with _Elsewhere(stream, dev, (rows, weights, offsets, out)):
-            return _product(what, entry, rows, weights, offsets, out, None, R, N, K, E, width,
-                            out_width)
+            return _product(what, name, entry, rows, weights, offsets, out, None, R, N, K, E,
+                            width, out_width)
     if out is None:
         out = rows.new_empty((R, out_width))
     check(entry(code, R, N, K, E, rows.data_ptr(), weights.data_ptr(), offsets.data_ptr(),

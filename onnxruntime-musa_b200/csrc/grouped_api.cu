@@ -1,5 +1,6 @@
 // C entries of the expert products (moe_b200_grouped_matmul*) and the adapter projection
 // (moe_b200_lora_matmul): argument checks and the choice of kernel.
+#include <algorithm>
 #include <atomic>
 #include <cstdlib>
 
@@ -82,14 +83,23 @@ int finish(const char* what, cudaStream_t s) {
   return MOE_B200_OK;
 }
 
-// The pair kernel once its 256-row tiles are filled (mean rows per group) and there are
-// enough of them for the SM pairs; else the weight-streaming kernel.
+// The CTA-pair kernel or the weight-streaming kernel, by what was measured (bf16, us, forward /
+// grad_input, streaming : pair):
+//   8 experts [4096, 4096]   64 rows each 49 : 52 / 45 : 50, 96 rows 60 : 54 / 61 : 51,
+//                            256 rows 95 : 75 / 99 : 82
+//   64 experts [768, 2048]   16 rows each 41.2 : 41.0 / 44.5 : 38.6 (a contraction of 768)
+//   1 group [4096, 4096]     192 rows 14.7 : 25.0, 1024 rows 34 : 30
+// The pair kernel needs tiles for the SM pairs; then it wins from about 80 rows a group, and
+// with short contractions for any number, because it is persistent (the streaming kernel pays
+// its start-up for every tile).
 bool use_pair(const moe::GroupedArgs& g, int sms) {
   if (g.dir == moe::kGmmGradWeight) return true;
   const int64_t feat = g.dir == moe::kGmmForward ? g.N : g.K;
-  const int64_t per = g.rows / g.E;
-  const int64_t tiles = (per + 255) / 256 * g.E * ((feat + 255) / 256);
-  return per >= 128 && tiles >= sms / 2 * 3 / 4;
+  const int64_t con = g.dir == moe::kGmmForward ? g.K : g.N;
+  const int64_t groups = std::min<int64_t>(g.rows, g.E), per = g.rows / groups;
+  const int64_t tiles = (per + 255) / 256 * groups * ((feat + 255) / 256);
+  const int pairs = sms / 2;
+  return (per >= 80 && tiles >= pairs * 3 / 4) || (con <= 2048 && tiles >= 2 * pairs);
 }
 
 cudaError_t launch_tc(const moe::GroupedArgs& g, const moe::LoraTerm* lora, cudaStream_t s) {

@@ -386,7 +386,10 @@ cudaError_t launch_small(const GroupedArgs& g, const LoraTerm* lora, int num_sms
   // of these kernels takes at least 90 KB of shared memory per 256 columns), so an
   // allocation never waits for a CTA that waits for its own cluster.
   p.tmem_cols = static_cast<uint32_t>(std::max(32, p.cap * (LORA > 0 ? 2 : 1)));
-  const int64_t tiles = (g.rows / p.cap + std::min<int64_t>(g.rows, g.E)) * p.m_tiles;
+  // The tile count lives on the device; each ragged group adds at most one.
+  const int64_t tiles = (g.E == 1 ? (g.rows + p.cap - 1) / p.cap
+                                  : g.rows / p.cap + std::min<int64_t>(g.rows, g.E)) *
+                        p.m_tiles;
   // CTAs an SM: two, sharing its memory, up to 128 rows; one at 256.  (One alone with 130 KB
   // was slower: clusters of such CTAs do not all find room at once, 16.5 against 13.4 us for
   // 64 rows, 4096 x 4096.)  With adapters two have 192 threads, and of 32 or 64 rows 85 KB, which
@@ -395,11 +398,14 @@ cudaError_t launch_small(const GroupedArgs& g, const LoraTerm* lora, int num_sms
   const int resident = p.cap > 128 ? 1 : 2;
   const int budget = (p.cap > 128 ? 220 : LORA > 0 && (p.cap == 32 || p.cap == 64) ? 86 : 113) * 1024;
   const int threads = LORA > 0 && resident == 2 ? 192 : kThreads;
-  // Splits: until the grid fills these, with at least two slices each.
+  // Splits: until the grid fills these, with at least two slices each.  Clusters of eight CTAs
+  // that each take an SM do not all find room at once (384 rows, [1024, 4096]: 21 us, by four
+  // 14), except a few of them (192 rows: 11.6 us, by four 13.3).
   const int64_t fill = static_cast<int64_t>(num_sms) * resident;
   const int slices = (p.con + kBK - 1) / kBK;
+  const int most = resident == 1 && tiles * 8 > 64 ? 4 : 8;
   p.splits = 1;
-  while (p.splits < 8 && tiles * p.splits * 2 <= fill && slices >= 4 * p.splits) p.splits *= 2;
+  while (p.splits < most && tiles * p.splits * 2 <= fill && slices >= 4 * p.splits) p.splits *= 2;
   // The exchange has its own memory up to 64 rows (at most 28 KB); above, it reuses the ring
   // and the cluster meets once more before it.
   const int blocks_owned = (p.cap / 8 + p.splits - 1) / p.splits;

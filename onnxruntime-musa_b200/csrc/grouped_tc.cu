@@ -720,7 +720,9 @@ cudaError_t launch_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
   const int64_t tiles =
           DIR == kGmmGradWeight
               ? static_cast<int64_t>(g.E) * p.m_tiles * p.n_tiles
-              : (g.rows / p.tile_rows + std::min<int64_t>(g.rows, g.E)) * p.m_tiles;
+              : (g.E == 1 ? (g.rows + p.tile_rows - 1) / p.tile_rows
+                         : g.rows / p.tile_rows + std::min<int64_t>(g.rows, g.E)) *
+                    p.m_tiles;
   static SmemOptIn opt_in;
   cudaError_t st = opt_in.set(grouped_pair_kernel<T, DIR, LORA>, kSmem);
   if (st != cudaSuccess) return st;
