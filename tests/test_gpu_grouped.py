@@ -308,3 +308,35 @@ def test_no_rows(pkg, dev):
     out = torch.full((3, 16, 24), 5.0, device=dev, dtype=torch.float16)
     pkg.grouped_matmul_grad_weight(x, dy, off, out=out)
     assert not out.any()
+
+
+# Long fp32 contractions.  Every product is c = 1 + 2^-13 - 2^-16 (times a power of two per row),
+# chosen so that one running sum of 4096 or more of them rounds the same way at every step: off
+# by 4.7e-5 to 9.2e-5 of the sum for 1 to 4 such sums, computed in fp32.  Sums of 512 and then a
+# sum of those lose at most one half step per addition on the way of a product:
+# 512 + 16384 / 512 additions, four more where the contraction is split.
+LONG = 16384
+
+
+def long_bound(exact):
+    return np.abs(exact) * (512 + LONG // 512 + 4) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("rows,feat,E", [(4, 24, 1), (24, 40, 2), (70, 72, 1), (768, 896, 1)])
+def test_fp32_long_sums(pkg, dev, rows, feat, E):
+    import torch
+    c = 1 + 2.0 ** -13 - 2.0 ** -16
+    off, _ = offsets_of([rows // E] * E, dev)
+    scale = torch.tensor([2.0 ** (i % 5 - 2) for i in range(rows)], device=dev)
+    a = scale[:, None].expand(rows, LONG).contiguous()
+    exact = (as_np(scale) * c * LONG)[:, None]
+    got = as_np(pkg.grouped_matmul(a, torch.full((E, feat, LONG), c, device=dev), off))
+    assert (np.abs(got - exact) <= long_bound(exact)).all()
+    got = as_np(pkg.grouped_matmul_grad_input(a, torch.full((E, LONG, feat), c, device=dev), off))
+    assert (np.abs(got - exact) <= long_bound(exact)).all()
+    # The weights' gradient sums over rows: an expert with all of them, beside an empty one.
+    off, _ = offsets_of([LONG, 0], dev)
+    dy = scale[None, :].expand(LONG, rows).contiguous()
+    got = as_np(pkg.grouped_matmul_grad_weight(torch.full((LONG, feat), c, device=dev), dy, off))
+    assert (np.abs(got[0] - exact) <= long_bound(exact)).all()
+    assert (got[1] == 0).all()
