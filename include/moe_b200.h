@@ -322,8 +322,8 @@ int moe_b200_norm_router(int32_t dtype, int64_t num_rows, int64_t hidden_size,
  * [0, num_rows] are clamped to it.)  weights [E, n, k], k contiguous; float, float16 or
  * bfloat16 throughout, sums in fp32.  1 <= n, k <= 2^20; E <= 256.  Buffers need the
  * alignment of their elements; 16-bit types with n and k multiples of 8 and 16-byte
- * aligned buffers run on the tensor cores.  Outputs must not overlap inputs.  No host
- * synchronisation, no allocation; results are the same bits on every call.
+ * aligned buffers run on the tensor cores.  Outputs and workspaces that overlap another buffer of the
+ * call are refused.  No host synchronisation, no allocation; results are the same bits on every call.
  * Analog of the reference's batched product (musa/ep/src/kernels/math/matmul.cc:239-332,
  * shared_inc/blas_utils.h:237-262), which takes equal sizes only. */
 

@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdlib>
+#include <initializer_list>
 
 #include "../../include/moe_b200.h"
 #include "grouped.h"
@@ -50,6 +51,23 @@ int check_pointers(const char* what, int32_t dtype, const void* const* ptrs, int
     if (reinterpret_cast<uintptr_t>(q) % (i < n ? es : 4) != 0)
       return set_error(MOE_B200_INVALID_ARGUMENT,
                        "%s: buffers must be aligned to their element size", what);
+  }
+  return MOE_B200_OK;
+}
+
+struct Range {
+  const void* at;
+  int64_t bytes;
+};
+
+// What a call writes must not lie in what it reads: tiles finish in any order.
+int check_overlap(const char* what, const Range& written, std::initializer_list<Range> others) {
+  const uintptr_t w = reinterpret_cast<uintptr_t>(written.at);
+  for (const Range& r : others) {
+    const uintptr_t q = reinterpret_cast<uintptr_t>(r.at);
+    if (w < q + static_cast<uintptr_t>(r.bytes) && q < w + static_cast<uintptr_t>(written.bytes))
+      return set_error(MOE_B200_INVALID_ARGUMENT,
+                       "%s: outputs and the workspace must not overlap other buffers", what);
   }
   return MOE_B200_OK;
 }
@@ -139,6 +157,11 @@ int moe_b200_grouped_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t 
   const void* words[] = {expert_offsets};
   rc = check_pointers(kWhat, dtype, ptrs, 3, words, 1);
   if (rc != MOE_B200_OK) return rc;
+  const int64_t es = moe::dtype_bytes(dtype);
+  rc = check_overlap(kWhat, {y, num_rows * n * es},
+                     {{x, num_rows * k * es}, {weights, num_experts * n * k * es},
+                      {expert_offsets, (num_experts + 1) * 4}});
+  if (rc != MOE_B200_OK) return rc;
   moe::GroupedArgs g{};
   g.dtype = dtype;
   g.dir = moe::kGmmForward;
@@ -163,6 +186,11 @@ int moe_b200_grouped_matmul_grad_input(int32_t dtype, int64_t num_rows, int64_t 
   const void* ptrs[] = {dy, weights, dx};
   const void* words[] = {expert_offsets};
   rc = check_pointers(kWhat, dtype, ptrs, 3, words, 1);
+  if (rc != MOE_B200_OK) return rc;
+  const int64_t es = moe::dtype_bytes(dtype);
+  rc = check_overlap(kWhat, {dx, num_rows * k * es},
+                     {{dy, num_rows * n * es}, {weights, num_experts * n * k * es},
+                      {expert_offsets, (num_experts + 1) * 4}});
   if (rc != MOE_B200_OK) return rc;
   moe::GroupedArgs g{};
   g.dtype = dtype;
@@ -218,6 +246,13 @@ int moe_b200_grouped_matmul_grad_weight(int32_t dtype, int64_t num_rows, int64_t
                                               reinterpret_cast<uintptr_t>(workspace) % 256 != 0)))
     return set_error(MOE_B200_INVALID_ARGUMENT,
                      "%s: workspace must be 256-byte aligned and hold %zu bytes", kWhat, need);
+  const int64_t es = moe::dtype_bytes(dtype);
+  const Range in[] = {{x, num_rows * k * es}, {dy, num_rows * n * es},
+                      {expert_offsets, (num_experts + 1) * 4}};
+  const Range ws = {workspace, static_cast<int64_t>(need)};
+  rc = check_overlap(kWhat, {dw, num_experts * n * k * es}, {in[0], in[1], in[2], ws});
+  if (rc == MOE_B200_OK) rc = check_overlap(kWhat, ws, {in[0], in[1], in[2]});
+  if (rc != MOE_B200_OK) return rc;
   moe::GroupedArgs g{};
   g.dtype = dtype;
   g.dir = moe::kGmmGradWeight;
@@ -267,6 +302,15 @@ int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
       reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
     return set_error(MOE_B200_INVALID_ARGUMENT,
                      "%s: workspace must be 256-byte aligned and hold %zu bytes", kWhat, need);
+  const int64_t es = moe::dtype_bytes(dtype);
+  const Range in[] = {{x, num_rows * k * es}, {weight, n * k * es},
+                      {lora_a, num_adapters * rank * k * es},
+                      {lora_b, num_adapters * n * rank * es}, {adapter_ids, num_rows * 4},
+                      {scales, num_adapters * 4}};
+  const Range ws = {workspace, static_cast<int64_t>(need)};
+  rc = check_overlap(kWhat, {y, num_rows * n * es}, {in[0], in[1], in[2], in[3], in[4], in[5], ws});
+  if (rc == MOE_B200_OK) rc = check_overlap(kWhat, ws, {in[0], in[1], in[2], in[3], in[4], in[5]});
+  if (rc != MOE_B200_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   moe::LoraShrink l{};
   l.dtype = dtype;

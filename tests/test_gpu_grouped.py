@@ -340,3 +340,75 @@ def test_fp32_long_sums(pkg, dev, rows, feat, E):
     got = as_np(pkg.grouped_matmul_grad_weight(torch.full((LONG, feat), c, device=dev), dy, off))
     assert (np.abs(got[0] - exact) <= long_bound(exact)).all()
     assert (got[1] == 0).all()
+
+
+def test_output_over_an_input_is_refused(pkg, dev):
+    import torch
+    x = torch.zeros(8, 16, dtype=torch.float16, device=dev)
+    w = torch.zeros(1, 16, 16, dtype=torch.float16, device=dev)
+    off, _ = offsets_of([8], dev)
+    for call in (pkg.grouped_matmul, pkg.grouped_matmul_grad_input):
+        with pytest.raises(pkg.MoeB200Error, match="overlap"):
+            call(x, w, off, out=x)
+    both = torch.zeros(2, 8, 16, dtype=torch.float16, device=dev)
+    call(both[0], w, off, out=both[1])  # neighbours do not overlap
+
+
+# One process: its first call of every kernel happens inside a capture.
+FIRST_CALL_CAPTURED = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+from __graft_entry__ import load_package
+pkg = load_package()
+dev = torch.device("cuda", 0)
+off = torch.tensor([0, 300, 300, 600], dtype=torch.int32, device=dev)
+ids = torch.arange(600, dtype=torch.int32, device=dev) % 5 - 1
+sc = torch.ones(4, device=dev)
+calls = []
+for dt in (torch.float32, torch.bfloat16):
+    t = lambda *s: torch.randn(*s, device=dev).to(dt)
+    x, w, dy, a, b = t(600, 64), t(3, 128, 64), t(600, 128), t(4, 16, 64), t(4, 128, 16)
+    calls += [lambda x=x, w=w: pkg.grouped_matmul(x, w, off),
+              lambda dy=dy, w=w: pkg.grouped_matmul_grad_input(dy, w, off),
+              lambda x=x, dy=dy: pkg.grouped_matmul_grad_weight(x, dy, off),
+              lambda x=x, w=w, a=a, b=b: pkg.lora_matmul(x, w[0], a, b, ids, sc),
+              lambda x=x, w=w, a=a, b=b: pkg.lora_matmul(x[:3], w[0], a, b, ids[:3], sc)]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = [c() for c in calls]
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(o, c()) for o, c in zip(out, calls))
+"""
+
+
+def test_first_call_may_be_captured(dev):
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED, root], cwd=root, timeout=300,
+                          capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_traced_calls(pkg, dev, monkeypatch):
+    """With MOE_B200_TRACE_SYNC every call waits and looks for a device error: same bits."""
+    import torch
+    x, w, dy = make(dev, [300, 5, 0], 72, 64, "float16", seed=3)
+    off, _ = offsets_of([300, 5, 0], dev)
+    ids = torch.arange(x.shape[0], dtype=torch.int32, device=dev) % 3 - 1
+    a = torch.randn(2, 8, 64, device=dev).half()
+    b = torch.randn(2, 72, 8, device=dev).half()
+    sc = torch.ones(2, device=dev)
+
+    def all4():
+        return (pkg.grouped_matmul(x, w, off), pkg.grouped_matmul_grad_input(dy, w, off),
+                pkg.grouped_matmul_grad_weight(x, dy, off),
+                pkg.lora_matmul(x, w[0], a, b, ids, sc),
+                pkg.lora_matmul(x[:4], w[0], a, b, ids[:4], sc))
+
+    want = all4()
+    monkeypatch.setenv("MOE_B200_TRACE_SYNC", "1")
+    assert all(torch.equal(p, q) for p, q in zip(want, all4()))

@@ -127,3 +127,44 @@ def test_oracle_known_answers(orc):
     assert not dw[1].any()
     y, _, _ = orc.lora_matmul(x, np.eye(2), [[[1., 1.]]], [[[1.], [2.]]], [0, -1, 7], [0.5])
     np.testing.assert_array_equal(y, [[2.5, 5.0], [3, 4], [5, 6]])
+
+
+# Buffers of 4 rows, 16 x 16 and two groups or adapters, far apart but for the pair under test.
+FAR = [BUF + (i << 16) for i in range(8)]
+
+
+def _moved(i, to):
+    return [to if j == i else q for j, q in enumerate(FAR)]
+
+
+@pytest.mark.parametrize("call", [_fwd, _gin])
+@pytest.mark.parametrize("other,last", [("x", 4 * 16 * 2 - 16), ("w", 2 * 16 * 16 * 2 - 16),
+                                        ("off", 8)])
+def test_products_refuse_overlapping_output(pkg, call, other, last):
+    at = dict(x=FAR[0], w=FAR[1], off=FAR[2])
+    for y in (at[other], at[other] + last):
+        assert call(pkg, y=y, **at) == pkg.INVALID_ARGUMENT
+        assert b"overlap" in pkg.lib().moe_b200_last_error()
+
+
+@pytest.mark.parametrize("other,last", [("x", 4 * 16 * 2 - 16), ("w", 4 * 16 * 2 - 16),
+                                        ("off", 8)])
+def test_grad_weight_refuses_overlapping_buffers(pkg, other, last):
+    at = dict(x=FAR[0], w=FAR[1], off=FAR[2])  # (`w` is where this call takes dy)
+    for y in (at[other], at[other] + last, FAR[4]):
+        assert _gw(pkg, y=y, ws=FAR[4], **at) == pkg.INVALID_ARGUMENT
+        assert b"overlap" in pkg.lib().moe_b200_last_error()
+    assert _gw(pkg, y=FAR[3], ws=at[other], **at) == pkg.INVALID_ARGUMENT
+    assert b"overlap" in pkg.lib().moe_b200_last_error()
+
+
+@pytest.mark.parametrize("i", [0, 1, 2, 3, 4, 5, 7])
+def test_lora_refuses_overlapping_buffers(pkg, i):
+    # x, weight, lora_a, lora_b, adapter_ids, scales, y (6), workspace
+    at = _moved(6, FAR[i])
+    assert _lora(pkg, ptrs=tuple(at[:7]), ws=at[7]) == pkg.INVALID_ARGUMENT
+    assert b"overlap" in pkg.lib().moe_b200_last_error()
+    if i < 6:
+        at = _moved(7, FAR[i])
+        assert _lora(pkg, ptrs=tuple(at[:7]), ws=at[7]) == pkg.INVALID_ARGUMENT
+        assert b"overlap" in pkg.lib().moe_b200_last_error()
