@@ -55,34 +55,45 @@ struct Tile {
 };
 
 // Tile `L` of the list that holds, expert by expert, ceil(rows_e / tile_rows) tiles;
-// false when the list is shorter.  Called by all kThreads (>= E) threads.
+// false when the list is shorter.  Called by all NT threads, each of kMaxExperts / NT experts.
+template <int NT>
 __device__ bool find_tile(const int32_t* off, int E, int rows, int tile_rows, int L, Tile* out) {
-  __shared__ int s_warp[kThreads / 32];
+  constexpr int kPer = (kMaxExperts + NT - 1) / NT;
+  __shared__ int s_warp[NT / 32];
   __shared__ Tile s_tile;
-  const int e = threadIdx.x, lane = e & 31, warp = e >> 5;
-  int begin = 0, end = 0, n = 0;
-  if (e < E) {
-    begin = group_begin(off, e, rows);
-    end = group_end(off, e, rows, begin);
-    n = (end - begin + tile_rows - 1) / tile_rows;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int begin[kPer], end[kPer], n[kPer], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = threadIdx.x * kPer + i;
+    begin[i] = end[i] = n[i] = 0;
+    if (e < E) {
+      begin[i] = group_begin(off, e, rows);
+      end[i] = group_end(off, e, rows, begin[i]);
+      n[i] = (end[i] - begin[i] + tile_rows - 1) / tile_rows;
+    }
+    sum += n[i];
   }
-  int incl = n;
+  int incl = sum;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const int v = __shfl_up_sync(0xffffffffu, incl, d);
     if (lane >= d) incl += v;
   }
   if (lane == 31) s_warp[warp] = incl;
-  if (e == 0) s_tile.e = -1;
+  if (threadIdx.x == 0) s_tile.e = -1;
   __syncthreads();
-  int base = 0;
-  for (int w = 0; w < warp; ++w) base += s_warp[w];
-  const int first = base + incl - n;
-  if (n > 0 && L >= first && L < first + n) {
-    s_tile.e = e;
-    s_tile.index = L - first;
-    s_tile.begin = begin;
-    s_tile.end = end;
+  int first = incl - sum;
+  for (int w = 0; w < warp; ++w) first += s_warp[w];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (n[i] > 0 && L >= first && L < first + n[i]) {
+      s_tile.e = threadIdx.x * kPer + i;
+      s_tile.index = L - first;
+      s_tile.begin = begin[i];
+      s_tile.end = end[i];
+    }
+    first += n[i];
   }
   __syncthreads();
   *out = s_tile;
@@ -112,18 +123,18 @@ __device__ __forceinline__ float4 load4(const T* p, int n, int vec) {
 
 // One operand's slice: X rows x kDepth contraction entries into s[kDepth][X + pad].  CONTIG_C: element (i, c)
 // at p[i * ld + c], else at p[c * ld + i]; i < ni and c < nc are valid.
-template <typename T, int X, int kDepth, bool CONTIG_C>
+template <typename T, int X, int kDepth, bool CONTIG_C, int NT>
 struct Slice {
   static constexpr int kPitch = X + 4;
   static constexpr int kAll = X * kDepth / 4;
-  static constexpr int kQuads = (kAll + kThreads - 1) / kThreads;
+  static constexpr int kQuads = (kAll + NT - 1) / NT;
   float4 v[kQuads];
 
   __device__ __forceinline__ void load(const T* p, int64_t ld, int ni, int c0, int nc, int vec) {
 #pragma unroll
     for (int j = 0; j < kQuads; ++j) {
-      const int q = threadIdx.x + j * kThreads;
-      if (kAll % kThreads != 0 && q >= kAll) continue;
+      const int q = threadIdx.x + j * NT;
+      if (kAll % NT != 0 && q >= kAll) continue;
       if (CONTIG_C) {
         const int i = q / (kDepth / 4), c = c0 + (q % (kDepth / 4)) * 4;
         v[j] = i < ni && c < nc ? load4<T>(p + i * ld + c, nc - c, vec)
@@ -138,8 +149,8 @@ struct Slice {
   __device__ __forceinline__ void store(float* s) const {
 #pragma unroll
     for (int j = 0; j < kQuads; ++j) {
-      const int q = threadIdx.x + j * kThreads;
-      if (kAll % kThreads != 0 && q >= kAll) continue;
+      const int q = threadIdx.x + j * NT;
+      if (kAll % NT != 0 && q >= kAll) continue;
       if (CONTIG_C) {
         const int i = q / (kDepth / 4), c = (q % (kDepth / 4)) * 4;
         s[(c + 0) * kPitch + i] = v[j].x;
@@ -169,19 +180,25 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
-// CTA tile (16 TM) x (16 TN), TN a multiple of 4 and TM too or 1: thread (ty, tx) owns rows
-// ty * 4 + 64 i + [0, 4) (TM = 1: row ty) and columns tx * 4 + 64 j + [0, 4).
+// CTAs an SM: four of up to 64 rows, two of 128.  (64 x 64 tiles by 128 threads of 8 x 4 sums:
+// by 256 of 4 x 4, which load twice as much of shared memory for an FMA, 2000 rows in 4 groups of
+// [1111, 999] took 182 us in grad_input against 147; five CTAs an SM spill, 161.  128 x 128 by 128
+// threads of 16 x 8 took 817 us against 792 at 4096 rows, [2048, 2048], and spills when split.)
+__host__ __device__ constexpr int resident(int tm, int nt) { return tm * nt / 16 <= 64 ? 4 : 2; }
+
+// CTA tile (TY TM) x (16 TN) of NT = 16 TY threads, TN a multiple of 4 and TM too or 1: thread
+// (ty, tx) owns rows ty * 4 + 4 TY i + [0, 4) (TM = 1: row ty) and columns tx * 4 + 64 j + [0, 4).
 // SPLIT: the contraction may be split over a cluster; LORA: with the adapter term.  (Both in
 // every kernel spilled registers in the main loop of the 128 x 128 tiles: 10% of its time.)
-template <typename T, int DIR, int TM, int TN, bool SPLIT, bool LORA>
-__global__ void __launch_bounds__(kThreads, TM <= 4 ? 4 : 2)
+template <typename T, int DIR, int TM, int TN, int NT, bool SPLIT, bool LORA>
+__global__ void __launch_bounds__(NT, resident(TM, NT))
 grouped_simt_kernel(const SimtParams p) {
-  constexpr int BM = 16 * TM, BN = 16 * TN;
-  constexpr int kDepth = TM <= 4 ? 32 : 16;
+  constexpr int TY = NT / 16, BM = TY * TM, BN = 16 * TN;
+  constexpr int kDepth = BM <= 64 ? 32 : 16;
   constexpr bool kAC = DIR != kGmmGradWeight;  // contraction contiguous in A
   constexpr bool kBC = DIR == kGmmForward;
-  using SA = Slice<T, BM, kDepth, kAC>;
-  using SB = Slice<T, BN, kDepth, kBC>;
+  using SA = Slice<T, BM, kDepth, kAC, NT>;
+  using SB = Slice<T, BN, kDepth, kBC, NT>;
   constexpr int kSlice = kDepth * (SA::kPitch + SB::kPitch);
   __shared__ __align__(16) float operands[2 * kSlice];
   auto sa = [&](int buf) { return operands + buf * kSlice; };
@@ -208,7 +225,7 @@ grouped_simt_kernel(const SimtParams p) {
     nn = p.K - col0;
   } else {
     Tile t;
-    if (!find_tile(p.offsets, p.E, rows, BM, blockIdx.x, &t)) return;
+    if (!find_tile<NT>(p.offsets, p.E, rows, BM, blockIdx.x, &t)) return;
     const int feat = DIR == kGmmForward ? p.N : p.K;
     nc = DIR == kGmmForward ? p.K : p.N;
     row0 = t.begin + t.index * BM;
@@ -286,7 +303,7 @@ grouped_simt_kernel(const SimtParams p) {
 #pragma unroll
             for (int i = 0; i < TM; i += 4)
               *reinterpret_cast<float4*>(ra + i) =
-                  *reinterpret_cast<const float4*>(&a_now[c * SA::kPitch + ty * 4 + i * 16]);
+                  *reinterpret_cast<const float4*>(&a_now[c * SA::kPitch + ty * 4 + i * TY]);
           }
 #pragma unroll
           for (int j = 0; j < TN; j += 4)
@@ -328,7 +345,7 @@ grouped_simt_kernel(const SimtParams p) {
     // The cluster's parts: row i of each thread goes to CTA i S / TM (TM = 1: the thread's row to CTA ty % S), which
     // adds the parts in rank order; four columns at a time.
     float4* parts = reinterpret_cast<float4*>(operands);  // [S - 1][rows owned][256]
-    static_assert(sizeof(operands) >= 3 * ((TM + 3) / 4) * kThreads * 16, "parts fit the operands");
+    static_assert(sizeof(operands) >= 3 * ((TM + 3) / 4) * NT * 16, "parts fit the operands");
     const int per = TM == 1 ? 1 : TM / S;
 #pragma unroll
     for (int j = 0; j < TN; j += 4) {
@@ -338,7 +355,7 @@ grouped_simt_kernel(const SimtParams p) {
         const int owner = TM == 1 ? ty % S : i / per;
         if (owner == me) continue;
         const int slot = me < owner ? me : me - 1;
-        const uint32_t at = smem_u32(parts + (slot * per + i % per) * kThreads + threadIdx.x);
+        const uint32_t at = smem_u32(parts + (slot * per + i % per) * NT + threadIdx.x);
         asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
                          mapa_shared(at, owner)),
                      "f"(acc[i][j]), "f"(acc[i][j + 1]), "f"(acc[i][j + 2]), "f"(acc[i][j + 3])
@@ -352,7 +369,7 @@ grouped_simt_kernel(const SimtParams p) {
         for (int r = 0; r < S; ++r) {
           const float4 v =
               r == me ? make_float4(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3])
-                      : parts[((r < me ? r : r - 1) * per + i % per) * kThreads + threadIdx.x];
+                      : parts[((r < me ? r : r - 1) * per + i % per) * NT + threadIdx.x];
           sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
         }
         acc[i][j] = sum.x; acc[i][j + 1] = sum.y; acc[i][j + 2] = sum.z; acc[i][j + 3] = sum.w;
@@ -362,7 +379,7 @@ grouped_simt_kernel(const SimtParams p) {
 
   // Whether this CTA finishes row i of each thread.
   auto owned = [&](int i) { return S == 1 || (TM == 1 ? ty % S : i * S / TM) == me; };
-  auto row_of = [&](int i) { return TM == 1 ? ty : ty * 4 + (i / 4) * 64 + (i & 3); };
+  auto row_of = [&](int i) { return TM == 1 ? ty : ty * 4 + (i / 4) * 4 * TY + (i & 3); };
   if constexpr (LORA) {
     // The adapter term (t holds s_a A_a x).  Rows of other adapters skip an adapter's FMAs, so
     // that what it holds (an infinity, say) stays with its own rows.
@@ -370,12 +387,12 @@ grouped_simt_kernel(const SimtParams p) {
     __shared__ int s_count;
     if (threadIdx.x == 0) s_count = 0;
     const int r = p.lora.rank;
-    for (int m = threadIdx.x; m < BM; m += kThreads) {
+    for (int m = threadIdx.x; m < BM; m += NT) {
       const int id = m < nm ? __ldg(p.lora.ids + row0 + m) : -1;
       s_ad[m] = id >= 0 && id < p.lora.adapters ? id : -1;
     }
     __syncthreads();
-    for (int m = threadIdx.x; m < BM; m += kThreads) {
+    for (int m = threadIdx.x; m < BM; m += NT) {
       const int id = s_ad[m];
       int k = 0;
       if (id >= 0)
@@ -409,8 +426,8 @@ grouped_simt_kernel(const SimtParams p) {
     } else {
       // Few (prompts): slices of t against B_a, adapter by adapter.  (A row's sums come from one
       // adapter, so the list's order does not show.)
-      Slice<float, BM, kDepth, true> ft;
-      Slice<T, BN, kDepth, true> fl;
+      Slice<float, BM, kDepth, true, NT> ft;
+      Slice<T, BN, kDepth, true, NT> fl;
       const float *a_now = sa(0), *b_now = sb(0);
       for (int d = 0; d < s_count; ++d) {
         const int ad = s_list[d];
@@ -534,9 +551,9 @@ cudaError_t launch_gemv(const SimtParams& p, cudaStream_t s) {
                           dim3(kThreads), 0, s, p);
 }
 
-template <typename T, int DIR, int TM, int TN, bool LORA>
+template <typename T, int DIR, int TM, int TN, int NT, bool LORA>
 cudaError_t launch_tile(const GroupedArgs& g, SimtParams p, cudaStream_t s) {
-  constexpr int BM = 16 * TM, BN = 16 * TN;
+  constexpr int BM = NT / 16 * TM, BN = 16 * TN;
   dim3 grid;
   p.splits = 1;
   int64_t tiles, con;
@@ -554,12 +571,12 @@ cudaError_t launch_tile(const GroupedArgs& g, SimtParams p, cudaStream_t s) {
   }
   // Split until the SMs' resident CTAs run (four, of 128 x 128 tiles two), with a contraction
   // of at least 64 each.
-  const int64_t fill = 148 * (TM <= 4 ? 4 : 2);
+  const int64_t fill = 148 * resident(TM, NT);
   while (p.splits < 4 && tiles * p.splits * 2 <= fill && con >= 128 * p.splits) p.splits *= 2;
   grid.z *= p.splits;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(NT);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -570,9 +587,9 @@ cudaError_t launch_tile(const GroupedArgs& g, SimtParams p, cudaStream_t s) {
   attr[1].val.clusterDim.z = static_cast<unsigned>(p.splits);
   cfg.attrs = attr;
   cfg.numAttrs = p.splits > 1 ? 2 : 1;
-  if (TM <= 4 || p.splits > 1)
-    return cudaLaunchKernelEx(&cfg, grouped_simt_kernel<T, DIR, TM, TN, true, LORA>, p);
-  return cudaLaunchKernelEx(&cfg, grouped_simt_kernel<T, DIR, TM, TN, TM <= 4, LORA>, p);
+  if (BM <= 64 || p.splits > 1)
+    return cudaLaunchKernelEx(&cfg, grouped_simt_kernel<T, DIR, TM, TN, NT, true, LORA>, p);
+  return cudaLaunchKernelEx(&cfg, grouped_simt_kernel<T, DIR, TM, TN, NT, BM <= 64, LORA>, p);
 }
 
 template <typename T, int DIR, bool LORA>
@@ -596,8 +613,11 @@ cudaError_t launch_dir(const GroupedArgs& g, const LoraTerm* lora, cudaStream_t 
     if (g.rows <= (g.E == 1 ? kGemvRows : 4 * static_cast<int64_t>(g.E))) return launch_gemv<T>(p, s);
   }
   // 128 x 128 tiles where groups fill them and they, split four ways, fill the GPU (each thread
-  // then does 64 FMAs per 16 shared loads instead of 16 per 8); else 64 x 64, and 16 rows for
-  // groups of a few rows, which multiply less padding.
+  // then does 64 FMAs per 16 shared loads instead of 32 per 12); else 64 x 64, and 16 rows for
+  // groups of a few rows, which multiply less padding.  Several groups pad the tall tiles more
+  // and want twice as many of them (fp32, 128 : 64 rows, us: 500 rows in 4 groups, grad_input of
+  // [1024, 2048] 112 : 94, of [640, 2048] 75 : 60; one group of 1000 rows, [1024, 1024], 67 : 72;
+  // below 148 tiles the small ones won in every case measured, 4 groups [1024, 2048] 116 : 104).
   const int64_t feat = DIR == kGmmForward ? g.N : g.K;
   const int64_t big = DIR == kGmmGradWeight
                           ? static_cast<int64_t>(g.E) * ((g.N + 127) / 128) * ((g.K + 127) / 128)
@@ -605,11 +625,13 @@ cudaError_t launch_dir(const GroupedArgs& g, const LoraTerm* lora, cudaStream_t 
   const int64_t height = DIR == kGmmGradWeight ? g.N : g.rows / g.E;
   // (With element-wise loads the small tiles win until the big ones fill the GPU unsplit.)
   const int64_t ways = p.a_vec && p.b_vec ? 4 : 1;
-  if (height >= 96 && feat >= 96 && ways * big >= 148) return launch_tile<T, DIR, 8, 8, LORA>(g, p, s);
+  const int64_t enough = ways == 4 && g.E > 1 && DIR != kGmmGradWeight ? 300 : 148;
+  if (height >= 96 && feat >= 96 && ways * big >= enough)
+    return launch_tile<T, DIR, 8, 8, 256, LORA>(g, p, s);
   if constexpr (DIR != kGmmGradWeight) {
-    if (g.rows <= 16 * static_cast<int64_t>(g.E)) return launch_tile<T, DIR, 1, 4, LORA>(g, p, s);
+    if (g.rows <= 16 * static_cast<int64_t>(g.E)) return launch_tile<T, DIR, 1, 4, 256, LORA>(g, p, s);
   }
-  return launch_tile<T, DIR, 4, 4, LORA>(g, p, s);
+  return launch_tile<T, DIR, 8, 4, 128, LORA>(g, p, s);
 }
 
 template <typename T>
@@ -623,7 +645,6 @@ cudaError_t launch_type(const GroupedArgs& g, const LoraTerm* lora, cudaStream_t
 }  // namespace
 
 cudaError_t launch_grouped_simt(const GroupedArgs& g, const LoraTerm* lora, cudaStream_t s) {
-  static_assert(kThreads >= kMaxExperts, "find_tile needs a thread per expert");
   if (g.dtype == kDtF32) return launch_type<float>(g, lora, s);
   if (g.dtype == kDtF16) return launch_type<__half>(g, lora, s);
   if (g.dtype == kDtBF16) return launch_type<__nv_bfloat16>(g, lora, s);
