@@ -17,6 +17,9 @@
 // The adapter term (LORA) does not wait for the product: while the weights stream, the
 // epilogue warps form it for the blocks that they will finish and park it in the other half
 // of the CTA's tensor memory.
+//
+// A CTA with more than one segment of slices (kSegment) hands its accumulator to the epilogue
+// warps after each but the last; they keep the sum of the segments in the other half.
 #include <algorithm>
 
 #include "grouped_lora.cuh"
@@ -67,9 +70,6 @@ __device__ __forceinline__ void tmem_st_frag1(uint32_t taddr, const float (&v)[4
                "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3]))
                : "memory");
 }
-__device__ __forceinline__ void tmem_st_wait() {
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
 // 16 bytes to another CTA's shared memory, counted on that CTA's barrier `bar`.
 __device__ __forceinline__ void st_async_f4(uint32_t addr, const float (&v)[4], uint32_t bar) {
   asm volatile(
@@ -84,7 +84,8 @@ __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <typename T, int DIR, int LORA>
+// SEG: a CTA may have more than one segment of slices.
+template <typename T, int DIR, int LORA, bool SEG>
 __global__ void __launch_bounds__(LORA > 0 ? 512 : kThreads, LORA > 0 ? 1 : 2)  // 128 / 96 registers
 grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
                      const __grid_constant__ CUtensorMap map_x, const SmallParams p) {
@@ -98,9 +99,11 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
   uint64_t* empty = full + kMaxStages;
   uint64_t* tfull = empty + kMaxStages;
   uint64_t* xfull = tfull + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(xfull + 1);
+  uint64_t* sfull = xfull + 1;   // a segment that is not the last is complete
+  uint64_t* sempty = sfull + 1;  // ... and has been added to the sum
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sempty + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((2 * kMaxStages + 2) * 8 + 8 <= 256, "barrier block");
+  static_assert((2 * kMaxStages + 4) * 8 + 8 <= 256, "barrier block");
   GroupTable table;
   table.rows = reinterpret_cast<int2*>(full + 32);
   table.tiles = reinterpret_cast<int*>(table.rows + kMaxExperts);
@@ -116,6 +119,8 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
     }
     mbar_init(tfull, 1);
     mbar_init(xfull, 1);
+    mbar_init(sfull, 1);
+    mbar_init(sempty, blockDim.x / 32 - 2);
     *abort_flag = 0;
     fence_mbarrier_init();
     tma_prefetch_desc(&map_w);
@@ -157,6 +162,7 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
   // The CTAs of a cluster take the slices in turn: what they read at a time then lies side by
   // side in each weight row (2 to 4% on the streamed bytes).
   const int s0 = split, s1 = slices, ds = p.splits;
+  const int segments = SEG ? segments_of((s1 - s0 + ds - 1) / ds) : 1;
 
   if (warp == 0 && lane == 0) {
     const int boxes = (nt + p.box - 1) / p.box;
@@ -184,10 +190,17 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
     }
   } else if (warp == 1 && lane == 0) {
     const uint32_t idesc = idesc_f16(TcFormat<T>::kId, kTileM, nt) | (kAMn ? kIdescAMn : 0);
-    int stage = 0;
-    uint32_t phase = 0;
+    int stage = 0, left = kSegment;  // slices until the segment is complete
+    uint32_t phase = 0, seg = 0;
     for (int s = s0; s < s1; s += ds) {
-      if (!mbar_wait(&full[stage], phase)) {
+      bool ok = true;
+      if (SEG && left == 0) {
+        tc_commit(sfull);
+        if (LORA > 0) pdl_wait();  // the epilogue warps wait for the launch before
+        ok = mbar_wait(sempty, seg++ & 1);
+        left = kSegment;
+      }
+      if (!ok || !mbar_wait(&full[stage], phase)) {
         atomicExch(&g_small_error, kErrTimeoutMma);
         *abort_flag = 1;
         break;
@@ -199,8 +212,9 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
         const uint64_t ad = kAMn ? smem_desc_mn_sw128(w + k * 2048, kWBytes / 2)
                                  : smem_desc_k_sw128(w + k * 32);
         tc_mma_f16(tmem, ad, smem_desc_k_sw128(w + kWBytes + k * 32), idesc,
-                   (s != s0 || k != 0) ? 1u : 0u);
+                   (left != kSegment || k != 0) ? 1u : 0u);
       }
+      --left;
       tc_commit(&empty[stage]);
       if (++stage == p.stages) { stage = 0; phase ^= 1; }
     }
@@ -218,6 +232,8 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
   const int q = warp & 3, pair = (warp - 2) >> 2, turns = (blockDim.x - 64) / 128;
   const int feat = m0 + q * 32;
   const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16);
+  // Per block: the adapter term (of the owned blocks) and the segments before the last.
+  const uint32_t tsum = taddr + p.cap;
   if (threadIdx.x == 64 && S > 1 && owned > 0)
     mbar_arrive_expect_tx(xfull, owned * (S - 1) * kPartBytes);
   if constexpr (LORA > 0) {
@@ -255,8 +271,8 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
         }
         batch.apply(p.lora, p.total_rows, ad, row0 + row, feat, p.m_dim, parts, lo, hi);
         if (todo != 0) continue;
-        tmem_st_frag1(taddr + p.cap + 8 * i, lo);
-        tmem_st_frag1(taddr + (16u << 16) + p.cap + 8 * i, hi);
+        tmem_st_frag1(tsum + 8 * (i * S + split), lo);
+        tmem_st_frag1(tsum + (16u << 16) + 8 * (i * S + split), hi);
         i += turns;
         if (i >= owned) break;
         row = row_next;
@@ -273,6 +289,32 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
       pdl_wait();
     }
     __syncwarp();
+  }
+
+  for (int seg = 0; epi && seg < segments - 1; ++seg) {
+    if (!mbar_wait(sfull, seg & 1)) break;  // (tfull will not complete either)
+    tc_fence_after();
+    // Each warp adds what it will send or finish below.
+    auto add = [&](int b, bool first) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t at = (static_cast<uint32_t>(16 * h) << 16) + 8 * b;
+        float a[4], s[4] = {0.f, 0.f, 0.f, 0.f};
+        tmem_ld_frag1(taddr + at, a);
+        if (!first) tmem_ld_frag1(tsum + at, s);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] += a[j];
+        tmem_st_frag1(tsum + at, s);
+      }
+    };
+    for (int b = pair; b < blocks; b += turns)
+      if (b % S != split) add(b, seg == 0);
+    for (int i = pair; i < owned; i += turns) add(i * S + split, LORA == 0 && seg == 0);
+    tmem_st_wait();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(sempty);
   }
 
   const bool ok = mbar_wait(tfull, 0);
@@ -297,6 +339,14 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
           tmem_ld_frag1(taddr + 8 * b, lo);
           tmem_ld_frag1(taddr + (16u << 16) + 8 * b, hi);
           tmem_ld_wait();
+          if (segments > 1) {
+            float slo[4], shi[4];
+            tmem_ld_frag1(tsum + 8 * b, slo);
+            tmem_ld_frag1(tsum + (16u << 16) + 8 * b, shi);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { lo[j] += slo[j]; hi[j] += shi[j]; }
+          }
         }
         // Slot of this sender among the owner's S - 1, block b / S of the owner's.
         const int slot = split < owner ? split : split - 1;
@@ -324,9 +374,9 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
       tmem_ld_frag1(taddr + 8 * b, own_lo);
       tmem_ld_frag1(taddr + (16u << 16) + 8 * b, own_hi);
     }
-    if constexpr (LORA > 0) {
-      tmem_ld_frag1(taddr + p.cap + 8 * i, add_lo);
-      tmem_ld_frag1(taddr + (16u << 16) + p.cap + 8 * i, add_hi);
+    if (LORA > 0 || segments > 1) {
+      tmem_ld_frag1(tsum + 8 * b, add_lo);
+      tmem_ld_frag1(tsum + (16u << 16) + 8 * b, add_hi);
     }
     tmem_ld_wait();
     for (int r = 0; r < S; ++r) {  // the parts in rank order
@@ -342,7 +392,7 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
         hi[0] += c.x; hi[1] += c.y; hi[2] += c.z; hi[3] += c.w;
       }
     }
-    if constexpr (LORA > 0) {
+    if (LORA > 0 || segments > 1) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) { lo[j] += add_lo[j]; hi[j] += add_hi[j]; }
     }
@@ -386,8 +436,8 @@ cudaError_t launch_small(const GroupedArgs& g, const LoraTerm* lora, int num_sms
   p.stage_bytes = kWBytes + p.cap * kBK * 2;
   // Tensor memory of the CTAs that fit an SM together never exceeds its 512 columns (a CTA
   // of these kernels takes at least 90 KB of shared memory per 256 columns), so an
-  // allocation never waits for a CTA that waits for its own cluster.
-  p.tmem_cols = static_cast<uint32_t>(std::max(32, p.cap * (LORA > 0 ? 2 : 1)));
+  // allocation never waits for a CTA that waits for its own cluster.  (The second half: the
+  // adapter term, the sum of the segments.)
   // The tile count lives on the device; each ragged group adds at most one.
   const int64_t tiles = (g.E == 1 ? (g.rows + p.cap - 1) / p.cap
                                   : g.rows / p.cap + std::min<int64_t>(g.rows, g.E)) *
@@ -408,6 +458,8 @@ cudaError_t launch_small(const GroupedArgs& g, const LoraTerm* lora, int num_sms
   const int most = resident == 1 && tiles * 8 > 64 ? 4 : 8;
   p.splits = 1;
   while (p.splits < most && tiles * p.splits * 2 <= fill && slices >= 4 * p.splits) p.splits *= 2;
+  const bool seg = segments_of((slices + p.splits - 1) / p.splits) > 1;
+  p.tmem_cols = static_cast<uint32_t>(std::max(32, p.cap * (LORA > 0 || seg ? 2 : 1)));
   // The exchange has its own memory up to 64 rows (at most 28 KB); above, it reuses the ring
   // and the cluster meets once more before it.
   const int blocks_owned = (p.cap / 8 + p.splits - 1) / p.splits;
@@ -418,12 +470,15 @@ cudaError_t launch_small(const GroupedArgs& g, const LoraTerm* lora, int num_sms
       !grouped_map(&mx, g.dtype, DIR == kGmmForward ? g.x : g.dy, p.con, g.rows, 1, p.box))
     return cudaErrorInvalidValue;
   const int smem = kFixed + p.stages * p.stage_bytes + p.part_bytes;
-  static SmemOptIn opt_in;
-  cudaError_t st = opt_in.set(grouped_small_kernel<T, DIR, LORA>, 227 * 1024);
-  if (st != cudaSuccess) return st;
-  return launch_overlapped(grouped_small_kernel<T, DIR, LORA>,
-                           static_cast<unsigned>(tiles * p.splits), threads, smem, p.splits, s,
-                           mw, mx, p);
+  auto launch = [&](auto kernel, SmemOptIn& opt_in) {
+    cudaError_t st = opt_in.set(kernel, 227 * 1024);
+    if (st != cudaSuccess) return st;
+    return launch_overlapped(kernel, static_cast<unsigned>(tiles * p.splits), threads, smem,
+                             p.splits, s, mw, mx, p);
+  };
+  static SmemOptIn one, many;
+  return seg ? launch(grouped_small_kernel<T, DIR, LORA, true>, many)
+             : launch(grouped_small_kernel<T, DIR, LORA, false>, one);
 }
 
 template <typename T>

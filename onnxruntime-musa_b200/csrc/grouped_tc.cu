@@ -24,6 +24,13 @@
 // over 8 experts of [4096, 14336], fp16, 752 us (1.28); in long loops the power limit takes 15
 // to 20%.
 //
+// Contractions of more than one segment (kSegment slices: grad_weight of more than 16384 rows of
+// an expert, mostly) are added up in tensor memory: after each segment but the last the epilogue
+// warps add the accumulator to a sum in the other accumulator's columns and leave the rounding
+// error of that addition in the accumulator, where the next segment starts from it.  So the
+// length of the sum does not show in the result, and no wait is longer than a segment.  Such a
+// tile has both accumulators, and the tile after it waits for its epilogue.
+//
 // The adapter projection is the forward product of one group, and its adapter term more
 // slices of the same accumulator where sixteen adjacent rows (counted from the tile's first)
 // follow one adapter: B_a as the M operand, the rows' parts (grouped_lora.cuh) as the N
@@ -165,6 +172,34 @@ __device__ __forceinline__ void fence_proxy_async_all() {
   asm volatile("fence.proxy.async;" ::: "memory");
 }
 
+// Adds the 32 lanes x 32 columns of an accumulator at `acc` to the sum at `sum` and leaves the
+// rounding error of each addition (exact, by the six operations of a two-sum) in the
+// accumulator; a sum that is not finite leaves none.  After the last segment the whole sum goes
+// to the accumulator.
+__device__ __forceinline__ void add_segment(uint32_t acc, uint32_t sum, bool first, bool last) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h, acc += 16u << 16, sum += 16u << 16) {
+    float a[16], s[16];
+    tmem_ld_frag4(acc, a);
+    if (!first) tmem_ld_frag4(sum, s);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      if (first) {
+        s[j] = a[j];
+        a[j] = 0.f;
+      } else {
+        const float t = __fadd_rn(s[j], a[j]), u = __fsub_rn(t, s[j]);
+        const float e = __fadd_rn(__fsub_rn(s[j], __fsub_rn(t, u)), __fsub_rn(a[j], u));
+        s[j] = t;
+        a[j] = last ? t : isfinite(t) ? e : 0.f;
+      }
+    }
+    if (!last) tmem_st_frag4(sum, s);
+    tmem_st_frag4(acc, a);
+  }
+}
+
 // MMA steps of 16 in slice `b` of the tile.
 template <int DIR>
 __device__ __forceinline__ int block_steps(const PairTile& t, int b) {
@@ -180,7 +215,8 @@ __device__ __forceinline__ bool is_tail(const PairTile& t, int b) {
 }
 
 // LORA: 16-entry steps of the rank per register block of the adapter term, 0 without one.
-template <typename T, int DIR, int LORA>
+// SEG: contractions may have more than one segment.
+template <typename T, int DIR, int LORA, bool SEG>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LORA > 0 ? kLoraThreads : kThreads, 1)
 grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
                     const __grid_constant__ CUtensorMap map_b,
@@ -340,6 +376,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
     if (lane == 0 && leader) {
       int stage = 0;
       uint32_t phase = 0;
+      uint32_t fills = 0;   // bit a: parity of accumulator a's next fill
+      bool both = false;    // the tile before has its sum in the other accumulator
+      auto drained = [&](int a) { return mbar_wait(&tempty[a], (fills >> a & 1) ^ 1); };
       for (int i = 0;; ++i) {
         const int L = turn_tile(i, pair, npairs);
         if (L >= total || *abort_flag) break;
@@ -347,7 +386,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
         const uint32_t idesc = idesc_f16(TcFormat<T>::kId, kTileM, t.nt) |
                                (kAMn ? kIdescAMn : 0) | (kBMn ? kIdescBMn : 0);
         const int acc = i & 1;
-        if (!mbar_wait(&tempty[acc], ((i >> 1) & 1) ^ 1)) {
+        if (!drained(acc) || (SEG && both && !drained(acc ^ 1))) {
           atomicExch(&g_pair_error, kErrTimeoutMma);
           *abort_flag = 1;
           break;
@@ -355,8 +394,15 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
         tc_fence_after();
         const uint32_t d = tmem_base + acc * kTileN;
         bool ok = true;
+        both = t.blocks > kSegment;
         for (int b = 0; b < t.blocks; ++b) {
-          if (!mbar_wait(&full[stage], phase)) {
+          if (SEG && b != 0 && b % kSegment == 0) {  // a segment is complete: the epilogue takes it
+            tc_commit_pair(&tfull[acc], 0x3);
+            fills ^= 1u << acc;
+            ok = drained(acc);
+            tc_fence_after();
+          }
+          if (!ok || !mbar_wait(&full[stage], phase)) {
             atomicExch(&g_pair_error, kErrTimeoutMma);
             *abort_flag = 1;
             ok = false;
@@ -410,6 +456,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
         }
         if (!ok) break;
         tc_commit_pair(&tfull[acc], 0x3);
+        fills ^= 1u << acc;
       }
       tc_commit_pair(done, 0x1);
       mbar_wait(done, 0);
@@ -452,19 +499,34 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
     const uint8_t* rd_ptr = buf + rd_row * kStageRow + ((rd_blk ^ ((rd_row >> 1) & 3)) << 4);
     T* out = static_cast<T*>(p.out);
     if (LORA > 0) pdl_wait();
+    uint32_t fills = 0;  // as the MMA warp's
     for (int i = 0;; ++i) {
       const int L = turn_tile(i, pair, npairs);
       if (L >= total || *abort_flag) break;
       const PairTile t = pair_tile<DIR>(L, table, p);
-      const int acc = i & 1;
-      if (!mbar_wait(&tfull[acc], (i >> 1) & 1)) {
+      const int acc = i & 1, segments = SEG ? segments_of(t.blocks) : 1;
+      const uint32_t taddr =
+          tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * kTileN;
+      const uint32_t tsum = taddr + (acc ? -kTileN : kTileN);  // sum of the segments before
+      bool ok = true;
+      for (int seg = 0; ok && seg < segments; ++seg) {
+        ok = mbar_wait(&tfull[acc], fills >> acc & 1);
+        fills ^= 1u << acc;
+        tc_fence_after();
+        if (!ok || segments == 1) break;
+        for (int c = first; c < t.n; c += 64)
+          add_segment(taddr + c, tsum + c, seg == 0, seg == segments - 1);
+        tmem_st_wait();
+        if (seg == segments - 1) break;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));
+      }
+      if (!ok) {
         atomicExch(&g_pair_error, kErrTimeoutEpilogue);
         *abort_flag = 1;
         break;
       }
-      tc_fence_after();
-      const uint32_t taddr =
-          tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * kTileN;
       const int m = t.m0 + static_cast<int>(rank) * 128 + q * 32;  // first M entry of the warp
       const bool zero = DIR == kGmmGradWeight && t.cnt == 0;  // an expert without rows
       auto release = [&] {  // this warp has read the accumulator
@@ -671,7 +733,7 @@ int tile_rows_one_group(int64_t rows, int m_tiles, int pairs) {
   return best;
 }
 
-template <typename T, int DIR, int LORA>
+template <typename T, int DIR, int LORA, bool SEG>
 cudaError_t launch_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms, cudaStream_t s) {
   CUtensorMap ma, mb, mat, mbt;
   PairParams p{};
@@ -727,11 +789,20 @@ cudaError_t launch_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
                          : g.rows / p.tile_rows + std::min<int64_t>(g.rows, g.E)) *
                     p.m_tiles;
   static SmemOptIn opt_in;
-  cudaError_t st = opt_in.set(grouped_pair_kernel<T, DIR, LORA>, kSmem);
+  cudaError_t st = opt_in.set(grouped_pair_kernel<T, DIR, LORA, SEG>, kSmem);
   if (st != cudaSuccess) return st;
   const int64_t pairs = std::min<int64_t>(tiles, num_sms / 2);
-  return launch_overlapped(grouped_pair_kernel<T, DIR, LORA>, static_cast<unsigned>(2 * pairs),
+  return launch_overlapped(grouped_pair_kernel<T, DIR, LORA, SEG>, static_cast<unsigned>(2 * pairs),
                            LORA > 0 ? kLoraThreads : kThreads, kSmem, 0, s, ma, mb, mat, mbt, p);
+}
+
+template <typename T, int DIR, int LORA>
+cudaError_t launch_pair_seg(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
+                            cudaStream_t s) {
+  // The rows of an expert are known on the device only.
+  const int64_t con = DIR == kGmmForward ? g.K : DIR == kGmmGradInput ? g.N : g.rows;
+  return con <= kSegment * kBK ? launch_pair<T, DIR, LORA, false>(g, lora, num_sms, s)
+                               : launch_pair<T, DIR, LORA, true>(g, lora, num_sms, s);
 }
 
 template <typename T>
@@ -739,11 +810,11 @@ cudaError_t launch_pair_type(const GroupedArgs& g, const LoraTerm* lora, int num
                              cudaStream_t s) {
   // Ranks up to 16 keep one step in registers, larger ones blocks of four.
   if (lora != nullptr)
-    return lora->steps == 1 ? launch_pair<T, kGmmForward, 1>(g, lora, num_sms, s)
-                            : launch_pair<T, kGmmForward, 4>(g, lora, num_sms, s);
-  if (g.dir == kGmmForward) return launch_pair<T, kGmmForward, 0>(g, nullptr, num_sms, s);
-  if (g.dir == kGmmGradInput) return launch_pair<T, kGmmGradInput, 0>(g, nullptr, num_sms, s);
-  return launch_pair<T, kGmmGradWeight, 0>(g, nullptr, num_sms, s);
+    return lora->steps == 1 ? launch_pair_seg<T, kGmmForward, 1>(g, lora, num_sms, s)
+                            : launch_pair_seg<T, kGmmForward, 4>(g, lora, num_sms, s);
+  if (g.dir == kGmmForward) return launch_pair_seg<T, kGmmForward, 0>(g, nullptr, num_sms, s);
+  if (g.dir == kGmmGradInput) return launch_pair_seg<T, kGmmGradInput, 0>(g, nullptr, num_sms, s);
+  return launch_pair_seg<T, kGmmGradWeight, 0>(g, nullptr, num_sms, s);
 }
 
 }  // namespace

@@ -33,6 +33,37 @@ __device__ __forceinline__ void tmem_ld_frag4(uint32_t taddr, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// The reverse of tmem_ld_frag4; tmem_st_wait() before anyone else reads.
+__device__ __forceinline__ void tmem_st_frag4(uint32_t taddr, const float (&v)[16]) {
+  uint32_t r[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(v[i]);
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// Most slices (of 64 contraction entries) that one accumulator takes: 16384 entries.  tcgen05
+// cuts products off when it aligns them to the running sum, always towards zero, so a long sum
+// of one sign drifts: 2^19 rows in one accumulator came out 0.4% low, eight half steps of fp16.
+// 1024 steps of 16 entries lose at most 2^-12 of the magnitudes; longer contractions are added
+// up from such segments in fp32, rounded to nearest.  It also bounds every wait on an
+// accumulator: a segment is 256 slices of some 512 cycles, tens of microseconds.  (Shorter
+// segments lose less, but most layers' contractions then pay for the extra pass over tensor
+// memory: up to 16384 there is none.  The kernels that can add segments up are instantiations of
+// their own, taken where a contraction may be longer: in the others that code, never run, cost 2
+// to 5%, fc2 of 296 rows over 64 experts 38.2 -> 39.9 us.)
+constexpr int kSegment = 256;
+__host__ __device__ constexpr int segments_of(int slices) {
+  return slices <= kSegment ? 1 : (slices + kSegment - 1) / kSegment;
+}
+
 // Four 8 x 8 blocks of 16-bit elements to shared memory; lane 8i + t gives the address of
 // row t of block i (16 bytes).  _t: each block transposed.
 __device__ __forceinline__ void stmatrix4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,

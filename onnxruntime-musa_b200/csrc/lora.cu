@@ -8,7 +8,9 @@
 // of K.  The A_a of the chunk's distinct adapters are stacked as the MMA's M (128 / r
 // adapters a pass), its rows are the N, and each column keeps the lanes of its own adapter:
 // rows need no sorting, and another adapter's values never reach a row.  One prompt in a
-// chunk is one pass; a decode chunk of 4 rows is at most 4 adapters, read once each.
+// chunk is one pass; a decode chunk of 4 rows is at most 4 adapters, read once each.  A pass
+// over more than one segment of slices (kSegment) takes an accumulator for each, which the
+// epilogue adds up.
 // Bound: the bytes of A_a (decode) and of x (prefill); the products are few.  The splits of
 // a chunk are a cluster: each leaves its partial sums in shared memory, and each row's are
 // added in rank order by one warp, which scales them and splits them into the 16-bit parts
@@ -141,7 +143,8 @@ __device__ __forceinline__ void split_parts(const float4& v, uint2& hi, uint2& l
   lo = make_uint2(pack2<T>(v.x - h0, v.y - h1), pack2<T>(v.z - h2, v.w - h3));
 }
 
-template <typename T>
+// SEG: a CTA may have more than one segment of slices.
+template <typename T, bool SEG>
 __global__ void __launch_bounds__(kTcThreads)
 lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
                       const __grid_constant__ CUtensorMap map_a, const ShrinkParams p) {
@@ -232,6 +235,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
   const int slices = (p.K + kBK - 1) / kBK;
   const int s0 = static_cast<int>(static_cast<int64_t>(slices) * split / p.splits);
   const int s1 = static_cast<int>(static_cast<int64_t>(slices) * (split + 1) / p.splits);
+  const int segments = SEG ? segments_of(s1 - s0) : 1;
 
   if (warp == 0) {
     // Lane 0 waits for the slot and loads x; lane u loads the rows of unit u (up to 16 boxes
@@ -270,11 +274,13 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int ps = 0; ps < passes && ok; ++ps) {
-        const int acc = ps & 1;
-        ok = mbar_wait(&tempty[acc], ((ps >> 1) & 1) ^ 1);
+      for (int fill = 0; fill < passes * segments && ok; ++fill) {
+        const int acc = fill & 1;
+        ok = mbar_wait(&tempty[acc], ((fill >> 1) & 1) ^ 1);
         tc_fence_after();
-        for (int s = s0; s < s1 && ok; ++s) {
+        const int first = SEG ? s0 + fill % segments * kSegment : s0;
+        const int stop = SEG ? min(first + kSegment, s1) : s1;
+        for (int s = first; s < stop && ok; ++s) {
           ok = mbar_wait(&full[stage], phase);
           if (!ok) break;
           tc_fence_after();
@@ -283,7 +289,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
           for (int k = 0; k < kBK / 16; ++k)
             tc_mma_f16(tmem + acc * p.mma_n, smem_desc_k_sw128(w + k * 32),
                        smem_desc_k_sw128(w + p.a_bytes + k * 32), idesc,
-                       (s != s0 || k != 0) ? 1u : 0u);
+                       (s != first || k != 0) ? 1u : 0u);
           tc_commit(&empty[stage]);
           if (++stage == p.stages) { stage = 0; phase ^= 1; }
         }
@@ -298,15 +304,16 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
     const int q = warp & 3;
     const int lane_row = q * 32 + lane;
     const int u = lane_row / rows_u, j0 = lane_row - u * rows_u;
-    for (int ps = 0; ps < passes && !*abort_flag; ++ps) {
-      const int acc = ps & 1;
+    for (int fill = 0; fill < passes * segments && !*abort_flag; ++fill) {
+      const int acc = fill & 1, ps = fill / segments;
+      const bool more = fill % segments != 0;  // adds to the segments before
       const int unit = ps * per + u;
       const int j = (unit % blocks_u) * kM + j0;
       const int slot = u < per && unit < units && j < p.rank ? unit / blocks_u : -2;
       uint64_t own = 0;  // the rows that follow this lane's adapter
       for (int i = 0; i < n; ++i)
         if (s_slot[i] == slot) own |= uint64_t{1} << i;
-      if (!mbar_wait(&tfull[acc], (ps >> 1) & 1)) {
+      if (!mbar_wait(&tfull[acc], (fill >> 1) & 1)) {
         atomicExch(&g_shrink_error, kErrTimeoutEpilogue);
         *abort_flag = 1;
         break;
@@ -319,7 +326,10 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
         const unsigned bits = static_cast<unsigned>(own >> c);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (bits & (1u << i)) part[(c + i) * p.rank + j] = s0 < s1 ? v[i] : 0.f;
+          if (bits & (1u << i)) {
+            float& t = part[(c + i) * p.rank + j];
+            t = (more ? t : 0.f) + (s0 < s1 ? v[i] : 0.f);
+          }
       }
       tc_fence_before();
       __syncwarp();
@@ -442,13 +452,18 @@ cudaError_t shrink_tc(const LoraShrink& l, uint16_t* parts, float* row_scale, in
   if (!grouped_map(&mx, l.dtype, l.x, l.K, l.rows, 1, p.chunk) ||
       !grouped_map(&ma, l.dtype, l.a, l.K, l.rank, l.adapters, std::min(l.rank, kM)))
     return cudaErrorInvalidValue;
-  static SmemOptIn opt_in;
-  cudaError_t st = opt_in.set(lora_shrink_tc_kernel<T>, kTcSmemMax);
-  if (st != cudaSuccess) return st;
   const size_t smem =
       1024 + p.stages * p.stage_bytes + kABytes - p.a_bytes + p.chunk * p.rank * 4 + 256;
-  return launch_overlapped(lora_shrink_tc_kernel<T>, static_cast<unsigned>(chunks * p.splits),
-                           kTcThreads, smem, p.splits, s, mx, ma, p);
+  auto launch = [&](auto kernel, SmemOptIn& opt_in) {
+    cudaError_t st = opt_in.set(kernel, kTcSmemMax);
+    if (st != cudaSuccess) return st;
+    return launch_overlapped(kernel, static_cast<unsigned>(chunks * p.splits), kTcThreads, smem,
+                             p.splits, s, mx, ma, p);
+  };
+  static SmemOptIn one, many;
+  return segments_of((slices + p.splits - 1) / p.splits) > 1
+             ? launch(lora_shrink_tc_kernel<T, true>, many)
+             : launch(lora_shrink_tc_kernel<T, false>, one);
 }
 
 }  // namespace

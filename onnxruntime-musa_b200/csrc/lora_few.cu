@@ -8,7 +8,8 @@
 // CTAs split K; the leader receives the others' partial sums of the tile and of t in its
 // shared memory, adds them in rank order, and adds s_a B_a t with FMAs in fp32 -- t is never
 // rounded -- from the B rows that each thread (one output feature) fetched while the weights
-// streamed.
+// streamed.  Sums of more than one segment of slices (kSegment) are added up in the epilogue's
+// registers.
 // Bound: the weights' bytes; A_a adds rows x rank / 128 of them, from L2 after the first tile.
 // Measured: one row, rank 16, [4096, 4096], bf16, 11.8 us on the device (2.9 TB/s).
 #include <algorithm>
@@ -56,7 +57,8 @@ __device__ __forceinline__ void st_async_f1(uint32_t addr, float a, uint32_t bar
       : "memory");
 }
 
-template <typename T>
+// SEG: a CTA may have more than one segment of slices.
+template <typename T, bool SEG>
 __global__ void __launch_bounds__(kThreads, 2)
 lora_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                 const __grid_constant__ CUtensorMap map_a, const FewParams p) {
@@ -70,7 +72,10 @@ lora_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   uint64_t* empty = full + kMaxStages;
   uint64_t* tfull = empty + kMaxStages;
   uint64_t* xfull = tfull + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(xfull + 1);
+  uint64_t* sfull = xfull + 1;   // a segment that is not the last is complete
+  uint64_t* sempty = sfull + 1;  // ... and has been read
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sempty + 1);
+  static_assert((2 * kMaxStages + 4) * 8 + 4 <= 256, "barrier block");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int S = p.splits;
@@ -85,6 +90,8 @@ lora_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     }
     mbar_init(tfull, 1);
     mbar_init(xfull, 1);
+    mbar_init(sfull, 1);
+    mbar_init(sempty, 4);
     fence_mbarrier_init();
     tma_prefetch_desc(&map_w);
     tma_prefetch_desc(&map_x);
@@ -133,10 +140,16 @@ lora_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   } else if (warp == 1) {
     if (lane == 0) {
       const uint32_t idesc = idesc_f16(TcFormat<T>::kId, kTileM, 16);
-      int stage = 0;
-      uint32_t phase = 0;
+      int stage = 0, left = kSegment;  // slices until the segment is complete
+      uint32_t phase = 0, seg = 0;
       for (int s = split; s < slices; s += S) {
-        if (!mbar_wait(&full[stage], phase)) {
+        bool ok = true;
+        if (SEG && left == 0) {
+          tc_commit(sfull);
+          ok = mbar_wait(sempty, seg++ & 1);
+          left = kSegment;
+        }
+        if (!ok || !mbar_wait(&full[stage], phase)) {
           atomicExch(&g_few_error, kErrTimeoutMma);
           break;
         }
@@ -145,11 +158,12 @@ lora_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         const uint32_t x = w + kWBytes + p.a_bytes;
 #pragma unroll
         for (int k = 0; k < kBK / 16; ++k) {
-          const uint32_t more = (s != split || k != 0) ? 1u : 0u;
+          const uint32_t more = (left != kSegment || k != 0) ? 1u : 0u;
           tc_mma_f16(tmem, smem_desc_k_sw128(w + k * 32), smem_desc_k_sw128(x + k * 32), idesc, more);
           tc_mma_f16(tmem + 16, smem_desc_k_sw128(w + kWBytes + k * 32),
                      smem_desc_k_sw128(x + k * 32), idesc, more);
         }
+        --left;
         tc_commit(&empty[stage]);
         if (++stage == p.stages) { stage = 0; phase ^= 1; }
       }
@@ -175,21 +189,42 @@ lora_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       if (j == p.rank) { j = 0; row = min(row + 1, 31); }
     }
   }
-  const bool ok = mbar_wait(tfull, 0);
-  if (!ok) atomicExch(&g_few_error, kErrTimeoutEpilogue);
-  tc_fence_after();
-  if (S > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16);
+  const int row = me / p.rank;  // the row whose A entry this thread's is, and so its column
   float v[16], part_t = 0.f;
-  if (epi) {
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16);
+  auto fetch = [&] {
     float tv[16];
     tmem_ld16(lanes, v);
     tmem_ld16(lanes + 16, tv);
     tmem_ld_wait();
-    const int row = me / p.rank;  // the row whose A entry this is, and so its column
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (row == i) part_t = tv[i];
+  };
+  const int segments = SEG ? segments_of((slices - split + S - 1) / S) : 1;
+  float sum[8] = {}, sum_t = 0.f;
+  for (int seg = 0; epi && seg < segments - 1; ++seg) {
+    if (!mbar_wait(sfull, seg & 1)) break;  // (tfull will not complete either)
+    tc_fence_after();
+    fetch();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] += v[i];
+    sum_t += part_t;
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(sempty);
+  }
+  const bool ok = mbar_wait(tfull, 0);
+  if (!ok) atomicExch(&g_few_error, kErrTimeoutEpilogue);
+  tc_fence_after();
+  if (S > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (epi) {
+    fetch();
+    if (segments > 1) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += sum[i];
+      part_t += sum_t;
+    }
     if (split >= slices || !ok) {  // nothing accumulated
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = 0.f;
@@ -278,11 +313,15 @@ cudaError_t launch_few(const GroupedArgs& g, const LoraShrink& l, const void* b,
       !grouped_map(&mx, g.dtype, g.x, g.K, g.rows, 1, kXRows) ||
       !grouped_map(&ma, g.dtype, l.a, g.K, l.rank, l.adapters, l.rank))
     return cudaErrorInvalidValue;
-  static SmemOptIn opt_in;
-  cudaError_t st = opt_in.set(lora_few_kernel<T>, 113 * 1024);
-  if (st != cudaSuccess) return st;
-  return launch_overlapped(lora_few_kernel<T>, static_cast<unsigned>(tiles * p.splits), kThreads,
-                           fixed + p.stages * p.stage_bytes, p.splits, s, mw, mx, ma, p);
+  auto launch = [&](auto kernel, SmemOptIn& opt_in) {
+    cudaError_t st = opt_in.set(kernel, 113 * 1024);
+    if (st != cudaSuccess) return st;
+    return launch_overlapped(kernel, static_cast<unsigned>(tiles * p.splits), kThreads,
+                             fixed + p.stages * p.stage_bytes, p.splits, s, mw, mx, ma, p);
+  };
+  static SmemOptIn one, many;
+  return segments_of((slices + p.splits - 1) / p.splits) > 1 ? launch(lora_few_kernel<T, true>, many)
+                                                             : launch(lora_few_kernel<T, false>, one);
 }
 
 }  // namespace
