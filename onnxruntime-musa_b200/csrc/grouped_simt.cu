@@ -4,9 +4,11 @@
 // the operands to 11 bits, 2^13 times the rounding of an fp32 result).
 //
 // Mathematics: one tile C[m, n] = sum_c A(m, c) B(n, c) per CTA, summed in ascending c in
-// fp32, kFold entries at a time and then those sums: one running sum rounds at the magnitude it
-// has reached, and a grad_input over 10696 entries was off from float64 by 1.3e-6, relative,
-// where a blocked product is off by 4.7e-7 and this one now by 4.1e-7.  (Price: 735 -> 800 us
+// fp32, kFold entries at a time and then those sums, each of whose roundings starts the next kFold:
+// one running sum rounds at the magnitude it has reached, and a grad_input over 10696 entries was
+// off from float64 by 1.3e-6, relative, where a blocked product is off by 4.7e-7 and this one now
+// by 4.1e-7; grad_weight of 2^25 equal rows was off by 1.7e-4 before the roundings were kept, and
+// the number of rows shows in the result no more.  (Price: 735 -> 783 us
 // for 4096 rows, 8 experts of [2048, 2048] fp32.  Four other placements of the folds -- shared
 // memory, the end of the slice loop, its prologue again for each fold -- took 790 to 890.)
 // The three directions differ only in where the contraction index lies:
@@ -278,9 +280,13 @@ grouped_simt_kernel(const SimtParams p) {
       for (int j = 0; j < TN; j += 4)
         op(folds[i * (TN / 4) + j / 4], acc2[i][j / 2], acc2[i][j / 2 + 1]);
   };
-  auto add_fold = [](const float4& f, uint64_t& u, uint64_t& v) {
-    u = fma2(pair2(1.f, 1.f), u, pair2(f.x, f.y));
-    v = fma2(pair2(1.f, 1.f), v, pair2(f.z, f.w));
+  // The sum of the folds `f` and the next one.  `more` follow: that sum waits and its rounding
+  // error, exact by a two-sum, is what the next fold starts from (none beside an infinity).
+  auto add_fold = [](float& f, float& a, bool more) {
+    const float t = __fadd_rn(f, a), u = __fsub_rn(t, f);
+    const float e = __fadd_rn(__fsub_rn(f, __fsub_rn(t, u)), __fsub_rn(a, u));
+    f = t;
+    a = !more ? t : isfinite(t) ? e : 0.f;
   };
 #pragma unroll 1
   for (int s = from; s < slices;) {
@@ -323,13 +329,26 @@ grouped_simt_kernel(const SimtParams p) {
       }
       __syncthreads();
     }
-    if (first > from) each_fold(add_fold);
-    if (stop < slices)
+    const bool more = stop < slices;
+    if (first > from) {
+      each_fold([&](float4& f, uint64_t& u, uint64_t& v) {
+        float a, b, c, d;
+        unpair2(u, a, b);
+        unpair2(v, c, d);
+        add_fold(f.x, a, more);
+        add_fold(f.y, b, more);
+        add_fold(f.z, c, more);
+        add_fold(f.w, d, more);
+        u = pair2(a, b);
+        v = pair2(c, d);
+      });
+    } else if (more) {
       each_fold([](float4& f, uint64_t& u, uint64_t& v) {
         unpair2(u, f.x, f.y);
         unpair2(v, f.z, f.w);
         u = v = 0;
       });
+    }
   }
 
   float acc[TM][TN];
@@ -473,9 +492,11 @@ grouped_simt_kernel(const SimtParams p) {
 // takes kGemvCols output features and up to kGemvRows rows of the group at a time; its lanes
 // stride over the contraction, four entries each, and meet in a butterfly sum.  Bound: the
 // weights' bytes (a 64-row tile of the kernel above would multiply 64 rows whatever the group
-// has: 97 us for one row of [4096, 4096] fp32).
+// has: 97 us for one row of [4096, 4096] fp32).  A lane sums kFold entries at a time, as the tiles
+// do: 32768 equal ones in one sum were off by 3e-4.
 constexpr int kGemvRows = 8;
 constexpr int kGemvCols = 2;
+constexpr int kLaneFold = 32 * kFold;  // contraction entries of 32 lanes' running sums
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
@@ -490,27 +511,47 @@ grouped_gemv_kernel(const SimtParams p) {
   const T* x = static_cast<const T*>(p.a);
   for (int r0 = begin; r0 < end; r0 += kGemvRows) {
     const int nr = min(kGemvRows, end - r0);
-    float acc[kGemvCols][kGemvRows] = {};
+    float acc[kGemvCols][kGemvRows] = {}, folds[kGemvCols][kGemvRows] = {};
     const T* xr = x + static_cast<int64_t>(r0) * K;
-#pragma unroll 4
-    for (int c = lane * 4; c < K; c += 128) {
-      float4 w[kGemvCols];
+    auto take_fold = [&] {
 #pragma unroll
       for (int j = 0; j < kGemvCols; ++j)
-        w[j] = n0 + j < p.N ? load4<T>(w0 + static_cast<int64_t>(j) * K + c, K - c, p.b_vec)
-                            : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < kGemvRows; ++i) {
-        if (i >= nr) break;
-        const float4 v = load4<T>(xr + static_cast<int64_t>(i) * K + c, K - c, p.a_vec);
+        for (int i = 0; i < kGemvRows; ++i) {
+          folds[j][i] += acc[j][i];
+          acc[j][i] = 0.f;
+        }
+    };
+    for (int c0 = 0; c0 < K; c0 += kLaneFold) {
+      const int c1 = min(c0 + kLaneFold, K);
+      if (c0 > 0) take_fold();
+#pragma unroll 4
+      for (int c = c0 + lane * 4; c < c1; c += 128) {
+        float4 w[kGemvCols];
 #pragma unroll
-        for (int j = 0; j < kGemvCols; ++j) {
-          acc[j][i] = fmaf(w[j].x, v.x, acc[j][i]);
-          acc[j][i] = fmaf(w[j].y, v.y, acc[j][i]);
-          acc[j][i] = fmaf(w[j].z, v.z, acc[j][i]);
-          acc[j][i] = fmaf(w[j].w, v.w, acc[j][i]);
+        for (int j = 0; j < kGemvCols; ++j)
+          w[j] = n0 + j < p.N ? load4<T>(w0 + static_cast<int64_t>(j) * K + c, K - c, p.b_vec)
+                              : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < kGemvRows; ++i) {
+          if (i >= nr) break;
+          const float4 v = load4<T>(xr + static_cast<int64_t>(i) * K + c, K - c, p.a_vec);
+#pragma unroll
+          for (int j = 0; j < kGemvCols; ++j) {
+            acc[j][i] = fmaf(w[j].x, v.x, acc[j][i]);
+            acc[j][i] = fmaf(w[j].y, v.y, acc[j][i]);
+            acc[j][i] = fmaf(w[j].z, v.z, acc[j][i]);
+            acc[j][i] = fmaf(w[j].w, v.w, acc[j][i]);
+          }
         }
       }
+    }
+    if (K > kLaneFold) {
+      take_fold();
+#pragma unroll
+      for (int j = 0; j < kGemvCols; ++j)
+#pragma unroll
+        for (int i = 0; i < kGemvRows; ++i) acc[j][i] = folds[j][i];
     }
     if (p.lora.t != nullptr) {  // y += B_a t, the lanes striding over the rank
       const int r = p.lora.rank;

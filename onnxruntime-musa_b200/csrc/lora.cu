@@ -29,6 +29,7 @@ constexpr int kWarps = 8;
 // each, the lanes striding over K.  One pass over an A row serves all rows that follow its
 // adapter (rows of a prompt; A_a is what is read most).
 constexpr int kRows = 4;
+constexpr int kLaneFold = 32 * 512;  // contraction entries of 32 lanes' running sums
 
 template <typename T>
 __device__ __forceinline__ void load_vec(const T* p, int n, bool vec, float (&v)[4]) {
@@ -73,18 +74,32 @@ lora_shrink_simt_kernel(const T* __restrict__ x, const T* __restrict__ a,
     for (int i = 0; i < f; ++i) lead = lead && ad[i] != ad[f];
     if (!lead) continue;
     const T* ar = a + (static_cast<int64_t>(ad[f]) * rank + j) * K;
-    float sum[kRows] = {};
+    float sum[kRows] = {}, folds[kRows] = {};
+    for (int c0 = 0; c0 < K; c0 += kLaneFold) {
+      const int c1 = min(c0 + kLaneFold, K);
 #pragma unroll 8
-    for (int k = lane * 4; k < K; k += 128) {
-      float w[4], v[4];
-      load_vec(ar + k, K - k, vec, w);
+      for (int k = c0 + lane * 4; k < c1; k += 128) {
+        float w[4], v[4];
+        load_vec(ar + k, K - k, vec, w);
 #pragma unroll
-      for (int i = f; i < kRows; ++i) {
-        if (ad[i] != ad[f]) continue;
-        load_vec(x + (row0 + i) * K + k, K - k, vec, v);
+        for (int i = f; i < kRows; ++i) {
+          if (ad[i] != ad[f]) continue;
+          load_vec(x + (row0 + i) * K + k, K - k, vec, v);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) sum[i] = fmaf(w[q], v[q], sum[i]);
+          for (int q = 0; q < 4; ++q) sum[i] = fmaf(w[q], v[q], sum[i]);
+        }
       }
+      if (K > kLaneFold) {  // sums of 512 entries, then a sum of those
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          folds[i] += sum[i];
+          sum[i] = 0.f;
+        }
+      }
+    }
+    if (K > kLaneFold) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) sum[i] = folds[i];
     }
 #pragma unroll
     for (int i = f; i < kRows; ++i) {

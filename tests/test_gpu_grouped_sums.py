@@ -5,6 +5,10 @@ One MMA step adds sixteen products to the running fp32 sum and loses at most two
 in the last place (the products are aligned to the sum and cut off), 2^-22 of it.  An accumulator
 takes at most 16384 entries, 1024 steps, before it is added to a sum of its own: 2^-12 of the
 magnitudes, whatever the length, and half a step of the output type.
+
+FFMA kernels (float32).  512 products per running sum lose half a step each; the sums of those
+sums lose at most 64 more on their way (2^20 entries over 32 lanes) or, in the tiles, carry their
+rounding errors along; then up to five additions across lanes and four across a cluster.
 """
 
 import numpy as np
@@ -16,6 +20,7 @@ from test_gpu_grouped import FLOOR, HALF_STEP
 pytestmark = pytest.mark.gpu
 
 SEGMENT = 2.0 ** -12
+FFMA = (512 + 64 + 5 + 4) * 2.0 ** -24
 
 
 def positive(dev, shape, scale, dtype_name, seed):
@@ -139,3 +144,35 @@ def test_long_adapter_sums(pkg, dev, dtype_name, T, N, K, r, kind):
         exact[rows] += float(d["scales"][a]) * (t @ d["lora_b"][a].double().t())
     # t's own sum, its two 16-bit parts (2^-15) and the sum over the rank.
     assert_sums(y, exact, dtype_name, SEGMENT + 2.0 ** -15 + (r + 6) * 2.0 ** -23)
+
+
+LONG = 1 << 20
+
+
+@pytest.mark.parametrize("c", [1 + 2.0 ** -13 - 2.0 ** -16, np.float32(1.3)])
+def test_fp32_lanes(pkg, dev, c):
+    """A row or two per group: the lanes stride over the contraction, 32768 products each.  (One
+    running sum of equal products is off by 1e-4 and 3e-4.)"""
+    import torch
+    exact = torch.tensor(float(c) * LONG, device=dev, dtype=torch.float64)
+    for E, rows in ((1, 4), (2, 6)):
+        off = offsets(dev, [rows // E] * E)
+        x, w = torch.ones(rows, LONG, device=dev), torch.full((E, 24, LONG), float(c), device=dev)
+        assert_sums(pkg.grouped_matmul(x, w, off), exact.expand(rows, 24), "float32", FFMA)
+    # The adapter's own product, A x, seen through B = 1 beside a projection of zeros.
+    for T in (4, 70):
+        y = pkg.lora_matmul(torch.ones(T, LONG, device=dev), torch.zeros(5, LONG, device=dev),
+                            torch.full((1, 3, LONG), float(c), device=dev),
+                            torch.ones(1, 5, 3, device=dev) / 4,
+                            torch.zeros(T, dtype=torch.int32, device=dev), torch.ones(1, device=dev))
+        assert_sums(y, (0.75 * exact).expand(T, 5), "float32", FFMA + 5 * 2.0 ** -24)
+
+
+def test_fp32_grad_weight_of_many_rows(pkg, dev):
+    """33 M rows in one expert.  (Sums of 512 and one running sum of those: off by 1.1e-4.)"""
+    import torch
+    rows, c = 1 << 25, 1 + 2.0 ** -12 - 2.0 ** -16
+    x, dy = torch.full((rows, 1), c, device=dev), torch.ones(rows, 1, device=dev)
+    dw = pkg.grouped_matmul_grad_weight(x, dy, offsets(dev, [rows]))
+    exact = torch.full((1, 1, 1), c * rows, device=dev, dtype=torch.float64)
+    assert_sums(dw, exact, "float32", FFMA)
