@@ -427,6 +427,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
           if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
         if (LORA > 0 && ok) {
+          // What the rows follow comes from the launch before, which may take longer than any
+          // wait on a barrier: that launch is waited for first.
+          if (i == 0) pdl_wait();
           ok = mbar_wait(&cfull[i & 1], (i >> 1) & 1);
           RunWalk w(codes + (i & 1) * 16, (t.n + 15) / 16);
           while (ok && w.next()) {
