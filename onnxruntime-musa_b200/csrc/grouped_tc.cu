@@ -399,6 +399,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
           if (SEG && b != 0 && b % kSegment == 0) {  // a segment is complete: the epilogue takes it
             tc_commit_pair(&tfull[acc], 0x3);
             fills ^= 1u << acc;
+            if (LORA > 0 && i == 0) pdl_wait();  // the epilogue does
             ok = drained(acc);
             tc_fence_after();
           }
@@ -428,7 +429,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
         }
         if (LORA > 0 && ok) {
           // What the rows follow comes from the launch before, which may take longer than any
-          // wait on a barrier: that launch is waited for first.
+          // wait on a barrier counts: that launch is waited for first.
           if (i == 0) pdl_wait();
           ok = mbar_wait(&cfull[i & 1], (i >> 1) & 1);
           RunWalk w(codes + (i & 1) * 16, (t.n + 15) / 16);
