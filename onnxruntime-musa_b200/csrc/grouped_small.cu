@@ -192,6 +192,7 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
     const uint32_t idesc = idesc_f16(TcFormat<T>::kId, kTileM, nt) | (kAMn ? kIdescAMn : 0);
     int stage = 0, left = kSegment;  // slices until the segment is complete
     uint32_t phase = 0, seg = 0;
+    bool gave_up = false;
     for (int s = s0; s < s1; s += ds) {
       bool ok = true;
       if (SEG && left == 0) {
@@ -203,6 +204,7 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
       if (!ok || !mbar_wait(&full[stage], phase)) {
         atomicExch(&g_small_error, kErrTimeoutMma);
         *abort_flag = 1;
+        gave_up = true;
         break;
       }
       tc_fence_after();
@@ -219,6 +221,7 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
       if (++stage == p.stages) { stage = 0; phase ^= 1; }
     }
     tc_commit(tfull);
+    if (gave_up) drain_ring(full, p.stages, stage, phase);
   }
   __syncwarp();
 
@@ -292,7 +295,7 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
   }
 
   for (int seg = 0; epi && seg < segments - 1; ++seg) {
-    if (!mbar_wait(sfull, seg & 1)) break;  // (tfull will not complete either)
+    if (!warp_wait(sfull, seg & 1)) break;  // (tfull will not complete either)
     tc_fence_after();
     // Each warp adds what it will send or finish below.
     auto add = [&](int b, bool first) {
@@ -317,7 +320,7 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
     if (lane == 0) mbar_arrive(sempty);
   }
 
-  const bool ok = mbar_wait(tfull, 0);
+  const bool ok = warp_wait(tfull, 0);
   if (!ok) {
     atomicExch(&g_small_error, kErrTimeoutEpilogue);
     *abort_flag = 1;
@@ -356,7 +359,7 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
         st_async_f4(mapa_shared(dst, owner), lo, bar);
         st_async_f4(mapa_shared(dst + 512, owner), hi, bar);
       }
-    if (owned > 0 && !mbar_wait_cluster(xfull, 0)) atomicExch(&g_small_error, kErrTimeoutEpilogue);
+    if (owned > 0 && !wait_parts(xfull)) atomicExch(&g_small_error, kErrTimeoutEpilogue);
   }
 
   uint8_t* buf = stage_out + (warp & 7) * kEpiBytes;

@@ -379,9 +379,11 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
       uint32_t fills = 0;   // bit a: parity of accumulator a's next fill
       bool both = false;    // the tile before has its sum in the other accumulator
       auto drained = [&](int a) { return mbar_wait(&tempty[a], (fills >> a & 1) ^ 1); };
+      bool complete = false;
       for (int i = 0;; ++i) {
         const int L = turn_tile(i, pair, npairs);
-        if (L >= total || *abort_flag) break;
+        complete = L >= total;
+        if (complete || *abort_flag) break;
         const PairTile t = pair_tile<DIR>(L, table, p);
         const uint32_t idesc = idesc_f16(TcFormat<T>::kId, kTileM, t.nt) |
                                (kAMn ? kIdescAMn : 0) | (kBMn ? kIdescBMn : 0);
@@ -464,15 +466,17 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
       }
       tc_commit_pair(done, 0x1);
       mbar_wait(done, 0);
+      // (Copies into either CTA count on these barriers.)
+      if (!complete) drain_ring(full, kStages, stage, phase);
     }
   } else if (LORA > 0 && warp == 2 + kEpiWarps) {
     // ------------------------------------- what the tile's rows follow (both CTAs)
     pdl_wait();
     for (int i = 0;; ++i) {
       const int L = turn_tile(i, pair, npairs);
-      if (L >= total || *abort_flag) break;
+      if (L >= total || warp_stopped(abort_flag)) break;
       const PairTile t = pair_tile<DIR>(L, table, p);
-      if (!mbar_wait(&cempty[i & 1], ((i >> 1) & 1) ^ 1)) {
+      if (!warp_wait(&cempty[i & 1], ((i >> 1) & 1) ^ 1)) {
         atomicExch(&g_pair_error, kErrTimeoutProducer);
         *abort_flag = 1;
         break;
@@ -506,7 +510,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
     uint32_t fills = 0;  // as the MMA warp's
     for (int i = 0;; ++i) {
       const int L = turn_tile(i, pair, npairs);
-      if (L >= total || *abort_flag) break;
+      if (L >= total || warp_stopped(abort_flag)) break;
       const PairTile t = pair_tile<DIR>(L, table, p);
       const int acc = i & 1, segments = SEG ? segments_of(t.blocks) : 1;
       const uint32_t taddr =
@@ -514,7 +518,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
       const uint32_t tsum = taddr + (acc ? -kTileN : kTileN);  // sum of the segments before
       bool ok = true;
       for (int seg = 0; ok && seg < segments; ++seg) {
-        ok = mbar_wait(&tfull[acc], fills >> acc & 1);
+        ok = warp_wait(&tfull[acc], fills >> acc & 1);
         fills ^= 1u << acc;
         tc_fence_after();
         if (!ok || segments == 1) break;
@@ -586,7 +590,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
       };
       if constexpr (LORA > 0) {
         LoraFrags<LORA> frags;  // of this tile's features
-        if (!mbar_wait(&cfull[i & 1], (i >> 1) & 1)) {
+        if (!warp_wait(&cfull[i & 1], (i >> 1) & 1)) {
           atomicExch(&g_pair_error, kErrTimeoutEpilogue);
           *abort_flag = 1;
           break;

@@ -95,6 +95,33 @@ __device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t saddr, uint32_t 
 constexpr uint32_t kIdescAMn = 1u << 15;
 constexpr uint32_t kIdescBMn = 1u << 16;
 
+// mbar_wait() by a whole warp: its lanes leave together, whichever of them ran out of time, so
+// that what the warp does next as one (tensor memory loads, shuffles) stays whole.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+__device__ __forceinline__ bool warp_stopped(volatile int* abort_flag) {
+  return __any_sync(0xffffffffu, *abort_flag);
+}
+
+// Before a CTA that gave up leaves: waits for the copies that may still be under way into its
+// ring, in the order of the stages from the one that was waited for.  (A stage that was never
+// asked for runs out of time too and ends this.)
+__device__ __forceinline__ void drain_ring(uint64_t* full, int stages, int stage, uint32_t phase) {
+  for (int k = 0; k < stages; ++k) {
+    if (!mbar_wait(&full[stage], phase)) return;
+    if (++stage == stages) { stage = 0; phase ^= 1; }
+  }
+}
+
+// Parts from the other CTAs of a cluster, which send theirs (zeros) after a wait of their own ran
+// out, too: this wait is four times as long, so that nobody's parts arrive after its CTA has left.
+__device__ __forceinline__ bool wait_parts(uint64_t* bar) {
+  for (int k = 0; k < 4; ++k)
+    if (mbar_wait_cluster(bar, 0)) return true;
+  return false;
+}
+
 // Rows [x, y) of each group and the prefix of its tile counts, in shared memory.
 struct GroupTable {
   int2* rows;   // [E]

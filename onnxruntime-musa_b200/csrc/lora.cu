@@ -313,13 +313,14 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
       if (!ok) {
         atomicExch(&g_shrink_error, kErrTimeoutMma);
         *abort_flag = 1;
+        drain_ring(full, p.stages, stage, phase);
       }
     }
   } else {
     const int q = warp & 3;
     const int lane_row = q * 32 + lane;
     const int u = lane_row / rows_u, j0 = lane_row - u * rows_u;
-    for (int fill = 0; fill < passes * segments && !*abort_flag; ++fill) {
+    for (int fill = 0; fill < passes * segments && !warp_stopped(abort_flag); ++fill) {
       const int acc = fill & 1, ps = fill / segments;
       const bool more = fill % segments != 0;  // adds to the segments before
       const int unit = ps * per + u;
@@ -328,7 +329,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
       uint64_t own = 0;  // the rows that follow this lane's adapter
       for (int i = 0; i < n; ++i)
         if (s_slot[i] == slot) own |= uint64_t{1} << i;
-      if (!mbar_wait(&tfull[acc], (fill >> 1) & 1)) {
+      if (!warp_wait(&tfull[acc], (fill >> 1) & 1)) {
         atomicExch(&g_shrink_error, kErrTimeoutEpilogue);
         *abort_flag = 1;
         break;

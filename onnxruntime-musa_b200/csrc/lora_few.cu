@@ -142,6 +142,7 @@ lora_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       const uint32_t idesc = idesc_f16(TcFormat<T>::kId, kTileM, 16);
       int stage = 0, left = kSegment;  // slices until the segment is complete
       uint32_t phase = 0, seg = 0;
+      bool gave_up = false;
       for (int s = split; s < slices; s += S) {
         bool ok = true;
         if (SEG && left == 0) {
@@ -151,6 +152,7 @@ lora_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         }
         if (!ok || !mbar_wait(&full[stage], phase)) {
           atomicExch(&g_few_error, kErrTimeoutMma);
+          gave_up = true;
           break;
         }
         tc_fence_after();
@@ -168,6 +170,7 @@ lora_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         if (++stage == p.stages) { stage = 0; phase ^= 1; }
       }
       tc_commit(tfull);
+      if (gave_up) drain_ring(full, p.stages, stage, phase);
     }
   }
   __syncwarp();
@@ -204,7 +207,7 @@ lora_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   const int segments = SEG ? segments_of((slices - split + S - 1) / S) : 1;
   float sum[8] = {}, sum_t = 0.f;
   for (int seg = 0; epi && seg < segments - 1; ++seg) {
-    if (!mbar_wait(sfull, seg & 1)) break;  // (tfull will not complete either)
+    if (!warp_wait(sfull, seg & 1)) break;  // (tfull will not complete either)
     tc_fence_after();
     fetch();
 #pragma unroll
@@ -214,7 +217,7 @@ lora_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     __syncwarp();
     if (lane == 0) mbar_arrive(sempty);
   }
-  const bool ok = mbar_wait(tfull, 0);
+  const bool ok = warp_wait(tfull, 0);
   if (!ok) atomicExch(&g_few_error, kErrTimeoutEpilogue);
   tc_fence_after();
   if (S > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -239,7 +242,7 @@ lora_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     }
   }
   if (split == 0 && epi) {
-    if (S > 1 && !mbar_wait_cluster(xfull, 0)) atomicExch(&g_few_error, kErrTimeoutEpilogue);
+    if (S > 1 && !wait_parts(xfull)) atomicExch(&g_few_error, kErrTimeoutEpilogue);
     for (int r = 1; r < S; ++r) {  // the parts in rank order
       const uint8_t* src = parts + (r - 1) * part_bytes(p.quads);
       const float4 a = *reinterpret_cast<const float4*>(src + me * 16);
