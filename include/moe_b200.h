@@ -323,10 +323,18 @@ int moe_b200_norm_router(int32_t dtype, int64_t num_rows, int64_t hidden_size,
  * bfloat16 throughout, sums in fp32.  1 <= n, k <= 2^20; E <= 256.  Buffers need the
  * alignment of their elements; 16-bit types with n and k multiples of 8 and 16-byte
  * aligned buffers run on the tensor cores.  Outputs and workspaces that overlap another buffer of the
- * call are refused.  No host synchronisation, no allocation; results are the same bits on every call.
+ * call are refused.  No host synchronisation, no allocation behind the first call (a few pinned words);
+ * results are the same bits on every call.
+ * Every wait in the kernels is bounded (2 s of wall time).  A call whose wait ran out leaves its output
+ * incomplete; the next of these calls on the device returns EP_FAIL and does nothing else, or
+ * moe_b200_take_device_error gives the code once the stream is synchronised.  With
+ * MOE_B200_TRACE_SYNC set every call waits for itself and returns its own error.
  * Analog of the reference's batched product (musa/ep/src/kernels/math/matmul.cc:239-332,
  * shared_inc/blas_utils.h:237-262), which takes equal sizes only. */
 
+/* Error code of a call of this section on the current device whose wait ran out, 0 for none; reads
+ * and clears it. */
+int moe_b200_take_device_error(int32_t* code);
 /* y[p] = weights[e] x[p]:  x [num_rows, k], y [num_rows, n]. */
 int moe_b200_grouped_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
                             int64_t num_experts, const void* x, const void* weights,

@@ -154,6 +154,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "moe_b200_route_noalloc": (ctypes.c_int, [_VP, _I32, _I64, _I64, _I32, _I32, _VP, _VP, _VP]),
     "moe_b200_permute_workspace_size": (_SZ, [_I64, _I32, _I64]),
     "moe_b200_permute": (ctypes.c_int, [_VP, _I64, _I32, _I64, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "moe_b200_take_device_error": (ctypes.c_int, [_PI32]),
     "moe_b200_grouped_matmul": (ctypes.c_int, [_I32, _I64, _I64, _I64, _I64, _VP, _VP, _VP, _VP,
                                                _VP]),
     "moe_b200_grouped_matmul_grad_input": (ctypes.c_int, [_I32, _I64, _I64, _I64, _I64, _VP, _VP,
@@ -766,6 +767,15 @@ def permute(expert_idx, num_experts: int, stream=None):
 
 
 # ------------------------------------------------------- expert products, adapters
+
+def take_device_error() -> int:
+    """Error code of an expert product or adapter projection on the current device that gave up
+    waiting and left its output incomplete, 0 for none; reads and clears it.  (Synchronise the
+    stream first.  The next such call raises :class:`EPFail` for it otherwise.)"""
+    code = ctypes.c_int32(0)
+    check(lib().moe_b200_take_device_error(ctypes.byref(code)))
+    return code.value
+
 
 # The checks below run on every call of operators that take a few microseconds on the GPU,
 # so the usual case is one chained comparison per tensor and the messages are composed only

@@ -25,6 +25,8 @@ struct GroupedArgs {
   const int32_t* offsets;  // [E + 1]; nullptr: one group of all rows (E = 1)
   void* out;
   void* workspace = nullptr;  // grad_weight on tensor cores: padded row tails
+  int* error = nullptr;       // where the tensor-core kernels report a wait that ran out
+  int test_stall = 0;         // test hook: their producers issue no loads
 };
 
 // The adapter term of lora_matmul, added to the forward product of one group.
@@ -60,6 +62,8 @@ struct LoraShrink {
   const void* a;           // [L, r, K]
   const int32_t* ids;
   const float* scales;     // [L]
+  int* error;              // as GroupedArgs
+  int test_stall;
 };
 // Any type and alignment: s_a t in fp32, [rows][rank].
 cudaError_t launch_lora_shrink_simt(const LoraShrink& l, float* t, cudaStream_t s);
@@ -79,11 +83,6 @@ cudaError_t launch_grouped_pair(const GroupedArgs& g, const LoraTerm* lora, int 
                                 cudaStream_t s);
 cudaError_t launch_grouped_small(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
                                  cudaStream_t s);
-// Error words of the tensor-core kernels on the current device (each synchronises), cleared.
-cudaError_t take_grouped_pair_error(int* err);
-cudaError_t take_grouped_small_error(int* err);
-cudaError_t take_lora_error(int* err);
-cudaError_t take_lora_few_error(int* err);
 
 // The whole adapter projection of a few rows in one launch (same types, sizes and alignment as
 // the two launches; b: lora_b).

@@ -3,7 +3,9 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdlib>
+#include <cstring>
 #include <initializer_list>
+#include <mutex>
 
 #include "../../include/moe_b200.h"
 #include "grouped.h"
@@ -84,21 +86,88 @@ int sm_count() {
   return n;
 }
 
-// With MOE_B200_TRACE_SYNC set: wait for the call and report a device-side timeout.
-int finish(const char* what, cudaStream_t s) {
-  const char* v = std::getenv("MOE_B200_TRACE_SYNC");
-  if (v == nullptr || *v == '\0' || *v == '0') return MOE_B200_OK;
-  int rc = cuda_status(cudaStreamSynchronize(s), what);
-  if (rc != MOE_B200_OK) return rc;
-  for (auto take : {moe::take_grouped_pair_error, moe::take_grouped_small_error,
-                    moe::take_lora_error, moe::take_lora_few_error}) {
-    int err = 0;
-    rc = cuda_status(take(&err), what);
-    if (rc == MOE_B200_OK && err != 0)
-      rc = set_error(MOE_B200_EP_FAIL, "%s: device error code %d", what, err);
-    if (rc != MOE_B200_OK) return rc;
+bool env_flag(const char* name) {
+  const char* v = std::getenv(name);
+  return v != nullptr && v[0] != '\0' && std::strcmp(v, "0") != 0;
+}
+
+// Words of pinned host memory in which kernels report a wait that ran out: one for every device,
+// which the next call on it looks at (and moe_b200_take_device_error), and some that traced calls
+// take in turn, so that each finds its own error.  Allocated once, for the life of the process
+// (a captured graph keeps the address); nullptr if that fails.
+constexpr int kDevices = 64, kTracedCalls = 64;
+std::atomic<int*> g_error_words{nullptr};
+
+int* error_words() {
+  int* words = g_error_words.load(std::memory_order_acquire);
+  if (words != nullptr) return words;
+  static std::mutex mutex;
+  std::lock_guard<std::mutex> lock(mutex);
+  words = g_error_words.load(std::memory_order_acquire);
+  if (words != nullptr) return words;
+  // The first call may be captured: allocating is no work on a stream, so it may be done then.
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+  void* at = nullptr;
+  const cudaError_t st = cudaHostAlloc(&at, (kDevices + kTracedCalls) * sizeof(int),
+                                       cudaHostAllocPortable | cudaHostAllocMapped);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (st != cudaSuccess) return nullptr;
+  words = static_cast<int*>(at);
+  std::fill(words, words + kDevices + kTracedCalls, 0);
+  g_error_words.store(words, std::memory_order_release);
+  return words;
+}
+
+int* device_word(int* words) {
+  int dev = 0;
+  return words + (cudaGetDevice(&dev) == cudaSuccess && dev > 0 ? dev % kDevices : 0);
+}
+
+// Reads and clears a word; the store of a kernel may come at any time.
+int take_word(int* word) {
+  return *static_cast<volatile int*>(word) == 0 ? 0 : __atomic_exchange_n(word, 0, __ATOMIC_ACQ_REL);
+}
+
+struct Call {
+  int* error;   // the kernels' word
+  bool traced;  // MOE_B200_TRACE_SYNC: wait for the call and report its own error
+  int stall;    // MOE_B200_TEST_STALL: the tensor-core kernels' producers issue no loads
+};
+
+// In front of a call's launches.  An earlier call whose wait ran out has left its output
+// incomplete and nobody has been told: this one reports it and does nothing.
+int begin(const char* what, Call* c) {
+  int* words = error_words();
+  if (words == nullptr)
+    return set_error(MOE_B200_EP_FAIL, "%s: no pinned host memory for the error words", what);
+  c->error = device_word(words);
+  const int err = take_word(c->error);
+  if (err != 0)
+    return set_error(MOE_B200_EP_FAIL,
+                     "%s: an earlier expert product or adapter projection on this device gave up "
+                     "waiting and its output is incomplete (device error code %d); this call was "
+                     "not made", what, err);
+  c->stall = env_flag("MOE_B200_TEST_STALL") ? 1 : 0;
+  c->traced = env_flag("MOE_B200_TRACE_SYNC");
+  if (c->traced) {
+    static std::atomic<unsigned> turn{0};
+    c->error = words + kDevices + turn.fetch_add(1, std::memory_order_relaxed) % kTracedCalls;
+    take_word(c->error);
   }
   return MOE_B200_OK;
+}
+
+// Behind them.  (A captured call has not run yet: there is nothing to wait for.)
+int finish(const char* what, const Call& c, cudaStream_t s) {
+  if (!c.traced) return MOE_B200_OK;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  int rc = cuda_status(cudaStreamIsCapturing(s, &capture), what);
+  if (rc != MOE_B200_OK || capture != cudaStreamCaptureStatusNone) return rc;
+  rc = cuda_status(cudaStreamSynchronize(s), what);
+  if (rc != MOE_B200_OK) return rc;
+  const int err = take_word(c.error);
+  return err == 0 ? MOE_B200_OK : set_error(MOE_B200_EP_FAIL, "%s: device error code %d", what, err);
 }
 
 // The CTA-pair kernel or the weight-streaming kernel, by what was measured (bf16, us, forward /
@@ -126,11 +195,16 @@ cudaError_t launch_tc(const moe::GroupedArgs& g, const moe::LoraTerm* lora, cuda
                           : moe::launch_grouped_small(g, lora, sms, s);
 }
 
-int run_grouped(const char* what, const moe::GroupedArgs& g, cudaStream_t s) {
+int run_grouped(const char* what, moe::GroupedArgs& g, cudaStream_t s) {
+  Call call{};
+  int rc = begin(what, &call);
+  if (rc != MOE_B200_OK) return rc;
+  g.error = call.error;
+  g.test_stall = call.stall;
   const cudaError_t st = moe::grouped_tc_supported(g) ? launch_tc(g, nullptr, s)
                                                       : moe::launch_grouped_simt(g, nullptr, s);
-  const int rc = cuda_status(st, what);
-  return rc != MOE_B200_OK ? rc : finish(what, s);
+  rc = cuda_status(st, what);
+  return rc != MOE_B200_OK ? rc : finish(what, call, s);
 }
 
 // Workspace of lora_matmul: four bytes per row and rank entry (two 16-bit parts, or t in
@@ -145,6 +219,15 @@ size_t lora_bytes(int64_t rows, int64_t rank) {
 }  // namespace
 
 extern "C" {
+
+int moe_b200_take_device_error(int32_t* code) {
+  static const char* kWhat = "take_device_error";
+  if (code == nullptr)
+    return set_error(MOE_B200_INVALID_ARGUMENT, "%s: code must be non-NULL", kWhat);
+  int* words = g_error_words.load(std::memory_order_acquire);
+  *code = words == nullptr ? 0 : take_word(device_word(words));
+  return MOE_B200_OK;
+}
 
 int moe_b200_grouped_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
                             int64_t num_experts, const void* x, const void* weights,
@@ -312,6 +395,9 @@ int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
   if (rc == MOE_B200_OK) rc = check_overlap(kWhat, ws, {in[0], in[1], in[2], in[3], in[4], in[5]});
   if (rc != MOE_B200_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  Call call{};
+  rc = begin(kWhat, &call);
+  if (rc != MOE_B200_OK) return rc;
   moe::LoraShrink l{};
   l.dtype = dtype;
   l.rows = num_rows;
@@ -322,6 +408,8 @@ int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
   l.a = lora_a;
   l.ids = adapter_ids;
   l.scales = scales;
+  l.error = call.error;
+  l.test_stall = call.stall;
   moe::GroupedArgs g{};
   g.dtype = dtype;
   g.dir = moe::kGmmForward;
@@ -332,11 +420,13 @@ int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
   g.x = x;
   g.w = weight;
   g.out = y;
+  g.error = call.error;
+  g.test_stall = call.stall;
   const bool a16 = (reinterpret_cast<uintptr_t>(lora_b) & 15) == 0;
   const bool tc = moe::grouped_tc_supported(g) && moe::lora_shrink_tc_supported(l) && a16;
   if (tc && moe::lora_few_supported(num_rows, rank)) {
     rc = cuda_status(moe::launch_lora_few(g, l, lora_b, sm_count(), s), kWhat);
-    return rc != MOE_B200_OK ? rc : finish(kWhat, s);
+    return rc != MOE_B200_OK ? rc : finish(kWhat, call, s);
   }
   moe::LoraTerm term{};
   term.rank = l.rank;
@@ -362,7 +452,7 @@ int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
   rc = cuda_status(st, kWhat);
   if (rc != MOE_B200_OK) return rc;
   rc = cuda_status(tc ? launch_tc(g, &term, s) : moe::launch_grouped_simt(g, &term, s), kWhat);
-  return rc != MOE_B200_OK ? rc : finish(kWhat, s);
+  return rc != MOE_B200_OK ? rc : finish(kWhat, call, s);
 }
 
 }  // extern "C"

@@ -27,8 +27,6 @@
 namespace moe {
 namespace {
 
-__device__ int g_small_error;
-
 constexpr int kBK = 64;
 constexpr int kTileM = 128;
 constexpr int kWBytes = kTileM * kBK * 2;
@@ -54,6 +52,8 @@ struct SmallParams {
   void* out;
   int64_t ldo;
   LoraTerm lora;
+  int* error;
+  int test_stall;
 };
 
 __device__ __forceinline__ void tmem_ld_frag1(uint32_t taddr, float (&v)[4]) {
@@ -168,9 +168,9 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
     const int boxes = (nt + p.box - 1) / p.box;
     int stage = 0;
     uint32_t phase = 0;
-    for (int s = s0; s < s1; s += ds) {
+    for (int s = p.test_stall ? s1 : s0; s < s1; s += ds) {
       if (!mbar_wait(&empty[stage], phase ^ 1)) {
-        atomicExch(&g_small_error, kErrTimeoutProducer);
+        report_error(p.error, kErrTimeoutProducer);
         *abort_flag = 1;
         break;
       }
@@ -202,7 +202,7 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
         left = kSegment;
       }
       if (!ok || !mbar_wait(&full[stage], phase)) {
-        atomicExch(&g_small_error, kErrTimeoutMma);
+        report_error(p.error, kErrTimeoutMma);
         *abort_flag = 1;
         gave_up = true;
         break;
@@ -322,7 +322,7 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
 
   const bool ok = warp_wait(tfull, 0);
   if (!ok) {
-    atomicExch(&g_small_error, kErrTimeoutEpilogue);
+    report_error(p.error, kErrTimeoutEpilogue);
     *abort_flag = 1;
   }
   tc_fence_after();
@@ -359,7 +359,7 @@ grouped_small_kernel(const __grid_constant__ CUtensorMap map_w,
         st_async_f4(mapa_shared(dst, owner), lo, bar);
         st_async_f4(mapa_shared(dst + 512, owner), hi, bar);
       }
-    if (owned > 0 && !wait_parts(xfull)) atomicExch(&g_small_error, kErrTimeoutEpilogue);
+    if (owned > 0 && !wait_parts(xfull)) report_error(p.error, kErrTimeoutEpilogue);
   }
 
   uint8_t* buf = stage_out + (warp & 7) * kEpiBytes;
@@ -429,6 +429,8 @@ cudaError_t launch_small(const GroupedArgs& g, const LoraTerm* lora, int num_sms
   p.m_tiles = (feat + kTileM - 1) / kTileM;
   p.out = g.out;
   p.ldo = feat;
+  p.error = g.error;
+  p.test_stall = g.test_stall;
   if (lora != nullptr) p.lora = *lora;
   // Tile cap: twice the mean rows per group (uneven groups then mostly stay one tile, and
   // their weights are streamed once), all of them when there is one group.
@@ -504,13 +506,6 @@ cudaError_t launch_grouped_small(const GroupedArgs& g, const LoraTerm* lora, int
   if (g.dtype == kDtF16) return launch_small_type<__half>(g, lora, num_sms, s);
   if (g.dtype == kDtBF16) return launch_small_type<__nv_bfloat16>(g, lora, num_sms, s);
   return cudaErrorInvalidValue;
-}
-
-cudaError_t take_grouped_small_error(int* err) {
-  cudaError_t st = cudaMemcpyFromSymbol(err, g_small_error, sizeof(int));
-  if (st != cudaSuccess || *err == 0) return st;
-  const int zero = 0;
-  return cudaMemcpyToSymbol(g_small_error, &zero, sizeof(int));
 }
 
 }  // namespace moe

@@ -47,11 +47,6 @@ namespace moe {
 
 namespace {
 
-// Set by a kernel whose bounded wait ran out (a DeviceError); read and cleared by the host
-// under MOE_B200_TRACE_SYNC.  One word per device, not per call: a call has no zeroed
-// workspace to put it in, and zeroing one would cost every call a launch.
-__device__ int g_pair_error;
-
 constexpr int kBK = 64;
 constexpr int kTileM = 256;
 constexpr int kTileN = 256;
@@ -82,6 +77,8 @@ struct PairParams {
   int64_t ldo;
   LoraTerm lora;
   int rank_blocks;  // of 64
+  int* error;
+  int test_stall;
 };
 
 struct PairTile {
@@ -295,7 +292,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
       uint32_t phase = 0;
       for (int i = 0;; ++i) {
         const int L = turn_tile(i, pair, npairs);
-        if (L >= total || *abort_flag) break;
+        if (L >= total || *abort_flag || p.test_stall) break;
         const PairTile t = pair_tile<DIR>(L, table, p);
         const int a0 = t.m0 + static_cast<int>(rank) * 128;
         // Rows of this CTA's half of the MMA's N, in boxes of 64.
@@ -304,7 +301,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
         const int b_boxes = DIR == kGmmGradWeight ? 2 : (half + 63) / 64;
         for (int b = 0; b < t.blocks; ++b) {
           if (!mbar_wait(&empty[stage], phase ^ 1)) {
-            atomicExch(&g_pair_error, kErrTimeoutProducer);
+            report_error(p.error, kErrTimeoutProducer);
             *abort_flag = 1;
             break;
           }
@@ -344,7 +341,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
             fence_proxy_async_all();
           }
           if (!mbar_wait(&cfull[i & 1], (i >> 1) & 1)) {
-            atomicExch(&g_pair_error, kErrTimeoutProducer);
+            report_error(p.error, kErrTimeoutProducer);
             *abort_flag = 1;
           }
           RunWalk w(codes + (i & 1) * 16, (t.n + 15) / 16);
@@ -354,7 +351,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
             const int r0 = t.n0 + w.begin * 16 + static_cast<int>(rank) * rows_half;
             for (int b = 0; b < 2 * p.rank_blocks; ++b) {
               if (!mbar_wait(&empty[stage], phase ^ 1)) {
-                atomicExch(&g_pair_error, kErrTimeoutProducer);
+                report_error(p.error, kErrTimeoutProducer);
                 *abort_flag = 1;
                 break;
               }
@@ -389,7 +386,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
                                (kAMn ? kIdescAMn : 0) | (kBMn ? kIdescBMn : 0);
         const int acc = i & 1;
         if (!drained(acc) || (SEG && both && !drained(acc ^ 1))) {
-          atomicExch(&g_pair_error, kErrTimeoutMma);
+          report_error(p.error, kErrTimeoutMma);
           *abort_flag = 1;
           break;
         }
@@ -406,7 +403,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
             tc_fence_after();
           }
           if (!ok || !mbar_wait(&full[stage], phase)) {
-            atomicExch(&g_pair_error, kErrTimeoutMma);
+            report_error(p.error, kErrTimeoutMma);
             *abort_flag = 1;
             ok = false;
             break;
@@ -456,7 +453,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
           }
           mbar_arrive(&cempty[i & 1]);
           if (!ok) {
-            atomicExch(&g_pair_error, kErrTimeoutMma);
+            report_error(p.error, kErrTimeoutMma);
             *abort_flag = 1;
           }
         }
@@ -477,7 +474,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
       if (L >= total || warp_stopped(abort_flag)) break;
       const PairTile t = pair_tile<DIR>(L, table, p);
       if (!warp_wait(&cempty[i & 1], ((i >> 1) & 1) ^ 1)) {
-        atomicExch(&g_pair_error, kErrTimeoutProducer);
+        report_error(p.error, kErrTimeoutProducer);
         *abort_flag = 1;
         break;
       }
@@ -531,7 +528,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
         if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));
       }
       if (!ok) {
-        atomicExch(&g_pair_error, kErrTimeoutEpilogue);
+        report_error(p.error, kErrTimeoutEpilogue);
         *abort_flag = 1;
         break;
       }
@@ -591,7 +588,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a,
       if constexpr (LORA > 0) {
         LoraFrags<LORA> frags;  // of this tile's features
         if (!warp_wait(&cfull[i & 1], (i >> 1) & 1)) {
-          atomicExch(&g_pair_error, kErrTimeoutEpilogue);
+          report_error(p.error, kErrTimeoutEpilogue);
           *abort_flag = 1;
           break;
         }
@@ -749,6 +746,8 @@ cudaError_t launch_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
   p.rows = static_cast<int>(g.rows);
   p.E = g.E;
   p.out = g.out;
+  p.error = g.error;
+  p.test_stall = g.test_stall;
   if (LORA > 0) p.lora = *lora;
   bool ok;
   if (DIR == kGmmGradWeight) {
@@ -860,13 +859,6 @@ cudaError_t launch_grouped_pair(const GroupedArgs& g, const LoraTerm* lora, int 
   if (g.dtype == kDtF16) return launch_pair_type<__half>(g, lora, num_sms, s);
   if (g.dtype == kDtBF16) return launch_pair_type<__nv_bfloat16>(g, lora, num_sms, s);
   return cudaErrorInvalidValue;
-}
-
-cudaError_t take_grouped_pair_error(int* err) {
-  cudaError_t st = cudaMemcpyFromSymbol(err, g_pair_error, sizeof(int));
-  if (st != cudaSuccess || *err == 0) return st;
-  const int zero = 0;
-  return cudaMemcpyToSymbol(g_pair_error, &zero, sizeof(int));
 }
 
 }  // namespace moe

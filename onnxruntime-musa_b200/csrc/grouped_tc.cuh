@@ -95,6 +95,12 @@ __device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t saddr, uint32_t 
 constexpr uint32_t kIdescAMn = 1u << 15;
 constexpr uint32_t kIdescBMn = 1u << 16;
 
+// Reports a wait that ran out (a DeviceError) to the host: `word` is pinned host memory.
+__device__ __forceinline__ void report_error(int* word, int code) {
+  *reinterpret_cast<volatile int*>(word) = code;
+  __threadfence_system();
+}
+
 // mbar_wait() by a whole warp: its lanes leave together, whichever of them ran out of time, so
 // that what the warp does next as one (tensor memory loads, shuffles) stays whole.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {

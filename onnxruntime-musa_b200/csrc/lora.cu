@@ -111,8 +111,6 @@ lora_shrink_simt_kernel(const T* __restrict__ x, const T* __restrict__ a,
   }
 }
 
-__device__ int g_shrink_error;
-
 constexpr int kBK = 64;
 constexpr int kM = 128;
 constexpr int kABytes = kM * kBK * 2;
@@ -138,6 +136,8 @@ struct ShrinkParams {
   int a_bytes;    // rows of A_a in a stage (the MMA reads on behind them, in other stages
                   // or the slack after the ring: lanes that nobody reads)
   int stages, stage_bytes;
+  int* error;
+  int test_stall;
 };
 
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
@@ -257,7 +257,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
     // a slice: issued by one thread they took longer than the transfer).
     int stage = 0;
     uint32_t phase = 0;
-    bool ok = true;
+    bool ok = p.test_stall == 0;
     for (int ps = 0; ps < passes && ok; ++ps) {
       const int u0 = ps * per, nu = min(per, units - u0);
       const int unit = u0 + lane;
@@ -272,7 +272,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
             mbar_arrive_expect_tx(&full[stage], (nu * rows_u + p.chunk) * kBK * 2);
             tma_load_3d(w + p.a_bytes, &map_x, &full[stage], s * kBK, static_cast<int>(row0), 0);
           } else {
-            atomicExch(&g_shrink_error, kErrTimeoutProducer);
+            report_error(p.error, kErrTimeoutProducer);
             *abort_flag = 1;
           }
         }
@@ -311,7 +311,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
         tc_commit(&tfull[acc]);  // after a timeout too: it waits for the MMAs issued
       }
       if (!ok) {
-        atomicExch(&g_shrink_error, kErrTimeoutMma);
+        report_error(p.error, kErrTimeoutMma);
         *abort_flag = 1;
         drain_ring(full, p.stages, stage, phase);
       }
@@ -330,7 +330,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
       for (int i = 0; i < n; ++i)
         if (s_slot[i] == slot) own |= uint64_t{1} << i;
       if (!warp_wait(&tfull[acc], (fill >> 1) & 1)) {
-        atomicExch(&g_shrink_error, kErrTimeoutEpilogue);
+        report_error(p.error, kErrTimeoutEpilogue);
         *abort_flag = 1;
         break;
       }
@@ -449,6 +449,8 @@ cudaError_t shrink_tc(const LoraShrink& l, uint16_t* parts, float* row_scale, in
   p.K = l.K;
   p.rank = l.rank;
   p.adapters = l.adapters;
+  p.error = l.error;
+  p.test_stall = l.test_stall;
   p.chunk = shrink_chunk(l.rows);
   p.mma_n = std::max(p.chunk, 16);
   // A stage holds the adapters that a chunk can have (one token: r rows), so that a short
@@ -504,13 +506,6 @@ cudaError_t launch_lora_shrink_tc(const LoraShrink& l, uint16_t* parts, float* r
   if (l.dtype == kDtBF16)
     return shrink_tc<__nv_bfloat16>(l, parts, row_scale, row_code, num_sms, s);
   return cudaErrorInvalidValue;
-}
-
-cudaError_t take_lora_error(int* err) {
-  cudaError_t st = cudaMemcpyFromSymbol(err, g_shrink_error, sizeof(int));
-  if (st != cudaSuccess || *err == 0) return st;
-  const int zero = 0;
-  return cudaMemcpyToSymbol(g_shrink_error, &zero, sizeof(int));
 }
 
 }  // namespace moe

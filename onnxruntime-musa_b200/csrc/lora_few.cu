@@ -19,8 +19,6 @@
 namespace moe {
 namespace {
 
-__device__ int g_few_error;
-
 constexpr int kBK = 64;
 constexpr int kTileM = 128;
 constexpr int kWBytes = kTileM * kBK * 2;
@@ -41,6 +39,8 @@ struct FewParams {
   int rows, N, K, rank, adapters;
   int splits, stages, stage_bytes, a_bytes;
   int quads;  // ceil(rows / 4)
+  int* error;
+  int test_stall;
 };
 
 __device__ __forceinline__ void st_async_f4(uint32_t addr, float a, float b, float c, float d,
@@ -118,7 +118,7 @@ lora_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     const int mine = __popc(__ballot_sync(0xffffffffu, ad >= 0));
     int stage = 0;
     uint32_t phase = 0;
-    for (int s = split; s < slices; s += S) {
+    for (int s = p.test_stall ? slices : split; s < slices; s += S) {
       uint8_t* w = ring + stage * p.stage_bytes;
       int ok = 1;
       if (lane == 0) {
@@ -129,7 +129,7 @@ lora_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
           tma_load_3d(w, &map_w, &full[stage], s * kBK, m0, 0);
           tma_load_3d(w + kWBytes + p.a_bytes, &map_x, &full[stage], s * kBK, 0, 0);
         } else {
-          atomicExch(&g_few_error, kErrTimeoutProducer);
+          report_error(p.error, kErrTimeoutProducer);
         }
       }
       if (!__shfl_sync(0xffffffffu, ok, 0)) break;
@@ -151,7 +151,7 @@ lora_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
           left = kSegment;
         }
         if (!ok || !mbar_wait(&full[stage], phase)) {
-          atomicExch(&g_few_error, kErrTimeoutMma);
+          report_error(p.error, kErrTimeoutMma);
           gave_up = true;
           break;
         }
@@ -218,7 +218,7 @@ lora_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     if (lane == 0) mbar_arrive(sempty);
   }
   const bool ok = warp_wait(tfull, 0);
-  if (!ok) atomicExch(&g_few_error, kErrTimeoutEpilogue);
+  if (!ok) report_error(p.error, kErrTimeoutEpilogue);
   tc_fence_after();
   if (S > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (epi) {
@@ -242,7 +242,7 @@ lora_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     }
   }
   if (split == 0 && epi) {
-    if (S > 1 && !wait_parts(xfull)) atomicExch(&g_few_error, kErrTimeoutEpilogue);
+    if (S > 1 && !wait_parts(xfull)) report_error(p.error, kErrTimeoutEpilogue);
     for (int r = 1; r < S; ++r) {  // the parts in rank order
       const uint8_t* src = parts + (r - 1) * part_bytes(p.quads);
       const float4 a = *reinterpret_cast<const float4*>(src + me * 16);
@@ -296,6 +296,8 @@ cudaError_t launch_few(const GroupedArgs& g, const LoraShrink& l, const void* b,
   p.ids = l.ids;
   p.scales = l.scales;
   p.y = g.out;
+  p.error = g.error;
+  p.test_stall = g.test_stall;
   p.rows = static_cast<int>(g.rows);
   p.N = g.N;
   p.K = g.K;
@@ -336,13 +338,6 @@ cudaError_t launch_lora_few(const GroupedArgs& g, const LoraShrink& l, const voi
   if (g.dtype == kDtF16) return launch_few<__half>(g, l, b, num_sms, s);
   if (g.dtype == kDtBF16) return launch_few<__nv_bfloat16>(g, l, b, num_sms, s);
   return cudaErrorInvalidValue;
-}
-
-cudaError_t take_lora_few_error(int* err) {
-  cudaError_t st = cudaMemcpyFromSymbol(err, g_few_error, sizeof(int));
-  if (st != cudaSuccess || *err == 0) return st;
-  const int zero = 0;
-  return cudaMemcpyToSymbol(g_few_error, &zero, sizeof(int));
 }
 
 }  // namespace moe
