@@ -149,13 +149,28 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   return v;
 }
 
-// Two 16-bit parts of each of four values.
+// Two 16-bit parts of a value.  A finite value that would round to infinity takes the largest
+// finite one and the rest; an infinity stays one part (its rest would be NaN).
+template <typename T> constexpr float kMaxFinite = 65504.f;
+template <> constexpr float kMaxFinite<__nv_bfloat16> = 3.3895313892515355e38f;
+template <typename T>
+__device__ __forceinline__ void split_part(float v, float& hi, float& lo) {
+  hi = to_f(from_f<T>(v));
+  lo = v - hi;
+  if (isinf(hi)) {
+    if (isfinite(v)) hi = copysignf(kMaxFinite<T>, v);
+    lo = isfinite(v) ? v - hi : 0.f;
+  }
+}
 template <typename T>
 __device__ __forceinline__ void split_parts(const float4& v, uint2& hi, uint2& lo) {
-  const float h0 = to_f(from_f<T>(v.x)), h1 = to_f(from_f<T>(v.y));
-  const float h2 = to_f(from_f<T>(v.z)), h3 = to_f(from_f<T>(v.w));
-  hi = make_uint2(pack2<T>(h0, h1), pack2<T>(h2, h3));
-  lo = make_uint2(pack2<T>(v.x - h0, v.y - h1), pack2<T>(v.z - h2, v.w - h3));
+  float h[4], l[4];
+  split_part<T>(v.x, h[0], l[0]);
+  split_part<T>(v.y, h[1], l[1]);
+  split_part<T>(v.z, h[2], l[2]);
+  split_part<T>(v.w, h[3], l[3]);
+  hi = make_uint2(pack2<T>(h[0], h[1]), pack2<T>(h[2], h[3]));
+  lo = make_uint2(pack2<T>(l[0], l[1]), pack2<T>(l[2], l[3]));
 }
 
 // SEG: a CTA may have more than one segment of slices.
@@ -385,15 +400,16 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x,
         }
         v[h].x *= sc; v[h].y *= sc; v[h].z *= sc; v[h].w *= sc;
       }
-      m = fmaxf(m, fmaxf(fmaxf(fabsf(v[h].x), fabsf(v[h].y)), fmaxf(fabsf(v[h].z), fabsf(v[h].w))));
+      auto size = [](float t) { return isfinite(t) ? fabsf(t) : 0.f; };  // (no scale helps others)
+      m = fmaxf(m, fmaxf(fmaxf(size(v[h].x), size(v[h].y)), fmaxf(size(v[h].z), size(v[h].w))));
     }
     int code = s_id[i];
     if (std::is_same<T, __half>::value) {
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
       float down = 1.f;
-      // Inside [2^-8, 2^15) the parts keep 16 bits of the row's largest entry as they are.
-      if ((m > 0.f && m < 0.00390625f) || (m >= 32768.f && m < __int_as_float(0x7f800000))) {
+      // Inside [2^-8, 2^15) the parts keep 16 bits of the row's largest finite entry as they are.
+      if ((m > 0.f && m < 0.00390625f) || m >= 32768.f) {
         const int e = min(max((__float_as_int(m) >> 23) - 127, -120), 120);
         const float up = __int_as_float((127 - e) << 23);
         down = __int_as_float((127 + e) << 23);
