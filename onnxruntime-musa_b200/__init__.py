@@ -821,6 +821,20 @@ def _device_of(what: str, t):
     return t.device
 
 
+def _refuse_gradients(what: str, *tensors) -> None:
+    """These calls record nothing for autograd: a result that dropped its history without a word
+    would train wrongly.  (Inside ``torch.autograd.Function`` and ``torch.no_grad()`` nothing is
+    recorded anyway.)"""
+    if not _torch().is_grad_enabled():
+        return
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise ValueError(f"{what}: an argument requires a gradient, which this call does not "
+                             "record; call it under torch.no_grad() or in a torch.autograd.Function "
+                             "(grouped_matmul_grad_input and grouped_matmul_grad_weight are the "
+                             "gradients of grouped_matmul)")
+
+
 class _Elsewhere:
     """A call on another device than the current one, or on a stream of the caller's: the
     device and stream are current inside (outputs and workspaces then come from that
@@ -867,8 +881,11 @@ def grouped_matmul(x, weights, expert_offsets, out=None, stream=None):
     ``x`` [R, K] in expert order (:func:`permute`, :func:`ep_dispatch`), ``weights``
     [E, N, K], ``expert_offsets`` int32 [E + 1] on the device; returns [R, N] (``out`` if
     given).  Rows from ``expert_offsets[E]`` on are neither read nor written.  float32,
-    float16 or bfloat16, fp32 sums."""
+    float16 or bfloat16, fp32 sums.  Nothing is recorded for autograd: arguments that require a
+    gradient are refused while gradients are enabled (the two functions below are the
+    gradients)."""
     what = "grouped_matmul"
+    _refuse_gradients(what, x, weights, out)
     R, K = _dims(what, "x", x, 2)
     E, N, _ = _dims(what, "weights", weights, 3)
     return _product(what, "x", lib().moe_b200_grouped_matmul, x, weights, expert_offsets, out,
@@ -879,6 +896,7 @@ def grouped_matmul_grad_input(dy, weights, expert_offsets, out=None, stream=None
     """Gradient of :func:`grouped_matmul` with respect to ``x``:
     ``dx[p] = weights[e].T @ dy[p]``; ``dy`` [R, N], returns [R, K]."""
     what = "grouped_matmul_grad_input"
+    _refuse_gradients(what, dy, weights, out)
     R, N = _dims(what, "dy", dy, 2)
     E, _, K = _dims(what, "weights", weights, 3)
     return _product(what, "dy", lib().moe_b200_grouped_matmul_grad_input, dy, weights,
@@ -910,6 +928,7 @@ def grouped_matmul_grad_weight(x, dy, expert_offsets, out=None, stream=None):
     ``dw[e] = sum_p outer(dy[p], x[p])`` over the rows of expert e (zeros if it has none);
     ``x`` [R, K], ``dy`` [R, N], returns [E, N, K]."""
     what = "grouped_matmul_grad_weight"
+    _refuse_gradients(what, x, dy, out)
     R, K = _dims(what, "x", x, 2)
     _, N = _dims(what, "dy", dy, 2)
     E = _dims(what, "expert_offsets", expert_offsets, 1)[0] - 1
@@ -951,6 +970,7 @@ def lora_matmul(x, weight, lora_a, lora_b, adapter_ids, scales, out=None, stream
     returns [T, N].  float32, float16 or bfloat16; the intermediate is not rounded to the
     16-bit type."""
     what = "lora_matmul"
+    _refuse_gradients(what, x, weight, lora_a, lora_b, scales, out)
     T, K = _dims(what, "x", x, 2)
     N, _ = _dims(what, "weight", weight, 2)
     A, r, _ = _dims(what, "lora_a", lora_a, 3)
