@@ -21,13 +21,16 @@ namespace moe {
 // that kernel reads) it calls pdl_wait(), which returns once the previous grid has
 // completed and its memory is visible; it calls pdl_wait() before exiting in any case,
 // so that its own completion implies its predecessor's.  pdl_launch_dependents() lets
-// the next such kernel launch.  Both are no-ops for a normal launch.
+// the next such kernel launch, whichever way its own kernel was launched (a layer's kernels
+// are launched normally, and an expert product behind one may start early).  In a kernel
+// that was launched normally pdl_wait() returns at once: everything in front has completed.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-// Host side, read once.  Decode chain (QMoE weight streaming): on unless MOE_B200_PDL=0.
+// Host side, read once.  Decode chain (QMoE weight streaming), expert products and adapter
+// projection: on unless MOE_B200_PDL=0.
 // Layer chain (planning, gather, GEMMs, combine): off unless MOE_B200_PDL_LAYER=1.  On
 // B200 the layer chain gained 6% of device time at C1 (0.114 -> 0.107 ms) but lost 21% of
 // end-to-end throughput through the host-buffer pipeline (2.39 -> 1.89 M tokens/s), whose

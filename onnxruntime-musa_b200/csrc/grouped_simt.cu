@@ -588,7 +588,7 @@ grouped_gemv_kernel(const SimtParams p) {
 template <typename T>
 cudaError_t launch_gemv(const SimtParams& p, cudaStream_t s) {
   const int per = kThreads / 32 * kGemvCols;
-  return launch_dependent(true, grouped_gemv_kernel<T>, dim3((p.N + per - 1) / per, p.E),
+  return launch_dependent(pdl_enabled(), grouped_gemv_kernel<T>, dim3((p.N + per - 1) / per, p.E),
                           dim3(kThreads), 0, s, p);
 }
 
@@ -621,7 +621,7 @@ cudaError_t launch_tile(const GroupedArgs& g, SimtParams p, cudaStream_t s) {
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = 1;
   attr[1].val.clusterDim.y = 1;

@@ -763,7 +763,7 @@ cudaError_t launch_pair(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
          grouped_map(&mbt, g.dtype, tx, g.K, static_cast<int64_t>(g.E) * kTailRows, 1, kTailRows);
     if (!ok) return cudaErrorInvalidValue;
     const int vecs = kTailRows * (g.N + g.K) / 8;
-    cudaError_t st = launch_dependent(true, tail_kernel,
+    cudaError_t st = launch_dependent(pdl_enabled(), tail_kernel,
                                       dim3(std::min(32, (vecs + 255) / 256), g.E), dim3(256), 0, s, g.offsets,
                                       p.rows, static_cast<const uint4*>(g.dy), g.N / 8,
                                       static_cast<const uint4*>(g.x), g.K / 8,

@@ -212,7 +212,7 @@ struct SmemOptIn {
   }
 };
 
-// Launches with programmatic stream serialisation: the kernel may start while the one before
+// Launches with programmatic stream serialisation (unless MOE_B200_PDL=0): the kernel may start while the one before
 // it on the stream drains, and calls pdl_wait() before it touches memory.  (Set up, barriers,
 // tensor memory and descriptors then overlap the launch before: 2 us of a 10 us call.)
 // `cluster` 0: the kernel's own.
@@ -226,7 +226,7 @@ cudaError_t launch_overlapped(void (*kernel)(KArgs...), unsigned grid, int block
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
   attr[1].val.clusterDim.y = 1;

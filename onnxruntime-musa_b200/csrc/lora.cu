@@ -444,7 +444,7 @@ cudaError_t shrink_simt(const LoraShrink& l, float* t, cudaStream_t s) {
   const bool vec = l.K % 4 == 0 &&
                    (reinterpret_cast<uintptr_t>(l.x) | reinterpret_cast<uintptr_t>(l.a)) %
                            (4 * sizeof(T)) == 0;
-  return launch_dependent(true, lora_shrink_simt_kernel<T>,
+  return launch_dependent(pdl_enabled(), lora_shrink_simt_kernel<T>,
                           dim3(static_cast<unsigned>((l.rows + kRows - 1) / kRows),
                                (l.rank + kWarps - 1) / kWarps),
                           dim3(kWarps * 32), 0, s, static_cast<const T*>(l.x),

@@ -1,5 +1,9 @@
 """The expert products and the adapter projection in the settings that a program calls them in."""
 
+import os
+import subprocess
+import sys
+
 import pytest
 
 from gpu_util import as_np
@@ -36,3 +40,51 @@ def test_training_through_an_autograd_function(pkg, orc, dev):
     hx, hw, hdy = as_np(x), as_np(w), as_np(dy)
     assert_close(dx, *orc.grouped_matmul_grad_input(hdy, hw, hoff), N, "float32")
     assert_close(dw, *orc.grouped_matmul_grad_weight(hx, hdy, hoff), max(counts), "float32")
+
+
+# One process, since the switch is read once: captures a chain of calls and counts the graph's
+# programmatic edges (a kernel that may start while the one in front drains).
+EDGES = """
+import ctypes, sys, torch
+sys.path.insert(0, sys.argv[1])
+from __graft_entry__ import load_package
+pkg = load_package()
+dev = torch.device("cuda", 0)
+off = torch.tensor([0, 30, 30, 60], dtype=torch.int32, device=dev)
+ids = torch.arange(60, dtype=torch.int32, device=dev) % 3
+sc = torch.ones(3, device=dev)
+calls = []
+for dt, rank in ((torch.float32, 5), (torch.bfloat16, 16)):
+    t = lambda *s: torch.randn(*s, device=dev).to(dt)
+    x, w, dy, a, b = t(60, 64), t(3, 128, 64), t(60, 128), t(3, rank, 64), t(3, 128, rank)
+    calls += [lambda x=x, w=w: pkg.grouped_matmul(x, w, off),
+              lambda dy=dy, w=w: pkg.grouped_matmul_grad_input(dy, w, off),
+              lambda x=x, dy=dy: pkg.grouped_matmul_grad_weight(x, dy, off),
+              lambda x=x, w=w, a=a, b=b: pkg.lora_matmul(x, w[0], a, b, ids, sc),
+              lambda x=x, w=w, a=a, b=b: pkg.lora_matmul(x[:3], w[0], a, b, ids[:3], sc)]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph(keep_graph=True)
+with torch.cuda.graph(g):
+    out = [c() for c in calls]
+drv = ctypes.CDLL("libcuda.so.1")
+raw, n = ctypes.c_void_p(g.raw_cuda_graph()), ctypes.c_size_t(0)
+assert drv.cuGraphGetEdges_v2(raw, None, None, None, ctypes.byref(n)) == 0
+nodes, data = (ctypes.c_void_p * n.value)(), (ctypes.c_ubyte * (8 * n.value))()
+assert drv.cuGraphGetEdges_v2(raw, nodes, (ctypes.c_void_p * n.value)(), data, ctypes.byref(n)) == 0
+print("edges", n.value, "programmatic", sum(data[8 * i + 2] == 1 for i in range(n.value)))
+g.instantiate()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(o, c()) for o, c in zip(out, calls))
+"""
+
+
+@pytest.mark.parametrize("switch", ["0", "1"])
+def test_overlapped_launches_can_be_turned_off(dev, switch):
+    """MOE_B200_PDL=0 holds for these calls too, with the same bits."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", EDGES, root], cwd=root, timeout=300,
+                          env=dict(os.environ, MOE_B200_PDL=switch), capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr[-2000:]
+    edges, programmatic = (int(w) for w in done.stdout.split()[1::2])
+    assert edges >= 10 and (programmatic == 0 if switch == "0" else programmatic >= 8)
