@@ -361,8 +361,13 @@ int moe_b200_grouped_matmul_grad_weight(int32_t dtype, int64_t num_rows, int64_t
  * int32 [num_rows], scales fp32 [L], y [num_rows, n]; 1 <= rank <= 256, an adapter of
  * smaller rank is padded with zeros.  Rows may follow any adapters in any order; a row is
  * touched by its own adapter only (an infinity or NaN in another one does not reach it).
- * The rank-sized intermediate is kept in fp32.  Types, sizes and alignment as above (rank
- * a multiple of 8 for the tensor cores).  `workspace`: 256-byte aligned, at least
+ * The rank-sized intermediate scales[a] lora_a[a] x[t] is held in fp32, and enters the second
+ * product in fp32 for float, on the FFMA kernels and up to eight rows with num_rows * rank <= 128.
+ * Other 16-bit calls on the tensor cores take it as the sum of two 16-bit parts, which keep each
+ * entry to 2^-16 of itself (bfloat16), or to the larger of 2^-22 of itself and 2^-17 of its row's
+ * largest finite entry (float16); an infinite entry of lora_b may come out as NaN there.
+ * Types, sizes and alignment as above (rank a multiple of 8 for the tensor cores; a call off
+ * that runs all of it on FFMA kernels, so pad ranks with zeros).  `workspace`: 256-byte aligned, at least
  * moe_b200_lora_matmul_workspace_size bytes, not shared by calls that may overlap.
  * No counterpart in the reference. */
 int moe_b200_lora_matmul_workspace_size(int32_t dtype, int64_t num_rows, int64_t rank,

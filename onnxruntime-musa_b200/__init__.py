@@ -968,7 +968,8 @@ def lora_matmul(x, weight, lora_a, lora_b, adapter_ids, scales, out=None, stream
     ``x`` [T, K], ``weight`` [N, K], ``lora_a`` [L, r, K], ``lora_b`` [L, N, r] (adapters of
     smaller rank padded with zeros), ``adapter_ids`` int32 [T], ``scales`` float32 [L];
     returns [T, N].  float32, float16 or bfloat16; the intermediate is not rounded to the
-    16-bit type."""
+    16-bit type (fp32, or the sum of two 16-bit parts on the tensor cores above eight rows: see
+    ``moe_b200_lora_matmul`` in the header)."""
     what = "lora_matmul"
     _refuse_gradients(what, x, weight, lora_a, lora_b, scales, out)
     T, K = _dims(what, "x", x, 2)

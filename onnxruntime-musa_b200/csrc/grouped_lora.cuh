@@ -3,10 +3,15 @@
 // on accumulator fragments as tmem_ld_frag* delivers them (32 features x 8 rows per warp).
 //
 // The rank-sized intermediate enters mma.m16n8k16 as the sum of two 16-bit parts,
-// hi = round(s_a t) and lo = round(s_a t - hi), which keeps 16 (bf16) or 22 (fp16) of its
-// bits; one part would leave an error of half an output step of the term itself.  fp16
-// rows outside [2^-8, 2^15) are first scaled by a power of two to |s_a t| < 2 (t may exceed
-// fp16's range), undone on the fp32 sum.  The shrink kernel (lora.cu) forms the parts.
+// hi = round(s_a t) and lo = round(s_a t - hi).  In bf16 they keep an entry to 2^-16 of itself (half
+// a step, 2^-8, of a rest that is at most 2^-8 of it); one part would leave an error of half an
+// output step of the term itself.  In fp16 to 2^-22 of itself (2^-11 twice), but not below 2^-25,
+// half the type's smallest step: rows whose largest finite entry lies outside [2^-8, 2^15) are first
+// scaled by a power of two to |s_a t| < 2 (t may exceed fp16's range), undone on the fp32 sum,
+// so that floor is at most 2^-17 of the row's largest entry.  (Every row scaled would hold it at 2^-25,
+// but sixteen rows with a scaled one among them go through mma.sync in the pair kernel's epilogue,
+// whose price stands there.)
+// The shrink kernel (lora.cu) forms the parts.
 // The eight rows of a fragment may follow different adapters: the products of each adapter
 // among them are formed for all eight columns in a sum of their own, and a column takes
 // only its own adapter's, so nothing of another adapter (an infinity, say) reaches a row.

@@ -1,8 +1,9 @@
 // Adapter projections of rows that follow different adapters: t[row] = A_a x[row].
 //
 // The second half, y += s_a B_a t, runs in the epilogue of the shared projection's kernels
-// (grouped_simt.cu, grouped_small.cu, grouped_tc.cu), so y is written once and t stays in
-// fp32.
+// (grouped_simt.cu, grouped_small.cu, grouped_tc.cu), so y is written once.  t is summed in fp32;
+// the FFMA kernels take it as it is, the tensor-core kernels in two 16-bit parts
+// (grouped_lora.cuh says what those keep).
 //
 // lora_shrink_tc_kernel (16-bit types): a CTA takes a chunk of adjacent rows and one split
 // of K.  The A_a of the chunk's distinct adapters are stacked as the MMA's M (128 / r
