@@ -91,6 +91,7 @@ cudaError_t launch_lora_few(const GroupedArgs& g, const LoraShrink& l, const voi
                             cudaStream_t s);
 
 // FFMA kernels: any size, alignment and float type.
-cudaError_t launch_grouped_simt(const GroupedArgs& g, const LoraTerm* lora, cudaStream_t s);
+cudaError_t launch_grouped_simt(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
+                                cudaStream_t s);
 
 }  // namespace moe

@@ -202,7 +202,7 @@ int run_grouped(const char* what, moe::GroupedArgs& g, cudaStream_t s) {
   g.error = call.error;
   g.test_stall = call.stall;
   const cudaError_t st = moe::grouped_tc_supported(g) ? launch_tc(g, nullptr, s)
-                                                      : moe::launch_grouped_simt(g, nullptr, s);
+                                                      : moe::launch_grouped_simt(g, nullptr, sm_count(), s);
   rc = cuda_status(st, what);
   return rc != MOE_B200_OK ? rc : finish(what, call, s);
 }
@@ -451,7 +451,7 @@ int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
   }
   rc = cuda_status(st, kWhat);
   if (rc != MOE_B200_OK) return rc;
-  rc = cuda_status(tc ? launch_tc(g, &term, s) : moe::launch_grouped_simt(g, &term, s), kWhat);
+  rc = cuda_status(tc ? launch_tc(g, &term, s) : moe::launch_grouped_simt(g, &term, sm_count(), s), kWhat);
   return rc != MOE_B200_OK ? rc : finish(kWhat, call, s);
 }
 

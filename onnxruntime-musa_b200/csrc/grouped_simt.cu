@@ -593,7 +593,7 @@ cudaError_t launch_gemv(const SimtParams& p, cudaStream_t s) {
 }
 
 template <typename T, int DIR, int TM, int TN, int NT, bool LORA>
-cudaError_t launch_tile(const GroupedArgs& g, SimtParams p, cudaStream_t s) {
+cudaError_t launch_tile(const GroupedArgs& g, SimtParams p, int num_sms, cudaStream_t s) {
   constexpr int BM = NT / 16 * TM, BN = 16 * TN;
   dim3 grid;
   p.splits = 1;
@@ -612,7 +612,7 @@ cudaError_t launch_tile(const GroupedArgs& g, SimtParams p, cudaStream_t s) {
   }
   // Split until the SMs' resident CTAs run (four, of 128 x 128 tiles two), with a contraction
   // of at least 64 each.
-  const int64_t fill = 148 * resident(TM, NT);
+  const int64_t fill = static_cast<int64_t>(num_sms) * resident(TM, NT);
   while (p.splits < 4 && tiles * p.splits * 2 <= fill && con >= 128 * p.splits) p.splits *= 2;
   grid.z *= p.splits;
   cudaLaunchConfig_t cfg{};
@@ -634,7 +634,7 @@ cudaError_t launch_tile(const GroupedArgs& g, SimtParams p, cudaStream_t s) {
 }
 
 template <typename T, int DIR, bool LORA>
-cudaError_t launch_dir(const GroupedArgs& g, const LoraTerm* lora, cudaStream_t s) {
+cudaError_t launch_dir(const GroupedArgs& g, const LoraTerm* lora, int num_sms, cudaStream_t s) {
   SimtParams p{};
   p.a = DIR == kGmmForward ? g.x : g.dy;
   p.b = DIR == kGmmGradWeight ? g.x : g.w;
@@ -666,29 +666,30 @@ cudaError_t launch_dir(const GroupedArgs& g, const LoraTerm* lora, cudaStream_t 
   const int64_t height = DIR == kGmmGradWeight ? g.N : g.rows / g.E;
   // (With element-wise loads the small tiles win until the big ones fill the GPU unsplit.)
   const int64_t ways = p.a_vec && p.b_vec ? 4 : 1;
-  const int64_t enough = ways == 4 && g.E > 1 && DIR != kGmmGradWeight ? 300 : 148;
-  if (height >= 96 && feat >= 96 && ways * big >= enough)
-    return launch_tile<T, DIR, 8, 8, 256, LORA>(g, p, s);
+  const bool twice = ways == 4 && g.E > 1 && DIR != kGmmGradWeight;
+  if (height >= 96 && feat >= 96 && (twice ? ways * big > 2 * num_sms : ways * big >= num_sms))
+    return launch_tile<T, DIR, 8, 8, 256, LORA>(g, p, num_sms, s);
   if constexpr (DIR != kGmmGradWeight) {
-    if (g.rows <= 16 * static_cast<int64_t>(g.E)) return launch_tile<T, DIR, 1, 4, 256, LORA>(g, p, s);
+    if (g.rows <= 16 * static_cast<int64_t>(g.E)) return launch_tile<T, DIR, 1, 4, 256, LORA>(g, p, num_sms, s);
   }
-  return launch_tile<T, DIR, 8, 4, 128, LORA>(g, p, s);
+  return launch_tile<T, DIR, 8, 4, 128, LORA>(g, p, num_sms, s);
 }
 
 template <typename T>
-cudaError_t launch_type(const GroupedArgs& g, const LoraTerm* lora, cudaStream_t s) {
-  if (lora != nullptr) return launch_dir<T, kGmmForward, true>(g, lora, s);
-  if (g.dir == kGmmForward) return launch_dir<T, kGmmForward, false>(g, nullptr, s);
-  if (g.dir == kGmmGradInput) return launch_dir<T, kGmmGradInput, false>(g, nullptr, s);
-  return launch_dir<T, kGmmGradWeight, false>(g, nullptr, s);
+cudaError_t launch_type(const GroupedArgs& g, const LoraTerm* lora, int num_sms, cudaStream_t s) {
+  if (lora != nullptr) return launch_dir<T, kGmmForward, true>(g, lora, num_sms, s);
+  if (g.dir == kGmmForward) return launch_dir<T, kGmmForward, false>(g, nullptr, num_sms, s);
+  if (g.dir == kGmmGradInput) return launch_dir<T, kGmmGradInput, false>(g, nullptr, num_sms, s);
+  return launch_dir<T, kGmmGradWeight, false>(g, nullptr, num_sms, s);
 }
 
 }  // namespace
 
-cudaError_t launch_grouped_simt(const GroupedArgs& g, const LoraTerm* lora, cudaStream_t s) {
-  if (g.dtype == kDtF32) return launch_type<float>(g, lora, s);
-  if (g.dtype == kDtF16) return launch_type<__half>(g, lora, s);
-  if (g.dtype == kDtBF16) return launch_type<__nv_bfloat16>(g, lora, s);
+cudaError_t launch_grouped_simt(const GroupedArgs& g, const LoraTerm* lora, int num_sms,
+                                cudaStream_t s) {
+  if (g.dtype == kDtF32) return launch_type<float>(g, lora, num_sms, s);
+  if (g.dtype == kDtF16) return launch_type<__half>(g, lora, num_sms, s);
+  if (g.dtype == kDtBF16) return launch_type<__nv_bfloat16>(g, lora, num_sms, s);
   return cudaErrorInvalidValue;
 }
 
