@@ -88,3 +88,66 @@ def test_overlapped_launches_can_be_turned_off(dev, switch):
     assert done.returncode == 0, done.stderr[-2000:]
     edges, programmatic = (int(w) for w in done.stdout.split()[1::2])
     assert edges >= 10 and (programmatic == 0 if switch == "0" else programmatic >= 8)
+
+
+LOADS = {
+    "all rows in one": [0] * 100 + [700] + [0] * 155,
+    "one row each": [1] * 256,
+    "a few each": [(7 * e) % 10 for e in range(256)],
+    "last only": [0] * 255 + [3],
+    "tiles of each": [90 - e % 5 for e in range(256)],
+}
+
+
+@pytest.mark.parametrize("dtype_name", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("load", sorted(LOADS))
+def test_as_many_experts_as_there_may_be(pkg, orc, dev, dtype_name, load):
+    """256 experts: every group table is full, and the rules that choose a kernel see the mean."""
+    counts, N, K = LOADS[load], 72, 136
+    x, w, dy = make(dev, counts, N, K, dtype_name, seed=13)
+    off, hoff = offsets_of(counts, dev)
+    hx, hw, hdy = as_np(x), as_np(w), as_np(dy)
+    assert_close(pkg.grouped_matmul(x, w, off), *orc.grouped_matmul(hx, hw, hoff), K, dtype_name)
+    assert_close(pkg.grouped_matmul_grad_input(dy, w, off),
+                 *orc.grouped_matmul_grad_input(hdy, hw, hoff), N, dtype_name)
+    assert_close(pkg.grouped_matmul_grad_weight(x, dy, off),
+                 *orc.grouped_matmul_grad_weight(hx, hdy, hoff), max(counts), dtype_name)
+
+
+def test_calls_from_several_threads(pkg, dev):
+    """Threads with a stream each, at once: the bits of a single thread."""
+    import threading
+    import torch
+    x, w, dy = make(dev, [300, 0, 5, 60], 264, 520, "bfloat16", seed=14)
+    off, _ = offsets_of([300, 0, 5, 60], dev)
+    ids = torch.arange(365, dtype=torch.int32, device=dev) % 4 - 1
+    a, b, sc = torch.randn(3, 16, 520, device=dev).bfloat16(), \
+        torch.randn(3, 264, 16, device=dev).bfloat16(), torch.rand(3, device=dev)
+
+    def all4(n):
+        return [pkg.grouped_matmul(x, w, off), pkg.grouped_matmul_grad_input(dy, w, off),
+                pkg.grouped_matmul_grad_weight(x, dy, off),
+                pkg.lora_matmul(x[:n], w[0], a, b, ids[:n], sc)]
+
+    rows = (3, 60, 365, 20)
+    want = [all4(n) for n in rows]
+    torch.cuda.synchronize()
+    got, errors = {}, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream(dev)):
+                for _ in range(20):
+                    out = all4(rows[i])
+                torch.cuda.current_stream().synchronize()
+            got[i] = out
+        except Exception as e:  # noqa: BLE001 -- shown below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(rows))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    assert all(torch.equal(p, q) for i in got for p, q in zip(want[i], got[i])) and len(got) == 4
