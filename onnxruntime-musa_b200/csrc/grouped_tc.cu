@@ -19,10 +19,10 @@
 // CTA stages its 128 of the 256 M entries and half of the N entries of a 64-deep slice
 // (32 KB, six stages); two 256-column accumulators, so the epilogue of a tile overlaps the
 // MMAs of the next.  Bound: the tensor pipe; a slice of the pair is 512 cycles of MMA
-// for 64 KB from L2.  Measured, few calls in a row: 131072 rows by a power law over 64 experts
-// of [768, 2048], bf16, forward 328 us (1.26 PFLOP/s), both gradients 727 us (1.13); 8192 rows
-// over 8 experts of [4096, 14336], fp16, 752 us (1.28); in long loops the power limit takes 15
-// to 20%.
+// for 64 KB from L2.  Measured in a replayed graph of ten calls: 131072 rows by a power law over
+// 64 experts of [768, 2048], bf16, forward 337 us (1.22 PFLOP/s), both gradients 745 us (1.11); 8192
+// rows over 8 experts of [4096, 14336], fp16, 769 us (1.25).  In long loops of calls the power
+// limit takes 15 to 20%: 394, 866 and 892 us.
 //
 // Contractions of more than one segment (kSegment slices: grad_weight of more than 16384 rows of
 // an expert, mostly) are added up in tensor memory: after each segment but the last the epilogue
