@@ -131,13 +131,14 @@ int take_word(int* word) {
 
 struct Call {
   int* error;   // the kernels' word
-  bool traced;  // MOE_B200_TRACE_SYNC: wait for the call and report its own error
+  bool traced;  // MOE_B200_TRACE_SYNC: wait for the call and report its own error (not of a captured
+                // call, which has not run when it returns: its replays report as untraced calls)
   int stall;    // MOE_B200_TEST_STALL: the tensor-core kernels' producers issue no loads
 };
 
 // In front of a call's launches.  An earlier call whose wait ran out has left its output
 // incomplete and nobody has been told: this one reports it and does nothing.
-int begin(const char* what, Call* c) {
+int begin(const char* what, Call* c, cudaStream_t s) {
   int* words = error_words();
   if (words == nullptr)
     return set_error(MOE_B200_EP_FAIL, "%s: no pinned host memory for the error words", what);
@@ -149,7 +150,12 @@ int begin(const char* what, Call* c) {
                      "waiting and its output is incomplete (device error code %d); this call was "
                      "not made", what, err);
   c->stall = env_flag("MOE_B200_TEST_STALL") ? 1 : 0;
-  c->traced = env_flag("MOE_B200_TRACE_SYNC");
+  if (env_flag("MOE_B200_TRACE_SYNC")) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    const int rc = cuda_status(cudaStreamIsCapturing(s, &capture), what);
+    if (rc != MOE_B200_OK) return rc;
+    c->traced = capture == cudaStreamCaptureStatusNone;
+  }
   if (c->traced) {
     static std::atomic<unsigned> turn{0};
     c->error = words + kDevices + turn.fetch_add(1, std::memory_order_relaxed) % kTracedCalls;
@@ -158,13 +164,10 @@ int begin(const char* what, Call* c) {
   return MOE_B200_OK;
 }
 
-// Behind them.  (A captured call has not run yet: there is nothing to wait for.)
+// Behind them.
 int finish(const char* what, const Call& c, cudaStream_t s) {
   if (!c.traced) return MOE_B200_OK;
-  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-  int rc = cuda_status(cudaStreamIsCapturing(s, &capture), what);
-  if (rc != MOE_B200_OK || capture != cudaStreamCaptureStatusNone) return rc;
-  rc = cuda_status(cudaStreamSynchronize(s), what);
+  const int rc = cuda_status(cudaStreamSynchronize(s), what);
   if (rc != MOE_B200_OK) return rc;
   const int err = take_word(c.error);
   return err == 0 ? MOE_B200_OK : set_error(MOE_B200_EP_FAIL, "%s: device error code %d", what, err);
@@ -197,7 +200,7 @@ cudaError_t launch_tc(const moe::GroupedArgs& g, const moe::LoraTerm* lora, cuda
 
 int run_grouped(const char* what, moe::GroupedArgs& g, cudaStream_t s) {
   Call call{};
-  int rc = begin(what, &call);
+  int rc = begin(what, &call, s);
   if (rc != MOE_B200_OK) return rc;
   g.error = call.error;
   g.test_stall = call.stall;
@@ -396,7 +399,7 @@ int moe_b200_lora_matmul(int32_t dtype, int64_t num_rows, int64_t n, int64_t k,
   if (rc != MOE_B200_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   Call call{};
-  rc = begin(kWhat, &call);
+  rc = begin(kWhat, &call, s);
   if (rc != MOE_B200_OK) return rc;
   moe::LoraShrink l{};
   l.dtype = dtype;

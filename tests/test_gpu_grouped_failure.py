@@ -91,3 +91,24 @@ def test_traced_call_may_be_captured(pkg, dev, monkeypatch):
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want) and call() is not None
+
+
+def test_replays_of_a_call_captured_while_traced_report_their_errors(pkg, dev, monkeypatch):
+    """A replay is waited for by nobody, so the next call has to tell."""
+    import torch
+    call = calls(pkg, dev)["streaming"]
+    want = call()
+    monkeypatch.setenv("MOE_B200_TEST_STALL", "1")
+    monkeypatch.setenv("MOE_B200_TRACE_SYNC", "1")
+    g = torch.cuda.CUDAGraph()
+    off = torch.tensor([0, 3], dtype=torch.int32, device=dev)
+    x, w = torch.ones(3, 64, device=dev).half(), torch.ones(1, 64, 64, device=dev).half()
+    with torch.cuda.graph(g):
+        pkg.grouped_matmul(x, w, off)
+    monkeypatch.delenv("MOE_B200_TEST_STALL")
+    monkeypatch.delenv("MOE_B200_TRACE_SYNC")
+    g.replay()
+    torch.cuda.synchronize()
+    with pytest.raises(pkg.EPFail, match="earlier .*device error code"):
+        call()
+    assert torch.equal(call(), want)
