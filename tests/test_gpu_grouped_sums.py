@@ -146,6 +146,45 @@ def test_long_adapter_sums(pkg, dev, dtype_name, T, N, K, r, kind):
     assert_sums(y, exact, dtype_name, SEGMENT + 2.0 ** -15 + (r + 6) * 2.0 ** -23)
 
 
+# 8 x 256 slices of 64 and one more: one CTA of a cluster of eight has a second segment (of one slice);
+# a pair's second segment has 8 entries; an expert of 16383 rows has 255 slices, a step and a tail.
+@pytest.mark.parametrize("dtype_name", ["float16", "bfloat16"])
+@pytest.mark.parametrize("T", [4, 9, 40, 100, 200])
+def test_segments_of_some_ctas(pkg, dev, dtype_name, T):
+    import torch
+    con = 8 * 16384 + 64
+    off = offsets(dev, [T])
+    a, w = positive(dev, (T, con), 2.0 ** -8, dtype_name, 1), positive(dev, (1, 72, con), 1.0, dtype_name, 2)
+    assert_sums(pkg.grouped_matmul(a, w, off), a.double() @ w[0].double().t(), dtype_name)
+    wt = w.transpose(1, 2).contiguous()
+    assert_sums(pkg.grouped_matmul_grad_input(a, wt, off), a.double() @ w[0].double().t(), dtype_name)
+    lora_a = positive(dev, (2, 16, con), 2.0 ** -6, dtype_name, 3)
+    lora_b = positive(dev, (2, 72, 16), 2.0 ** -4, dtype_name, 4)
+    ids = torch.arange(T, dtype=torch.int32, device=dev) % 2
+    y = pkg.lora_matmul(a, w[0], lora_a, lora_b, ids, torch.ones(2, device=dev))
+    exact = a.double() @ w[0].double().t()
+    for i in range(2):
+        exact[i::2] += a[i::2].double() @ lora_a[i].double().t() @ lora_b[i].double().t()
+    assert_sums(y, exact, dtype_name, SEGMENT + 2.0 ** -15 + 22 * 2.0 ** -23)
+
+
+@pytest.mark.parametrize("dtype_name", ["float16", "bfloat16"])
+@pytest.mark.parametrize("con", [16384, 16392])
+def test_pairs_at_the_end_of_a_segment(pkg, dev, dtype_name, con):
+    T, N = 2048, 1800
+    off = offsets(dev, [T])
+    a, w = positive(dev, (T, con), 2.0 ** -8, dtype_name, 1), positive(dev, (1, N, con), 1.0, dtype_name, 2)
+    assert_sums(pkg.grouped_matmul(a, w, off), a.double() @ w[0].double().t(), dtype_name)
+    counts = [16383, 1, 16384, 16385, 32769, 0, 16400]
+    x = positive(dev, (sum(counts), 72), 2.0 ** -8, dtype_name, 3)
+    dy = positive(dev, (sum(counts), 136), 1.0, dtype_name, 4)
+    dw = pkg.grouped_matmul_grad_weight(x, dy, offsets(dev, counts))
+    at = np.cumsum([0] + counts)
+    for e in range(len(counts)):
+        s = slice(at[e], at[e + 1])
+        assert_sums(dw[e], dy[s].double().t() @ x[s].double(), dtype_name)
+
+
 LONG = 1 << 20
 
 
